@@ -42,6 +42,11 @@ typedef bf16x8 frag8;
 
 extern "C" int sm_conv_cout_tile(int cout);
 
+// An empty statement behind the LDS arm's last atomic: without it hipcc sinks the second atomicAdd of the two arms into one on a
+// GENERIC pointer (a flat atomic where an LDS and a global one belong), and with packed f32 off the null test of that pointer
+// does not even encode.
+#define SM_KEEP_LDS_BRANCH() asm volatile("" ::: "memory")
+
 namespace {
 
 struct ConvKArgs {
@@ -909,6 +914,7 @@ __global__ __launch_bounds__(64 * WCO * WPOS * (1 + PROD), (WCO * WPOS == 4) ? 2
                 if (seg < GN_SEG) {
                   atomicAdd(&gn_bins[(seg * (BCO / 8) + (cl >> 3)) * 2 + 0], qs);
                   atomicAdd(&gn_bins[(seg * (BCO / 8) + (cl >> 3)) * 2 + 1], qss);
+                  SM_KEEP_LDS_BRANCH();
                 } else {
                   unsigned long long* st = gnp + (((long long)n_first * a.nlev + lev) * gn_groups + (c0 >> 3)) * 2;
                   atomicAdd(st, qs);
@@ -920,6 +926,7 @@ __global__ __launch_bounds__(64 * WCO * WPOS * (1 + PROD), (WCO * WPOS == 4) ? 2
               if (seg < GN_SEG) {
                 atomicAdd(&gn_bins[(seg * (BCO / 8) + (cl >> 3)) * 2 + 0], gn_fix(gs));
                 atomicAdd(&gn_bins[(seg * (BCO / 8) + (cl >> 3)) * 2 + 1], gn_fix(gss));
+                SM_KEEP_LDS_BRANCH();
               } else {
                 unsigned long long* st = gnp + (((long long)n_img * a.nlev + lev) * gn_groups + (c0 >> 3)) * 2;
                 atomicAdd(st, gn_fix(gs));
@@ -1025,6 +1032,7 @@ __global__ __launch_bounds__(64 * WCO * WPOS * (1 + PROD), (WCO * WPOS == 4) ? 2
       if (seg < GN_SEG) {
         atomicAdd(&gn_bins[(seg * (BCO / 8) + ec) * 2 + 0], gn_s);
         atomicAdd(&gn_bins[(seg * (BCO / 8) + ec) * 2 + 1], gn_ss);
+        SM_KEEP_LDS_BRANCH();
       } else {
         unsigned long long* st = gnp + (((long long)gn_n * a.nlev + lev) * gn_groups + (c0 >> 3)) * 2;
         atomicAdd(st, gn_s);
