@@ -764,6 +764,77 @@ int sm_track_clip(const float* det_feats, const float* det, const int64_t* det_l
                   float coeff_label, float* mem_feats, float* mem_boxes, int64_t* mem_labels, int32_t* mem_count,
                   int capacity, float* comp_ws, int32_t* ids, sm_stream_t stream);
 
+/* ---------------------------------------------------------------- rows of bf16 / f16 / f32 values: GroupNorm + activation, dropout */
+typedef enum { SM_DT_BF16 = 0, SM_DT_F16 = 1, SM_DT_F32 = 2 } sm_dtype;
+typedef enum { SM_ACT_NONE = 0, SM_ACT_RELU = 1, SM_ACT_SILU = 2, SM_ACT_GELU = 3 } sm_activation; /* GELU: t * Phi(t) */
+
+/* Dropout of every entry point below: element i of the call (row-major over rows x channels, row strides not counted) takes 16-bit
+ * lane i % 8 of the Philox-4x32-10 block with counter (i / 8, offset [+ *offset_dev]) and key seed, and is kept iff
+ * lane >= drop_threshold (0 = keep all .. 65536 = drop all); kept values are multiplied by 65536 / (65536 - drop_threshold).
+ * offset_dev (device, may be NULL) is read by the kernels: a captured graph draws new masks when it changes between replays. */
+
+/* GroupNorm + activation (+ dropout) on channels-last pyramid rows; level l holds batch * hw[l] rows from row0[l], image-major.
+ * Any channels % groups == 0; row strides are in elements (>= channels); 16-byte accesses are taken when channels % 8 == 0 and every
+ * pointer and stride is 16-byte aligned.  Levels of 0 rows and batch 0 are allowed. */
+typedef struct {
+  int32_t nlev, batch, channels, groups;
+  int32_t dtype, act; /* sm_dtype of x, y, dy, dx; sm_activation */
+  float eps;
+  int32_t drop_threshold;
+  int64_t hw[SM_MAX_LEVELS], row0[SM_MAX_LEVELS];
+  int64_t x_stride, y_stride, dy_stride, dx_stride;
+  uint64_t drop_seed, drop_offset;
+  const int64_t* drop_offset_dev;
+} sm_gn_act_desc;
+
+/* y = act(GroupNorm(x) * gamma + beta) [dropped out]; gamma / beta f32 [channels] or NULL (1 / 0).  stats (may be NULL when no
+ * backward follows): f64 [batch][nlev][groups][2] = (mean, 1 / sqrt(var + eps)).  workspace: sm_group_norm_act_workspace(d, 0) bytes,
+ * 16-byte aligned, contents irrelevant; y may be x.  No atomics: bit-reproducible. */
+int64_t sm_group_norm_act_workspace(const sm_gn_act_desc* d, int backward);
+int sm_group_norm_act(const sm_gn_act_desc* d, const void* x, const float* gamma, const float* beta, void* y, double* stats,
+                      void* workspace, int64_t workspace_bytes, sm_stream_t stream);
+/* dx (may be NULL), dgamma / dbeta f32 [channels] (may be NULL), written whole; x, gamma, beta, stats and the dropout arguments are
+ * the forward's.  workspace: sm_group_norm_act_workspace(d, 1).  dx may be dy. */
+int sm_group_norm_act_bwd(const sm_gn_act_desc* d, const void* x, const void* dy, const float* gamma, const float* beta,
+                          const double* stats, void* dx, float* dgamma, float* dbeta, void* workspace, int64_t workspace_bytes,
+                          sm_stream_t stream);
+
+/* y = dropout(x) [+ residual] on rows x cols values with row strides in elements; the backward of x is the same call on dy without
+ * a residual.  y may be x or residual. */
+int sm_dropout(int dtype, const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int64_t x_stride,
+               int64_t res_stride, int64_t y_stride, int drop_threshold, uint64_t seed, uint64_t offset,
+               const int64_t* offset_dev, sm_stream_t stream);
+
+/* ---------------------------------------------------------------- 8-bit (e4m3) products, one power-of-two scale per block of 128
+ * A quantised matrix of rows x cols: codes (OCP e4m3) uint8 [rows][sm_fp8_cols_padded(cols)], 16-byte aligned, zero codes behind the
+ * last column; scales (E8M0: 2^(byte - 127)) uint8 [rows / block_rows rounded up][sm_fp8_scale_cols(cols)], 4-byte aligned, one per
+ * block of block_rows x 128, 127 behind the last block.  scale = smallest power of two >= 2^-127 with max |x| / scale <= 448 (1 for a
+ * block of zeros), code = x / scale rounded to nearest even; Inf and NaN become the NaN code and leave the block's scale alone. */
+int64_t sm_fp8_cols_padded(int64_t cols); /* up to a multiple of 128 */
+int64_t sm_fp8_scale_cols(int64_t cols);  /* blocks of 128, up to a multiple of 4 */
+/* x [rows][cols] (row stride x_stride) -> q / scale; block_rows 1 or 128; transpose: q is the transpose (cols x rows, blocks along
+ * the rows of x) -- with block_rows 128 the same codes and scales, transposed. */
+int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, int transpose, void* q,
+                    void* scale, sm_stream_t stream);
+
+/* y [m][n] = a [m][k] . b [n][k]^T [+ bias f32 [n]] [+ residual [m][n]] [ReLU], f32 accumulation, one rounding to out_dtype
+ * (sm_dtype; also the residual's).  workspace: sm_fp8_matmul_workspace(d) bytes, 16-byte aligned.  residual may be y. */
+typedef struct {
+  int64_t m;
+  int32_t n, k;
+  int32_t a_block_rows, b_block_rows; /* 1 or 128 */
+  int32_t out_dtype, relu;
+  int64_t y_stride, res_stride; /* elements */
+} sm_fp8_matmul_desc;
+int64_t sm_fp8_matmul_workspace(const sm_fp8_matmul_desc* d);
+int sm_fp8_matmul(const sm_fp8_matmul_desc* d, const void* a, const void* a_scale, const void* b, const void* b_scale,
+                  const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, sm_stream_t stream);
+
+/* out f32 [cols] = column sums of x [rows][cols] (row stride x_stride); deterministic */
+int64_t sm_col_sum_workspace(int64_t rows, int cols);
+int sm_col_sum(int dtype, const void* x, int64_t rows, int cols, int64_t x_stride, float* out, void* workspace,
+               int64_t workspace_bytes, sm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

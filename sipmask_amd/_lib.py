@@ -4,6 +4,7 @@ The product path has NO fallback: if the shared library is missing or a call
 returns a non-zero status a RuntimeError is raised.  Build with
 ``python -c "import __graft_entry__ as g; g.build()"`` or ``make -C sipmask_amd/csrc``.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -80,6 +81,25 @@ class DetDesc(C.Structure):
         ("img_h", C.c_int32), ("img_w", C.c_int32), ("kmax", C.c_int32),
         ("scale_factor", C.c_float * 4), ("rescale", C.c_int32), ("reg_prescaled", C.c_int32),
         ("per_image", C.c_void_p),
+    ]
+
+
+class GnActDesc(C.Structure):
+    """sm_gn_act_desc"""
+    _fields_ = [
+        ("nlev", C.c_int32), ("batch", C.c_int32), ("channels", C.c_int32), ("groups", C.c_int32),
+        ("dtype", C.c_int32), ("act", C.c_int32), ("eps", C.c_float), ("drop_threshold", C.c_int32),
+        ("hw", _i64x5), ("row0", _i64x5),
+        ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("dy_stride", C.c_int64), ("dx_stride", C.c_int64),
+        ("drop_seed", C.c_uint64), ("drop_offset", C.c_uint64), ("drop_offset_dev", C.c_void_p),
+    ]
+
+
+class Fp8MatmulDesc(C.Structure):
+    """sm_fp8_matmul_desc"""
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("a_block_rows", C.c_int32), ("b_block_rows", C.c_int32),
+        ("out_dtype", C.c_int32), ("relu", C.c_int32), ("y_stride", C.c_int64), ("res_stride", C.c_int64),
     ]
 
 
@@ -188,6 +208,18 @@ PROTOTYPES = {
     "sm_crop_split_gt_fwd": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "sm_sigmoid_focal_loss_fwd": (_I, [_P, _P, _P, _I, _I, _F, _F, _P]),
     "sm_sigmoid_focal_loss_bwd": (_I, [_P, _P, _P, _P, _I, _I, _F, _F, _P]),
+    "sm_group_norm_act_workspace": (C.c_int64, [C.POINTER(GnActDesc), _I]),
+    "sm_group_norm_act": (_I, [C.POINTER(GnActDesc), _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_group_norm_act_bwd": (_I, [C.POINTER(GnActDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_dropout": (_I, [_I, _P, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _I, C.c_uint64, C.c_uint64, _P,
+                        _P]),
+    "sm_fp8_cols_padded": (C.c_int64, [C.c_int64]),
+    "sm_fp8_scale_cols": (C.c_int64, [C.c_int64]),
+    "sm_fp8_quantize": (_I, [_I, _P, C.c_int64, C.c_int64, C.c_int64, _I, _I, _P, _P, _P]),
+    "sm_fp8_matmul_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
+    "sm_fp8_matmul": (_I, [C.POINTER(Fp8MatmulDesc), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_col_sum_workspace": (C.c_int64, [C.c_int64, _I]),
+    "sm_col_sum": (_I, [_I, _P, C.c_int64, _I, C.c_int64, _P, _P, C.c_int64, _P]),
 }
 
 _lib = None
@@ -227,6 +259,13 @@ def ptr(t):
 
 def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on_device(t):
+    """context in which `t`'s device is the current one (launches, workspaces and stream_ptr() follow the current device)"""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def require_cuda(*tensors):

@@ -1411,3 +1411,145 @@ def scatter_stride_rows(t, batch, hw, out_hw, stride, c):
     _lib.check(lib.sm_scatter_stride_rows(_lib.ptr(t), batch, hw[0], hw[1], out_hw[0], out_hw[1], stride, c, _lib.ptr(out),
                                           _lib.stream_ptr()), "sm_scatter_stride_rows")
     return out
+
+
+# ------------------------------------------------------------------------------- rows of bf16 / f16 / f32: GroupNorm + activation, dropout
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}      # sm_dtype
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}         # sm_activation
+_MASK64 = (1 << 64) - 1
+
+
+def dtype_code(t, what):
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError("%s: bfloat16, float16 or float32, got %s" % (what, t.dtype))
+    return code
+
+
+def row_stride(t):
+    """elements between the rows of a 2-D tensor whose rows are dense (1 row: its width)"""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def dense_rows(t, cols):
+    """`t` [..., cols] as a 2-D tensor with dense, non-overlapping rows (copied only where its strides do not allow the view)"""
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= s
+    if cols > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    try:
+        r = t.view(rows, cols)
+    except RuntimeError:
+        r = t.contiguous().view(rows, cols)
+    if r.shape[0] > 1 and (r.stride(0) < cols or (cols == 1 and r.stride(0) < 1)):
+        r = r.contiguous()
+    return r
+
+
+def dropout_threshold(p):
+    """p -> round(65536 p): an element is dropped when its 16-bit draw is below"""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(p))
+    return int(round(p * 65536))
+
+
+def dropout_offset(offset, device):
+    """(host part, device tensor or None) of an offset given as an int or as a one-element int64 tensor on `device`"""
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() != 1 or offset.device != device:
+            raise ValueError("dropout offset: an int or a one-element int64 tensor on %s" % (device,))
+        return 0, offset
+    return int(offset) & _MASK64, None
+
+
+def group_norm_act_desc(x, lv, groups, eps, act, thr, seed, offset):
+    """sm_gn_act_desc of rows x [lv.rows, C]; y, dy and dx are dense rows unless the caller sets their strides"""
+    d = _lib.GnActDesc()
+    c = x.shape[1]
+    d.nlev, d.batch, d.channels, d.groups = len(lv), lv.batch, c, groups
+    d.dtype, d.act, d.eps, d.drop_threshold = dtype_code(x, "group_norm_act"), act, eps, thr
+    for l, (h, w) in enumerate(lv.sizes):
+        d.hw[l], d.row0[l] = h * w, lv.row0[l]
+    d.x_stride, d.y_stride, d.dy_stride, d.dx_stride = row_stride(x), c, c, c
+    host, dev = offset
+    d.drop_seed, d.drop_offset = int(seed) & _MASK64, host
+    d.drop_offset_dev = None if dev is None else dev.data_ptr()
+    return d
+
+
+def _workspace(need, device, what):
+    if need < 0:
+        _lib.check(int(need), what)
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def group_norm_act(d, x, gamma, beta, want_stats):
+    """-> (y dense rows, stats f64 [batch * nlev * groups, 2] or None)"""
+    lib = _lib.load()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(d.batch * d.nlev * d.groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
+    ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 0), x.device, "sm_group_norm_act")
+    _lib.check(lib.sm_group_norm_act(C.byref(d), _lib.ptr(x), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(y), _lib.ptr(stats),
+                                     _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_group_norm_act")
+    return y, stats
+
+
+def group_norm_act_bwd(d, x, dy, gamma, beta, stats, need_dx=True, dgamma=None, dbeta=None):
+    """-> dx dense rows or None; dgamma / dbeta f32 [C] buffers are written when given"""
+    lib = _lib.load()
+    d.dy_stride = row_stride(dy)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 1), x.device, "sm_group_norm_act_bwd")
+    _lib.check(lib.sm_group_norm_act_bwd(C.byref(d), _lib.ptr(x), _lib.ptr(dy), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(stats),
+                                         _lib.ptr(dx), _lib.ptr(dgamma), _lib.ptr(dbeta), _lib.ptr(ws), ws.numel(),
+                                         _lib.stream_ptr()), "sm_group_norm_act_bwd")
+    return dx
+
+
+def dropout_rows(x, residual, thr, seed, offset):
+    """x (and residual) [rows, cols] with dense rows -> dense rows"""
+    lib = _lib.load()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    host, dev = offset
+    _lib.check(lib.sm_dropout(dtype_code(x, "dropout"), _lib.ptr(x), _lib.ptr(residual), _lib.ptr(y), x.shape[0], x.shape[1],
+                              row_stride(x), 0 if residual is None else row_stride(residual), x.shape[1], thr,
+                              int(seed) & _MASK64, host, _lib.ptr(dev), _lib.stream_ptr()), "sm_dropout")
+    return y
+
+
+# ------------------------------------------------------------------------------- 8-bit products
+def fp8_quantize(x, block_rows, transpose):
+    """x [rows, cols] with dense rows -> (codes [r, cols_padded(c)] e4m3, scales uint8 [ceil(r / block_rows), scale_cols(c)]) of
+    (r, c) = (rows, cols), or (cols, rows) with transpose"""
+    lib = _lib.load()
+    r, c = (x.shape[1], x.shape[0]) if transpose else (x.shape[0], x.shape[1])
+    q = torch.empty(r, int(lib.sm_fp8_cols_padded(c)), dtype=torch.float8_e4m3fn, device=x.device)
+    s = torch.empty(-(-r // block_rows), int(lib.sm_fp8_scale_cols(c)), dtype=torch.uint8, device=x.device)
+    _lib.check(lib.sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _lib.ptr(x), x.shape[0], x.shape[1], row_stride(x), block_rows,
+                                   int(transpose), _lib.ptr(q), _lib.ptr(s), _lib.stream_ptr()), "sm_fp8_quantize")
+    return q, s
+
+
+def fp8_matmul(a, sa, a_block_rows, b, sb, b_block_rows, k, bias, residual, relu, out_dtype):
+    lib = _lib.load()
+    d = _lib.Fp8MatmulDesc()
+    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows = a.shape[0], b.shape[0], k, a_block_rows, b_block_rows
+    d.out_dtype, d.relu, d.y_stride = DTYPE_CODES[out_dtype], int(relu), b.shape[0]
+    d.res_stride = 0 if residual is None else row_stride(residual)
+    y = torch.empty(a.shape[0], b.shape[0], dtype=out_dtype, device=a.device)
+    ws = _workspace(lib.sm_fp8_matmul_workspace(C.byref(d)), a.device, "sm_fp8_matmul")
+    _lib.check(lib.sm_fp8_matmul(C.byref(d), _lib.ptr(a), _lib.ptr(sa), _lib.ptr(b), _lib.ptr(sb), _lib.ptr(bias),
+                                 _lib.ptr(residual), _lib.ptr(y), _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_fp8_matmul")
+    return y
+
+
+def col_sum(x):
+    """f32 column sums of x [rows, cols] with dense rows"""
+    lib = _lib.load()
+    out = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+    ws = _workspace(lib.sm_col_sum_workspace(x.shape[0], x.shape[1]), x.device, "sm_col_sum")
+    _lib.check(lib.sm_col_sum(dtype_code(x, "col_sum"), _lib.ptr(x), x.shape[0], x.shape[1], row_stride(x), _lib.ptr(out),
+                              _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_col_sum")
+    return out

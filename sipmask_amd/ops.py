@@ -9,6 +9,9 @@ for the SipMask hot path -- same names, argument meaning and error behaviour, HI
   multiclass_nms_idx            M/mmdet/core/post_processing/bbox_nms.py:79-146
   Scale                         M/mmdet/ops/scale.py:5-15
 
+and, beyond the reference, the layers of residual blocks on channels-last rows: group_norm_act (GroupNorm + activation + dropout),
+dropout (counter-based, no stored mask), quantize_fp8 / matmul_fp8 / linear_fp8 (e4m3 with a power-of-two scale per block of 128).
+
 There is no CPU implementation (as in the reference): CPU tensors raise
 NotImplementedError, a missing libsipmask_hip.so raises RuntimeError.
 """
@@ -290,6 +293,270 @@ class GroupNormFunction(Function):
 
 
 group_norm = GroupNormFunction.apply
+
+
+# ------------------------------------------------------------------------------- GroupNorm + activation, dropout
+class GroupNormActFunction(Function):
+    """act(GroupNorm(x)) [dropped out] of rows x [lv.rows, C] (sm_group_norm_act / _bwd).  The backward recomputes the normalised
+    values and the dropout mask; only x, the parameters and (mean, rstd) per (image, level, group) are kept."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, lv, groups, eps, act, thr, seed, offset, sink):
+        g32 = None if gamma is None else gamma.detach().float().contiguous()
+        b32 = None if beta is None else beta.detach().float().contiguous()
+        host, dev = H.dropout_offset(offset, x.device)
+        with _lib.on_device(x):
+            d = H.group_norm_act_desc(x, lv, groups, eps, act, thr, seed, (host, dev))
+            y, stats = H.group_norm_act(d, x, g32, b32, any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, g32, b32, stats, dev)      # (dev: an offset that changed before the backward is an error)
+        ctx.cfg = (lv, groups, eps, act, thr, seed, host, sink, None if gamma is None else gamma.dtype,
+                   None if beta is None else beta.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, g32, b32, stats, dev = ctx.saved_tensors
+        lv, groups, eps, act, thr, seed, host, sink, gdt, bdt = ctx.cfg
+        need_x, need_g, need_b = ctx.needs_input_grad[:3]
+        dy = H.dense_rows(dy, x.shape[1])
+        tg = H.GRAD_SINK.target(g32) if sink and need_g else None
+        tb = H.GRAD_SINK.target(b32) if sink and need_b else None
+        if (need_g and tg is None) or (need_b and tb is None):
+            tg = tb = None
+        new = lambda: torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+        dg = None if not need_g else (tg if tg is not None else new())
+        db = None if not need_b else (tb if tb is not None else new())
+        with _lib.on_device(x):
+            d = H.group_norm_act_desc(x, lv, groups, eps, act, thr, seed, (host, dev))
+            dx = H.group_norm_act_bwd(d, x, dy, g32, b32, stats, need_x, dg, db)
+        if tg is not None:
+            H.GRAD_SINK.commit(g32)
+            dg = None
+        if tb is not None:
+            H.GRAD_SINK.commit(b32)
+            db = None
+        return (dx, None if dg is None else dg.to(gdt), None if db is None else db.to(bdt)) + (None,) * 8
+
+
+def _gn_act_args(x, channels, weight, bias, groups, eps, activation, dropout_p, what):
+    """shared checks; -> (sm_activation, dropout threshold)"""
+    _lib.require_cuda(x, weight, bias)
+    H.dtype_code(x, what)
+    if activation not in H.ACTIVATIONS:
+        raise ValueError("%s: activation %r (one of %s)" % (what, activation, sorted(k for k in H.ACTIVATIONS if k)))
+    if groups < 1 or channels < 1 or channels % groups != 0:
+        raise ValueError("%s: %d channels in %d groups" % (what, channels, groups))
+    if not eps >= 0:
+        raise ValueError("%s: eps %r" % (what, eps))
+    for t in (weight, bias):
+        if t is not None and (t.shape != (channels,) or t.device != x.device or not t.is_floating_point()):
+            raise ValueError("%s: weight and bias are [%d] on %s" % (what, channels, x.device))
+    return H.ACTIVATIONS[activation], H.dropout_threshold(dropout_p)
+
+
+def group_norm_act(x, weight, bias, num_groups, eps=1e-5, activation="relu", dropout_p=0.0, seed=0, offset=0):
+    """act(F.group_norm(x, num_groups, weight, bias, eps)) on channels-last memory, optionally dropped out; differentiable in
+    x, weight and bias.
+
+    x [N, C, *] bf16 / f16 / f32 (channels_last memory, or a channel slice of it, is read in place; other layouts are copied
+    first); weight / bias [C] or None; activation "none", "relu", "silu" or "gelu" (t Phi(t)).  Returns x's type, channels-last.
+    dropout_p > 0: the mask is that of `dropout` with the channel as the fastest axis.  Statistics in f64, one rounding at the
+    end; results do not depend on scheduling."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 2:
+        raise ValueError("group_norm_act: x is [N, C, *]")
+    c = x.shape[1]
+    act, thr = _gn_act_args(x, c, weight, bias, num_groups, eps, activation, dropout_p, "group_norm_act")
+    last = x.movedim(1, -1)
+    hw = 1
+    for s in x.shape[2:]:
+        hw *= s
+    y = GroupNormActFunction.apply(H.dense_rows(last, c), weight, bias, H.Levels(x.shape[0], [(hw, 1)]), num_groups, eps, act, thr,
+                                   seed, offset, False)
+    return y.view(last.shape).movedim(-1, 1)
+
+
+class DropoutFunction(Function):
+    """x [rows, cols] with dense rows -> keep * x / (1 - p) [+ residual] (sm_dropout)"""
+
+    @staticmethod
+    def forward(ctx, x, residual, thr, seed, offset):
+        host, dev = H.dropout_offset(offset, x.device)
+        with _lib.on_device(x):
+            y = H.dropout_rows(x, residual, thr, seed, (host, dev))
+        ctx.save_for_backward(dev)
+        ctx.cfg = (thr, seed, host)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (dev,) = ctx.saved_tensors
+        thr, seed, host = ctx.cfg
+        dx = None
+        if ctx.needs_input_grad[0]:
+            g = H.dense_rows(dy, dy.shape[1])
+            with _lib.on_device(g):
+                dx = H.dropout_rows(g, None, thr, seed, (host, dev))
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x, p, seed, offset=0, residual=None, training=True):
+    """Inverted dropout with a counter-based generator: the mask is a function of (seed, offset, element index) and is neither
+    stored nor drawn from a global state, so the backward regenerates it and a step can be repeated exactly.
+
+    x of any shape, bf16 / f16 / f32; elements are numbered in row-major order of the shape (strides do not matter).  p in [0, 1]
+    is rounded to a multiple of 2^-16 and kept values are scaled by the reciprocal of that; dropped ones become 0 whatever they
+    were.  seed: any 64-bit int.  offset: a 64-bit int, or a one-element int64 tensor on x's device that the kernels read (advance it
+    between replays of a captured graph; it has to keep its value until the backward has run).  Use a different (seed, offset) for
+    every call.  residual: same shape and type, added to the result.  training=False: x (+ residual)."""
+    _lib.require_cuda(x, residual)
+    H.dtype_code(x, "dropout")
+    thr = H.dropout_threshold(p)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("dropout: residual %s %s for x %s %s" % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
+    if not training:
+        if residual is None:
+            return x
+        thr = 0
+    H.dropout_offset(offset, x.device)
+    cols = x.shape[-1] if x.dim() else 1
+    flat = x.is_contiguous() and (residual is None or residual.is_contiguous())
+    rows = lambda t: None if t is None else (t.reshape(1, -1) if flat else H.dense_rows(t, cols))
+    return DropoutFunction.apply(rows(x), rows(residual), thr, seed, offset).view(x.shape)
+
+
+# ------------------------------------------------------------------------------- 8-bit products
+class Fp8Blocks:
+    """A matrix [rows, cols] in e4m3 with one power-of-two scale per block of block_rows x 128 (include/sipmask_hip.h has the
+    layout): `codes` float8_e4m3fn [rows, cols padded to 128], `scales` uint8 (2^(byte - 127))."""
+    __slots__ = ("codes", "scales", "rows", "cols", "block_rows")
+
+    def __init__(self, codes, scales, rows, cols, block_rows):
+        self.codes, self.scales, self.rows, self.cols, self.block_rows = codes, scales, rows, cols, block_rows
+
+    @property
+    def shape(self):
+        return (self.rows, self.cols)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.float32):
+        """the values the codes stand for (for checks and for code without an 8-bit product)"""
+        nkb = -(-self.cols // 128)
+        s = ((self.scales[:, :nkb].to(torch.int64) + (1023 - 127)) << 52).view(torch.float64)
+        s = s.repeat_interleave(self.block_rows, 0)[:self.rows].repeat_interleave(128, 1)[:, :self.cols]
+        return (self.codes[:, :self.cols].to(torch.float64) * s).to(dtype)
+
+
+def quantize_fp8(x, block_rows=1, transpose=False):
+    """x [rows, cols] bf16 / f16 / f32 -> Fp8Blocks.  block_rows 1: a scale per row and 128 columns (activations, gradients);
+    128: per 128 x 128 (weights).  transpose: the transposed matrix, blocks along the rows of x.  Inf and NaN are stored as NaN.
+    Not differentiable (linear_fp8 is)."""
+    _lib.require_cuda(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError("quantize_fp8: x is [rows, cols >= 1], got %s" % (tuple(x.shape),))
+    H.dtype_code(x, "quantize_fp8")
+    if block_rows not in (1, 128):
+        raise ValueError("quantize_fp8: block_rows is 1 or 128")
+    if transpose and x.shape[0] == 0:
+        raise ValueError("quantize_fp8: the transpose of 0 rows has no columns")
+    x = H.dense_rows(x.detach(), x.shape[1])
+    with _lib.on_device(x):
+        q, s = H.fp8_quantize(x, block_rows, transpose)
+    r, c = (x.shape[1], x.shape[0]) if transpose else x.shape
+    return Fp8Blocks(q, s, r, c, block_rows)
+
+
+def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloat16):
+    """a [m, k] . b [n, k]^T (+ bias [n]) (+ residual [m, n] of out_dtype) (ReLU) of two Fp8Blocks: exact products, f32
+    accumulation, one rounding to out_dtype (bf16 / f16 / f32).  Not differentiable (linear_fp8 is)."""
+    if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
+        raise TypeError("matmul_fp8: operands come from quantize_fp8")
+    _lib.require_cuda(a.codes, b.codes, bias, residual)
+    if a.cols != b.cols or a.device != b.device:
+        raise ValueError("matmul_fp8: a %s on %s, b %s on %s" % (a.shape, a.device, b.shape, b.device))
+    if b.rows < 1:
+        raise ValueError("matmul_fp8: b has no rows")
+    if out_dtype not in H.DTYPE_CODES:
+        raise TypeError("matmul_fp8: out_dtype bfloat16, float16 or float32, got %s" % out_dtype)
+    if bias is not None:
+        if bias.shape != (b.rows,) or bias.device != a.device:
+            raise ValueError("matmul_fp8: bias is [%d] on %s" % (b.rows, a.device))
+        bias = bias.detach().float().contiguous()
+    if residual is not None:
+        if residual.shape != (a.rows, b.rows) or residual.dtype != out_dtype or residual.device != a.device:
+            raise ValueError("matmul_fp8: residual is %s %s" % ((a.rows, b.rows), out_dtype))
+        residual = H.dense_rows(residual.detach(), b.rows)
+    with _lib.on_device(a.codes):
+        return H.fp8_matmul(a.codes, a.scales, a.block_rows, b.codes, b.scales, b.block_rows, a.cols, bias, residual, relu, out_dtype)
+
+
+class LinearFp8Function(Function):
+    """y = q(x) q(w)^T + bias (ReLU);  dx = q(dy) q(w);  dw = q(dy^T) q(x^T)^T;  dbias = column sums of dy"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, relu, weight_q):
+        w = None if weight is None else weight.detach().reshape(weight.shape[0], -1)
+        wq = weight_q if weight_q is not None else quantize_fp8(w, 128)
+        y = matmul_fp8(quantize_fp8(x), wq, bias, relu, None, x.dtype)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, y if relu else None)
+        ctx.cfg = (relu, None if bias is None else bias.dtype, x.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, y = ctx.saved_tensors
+        relu, bdt, dt = ctx.cfg
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if relu:
+            dy = torch.where(y > 0, dy, torch.zeros((), dtype=dy.dtype, device=dy.device))
+        dy = H.dense_rows(dy, dy.shape[1])
+        dx = dw = db = None
+        if need_x:
+            wt = quantize_fp8(weight.detach().reshape(weight.shape[0], -1), 128, transpose=True)
+            dx = matmul_fp8(quantize_fp8(dy), wt, out_dtype=dt)
+        if need_w:
+            if dy.shape[0] == 0:
+                dw = torch.zeros_like(weight)
+            else:
+                dw = matmul_fp8(quantize_fp8(dy, transpose=True), quantize_fp8(x, transpose=True), out_dtype=torch.float32)
+                dw = dw.view(weight.shape).to(weight.dtype)
+        if need_b:
+            with _lib.on_device(dy):
+                db = H.col_sum(dy).to(bdt)
+        return dx, dw, db, None, None
+
+
+def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
+    """x [..., k] . weight [n, k]^T (+ bias) (ReLU) with both operands quantised to e4m3 blocks (1 x 128 for x, 128 x 128 for the
+    weight), f32 accumulation, result of x's type (bf16 / f16 / f32): the 8-bit form of a 1x1 conv_rows; a [n, k, 1, 1] conv weight is
+    taken as it is.  Differentiable in x, weight and bias: the gradients' products are 8-bit as well (dy in 1 x 128 blocks along the
+    axis each product sums over), dbias is exact.
+
+    Serving: weight_q = quantize_fp8(weight, block_rows=128), laid out once, with weight=None when x needs no gradient."""
+    _lib.require_cuda(x, weight, bias)
+    H.dtype_code(x, "linear_fp8")
+    if weight is None and weight_q is None:
+        raise ValueError("linear_fp8: weight or weight_q")
+    if weight is not None:
+        if weight.dim() not in (2, 4) or (weight.dim() == 4 and tuple(weight.shape[2:]) != (1, 1)) or weight.device != x.device:
+            raise ValueError("linear_fp8: weight is [n, k] or [n, k, 1, 1] on %s, got %s" % (x.device, tuple(weight.shape)))
+        H.dtype_code(weight, "linear_fp8 weight")
+    n, k = weight.shape[:2] if weight is not None else weight_q.shape
+    if weight_q is not None and (not isinstance(weight_q, Fp8Blocks) or weight_q.shape != (n, k) or weight_q.block_rows != 128):
+        raise ValueError("linear_fp8: weight_q is quantize_fp8(weight, block_rows=128) of [%d, %d]" % (n, k))
+    if x.dim() < 1 or x.shape[-1] != k or n < 1 or k < 1:
+        raise ValueError("linear_fp8: x %s for a weight of [%d, %d]" % (tuple(x.shape), n, k))
+    if bias is not None and (bias.shape != (n,) or bias.device != x.device):
+        raise ValueError("linear_fp8: bias is [%d] on %s" % (n, x.device))
+    if weight is None and torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("linear_fp8: a gradient of x needs the weight itself, not weight_q alone")
+    y = LinearFp8Function.apply(H.dense_rows(x, k), weight, bias, relu, weight_q)
+    return y.view(x.shape[:-1] + (n,))
 
 
 class UpsampleBilinearFunction(Function):

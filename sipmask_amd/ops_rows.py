@@ -12,6 +12,7 @@ into the conv launches:
                     residual, + ReLU), multi-level; backward = ReLU gate, dX as a conv with the flipped weights (bf16 rows
                     out), dW through sm_conv2d_bwd, both operand layouts produced by one sm_weight_prep launch each
   gn_rows           GroupNorm (+ReLU) over pyramid rows, statistics per (image, level, group)
+  gn_act_rows       GroupNorm + activation + dropout over pyramid rows of any float type and channel count
   deform_conv_rows  FeatureAlign's deformable conv over the whole pyramid
   mask_feat_rows    the [l0 | up2(l1) | up4(l2)] concatenation the mask branch reads (sipmask_head.py:266-275)
 
@@ -215,6 +216,19 @@ class GroupNormRowsFunction(Function):
 
 def gn_rows(x, lv, gamma, beta, groups=32, eps=1e-5, relu=True):
     return GroupNormRowsFunction.apply(x, gamma, beta, lv, groups, eps, relu)
+
+
+def gn_act_rows(x, lv, gamma, beta, groups=32, eps=1e-5, activation="relu", dropout_p=0.0, seed=0, offset=0):
+    """ops.group_norm_act on pyramid rows: x [lv.rows, C] bf16 / f16 / f32 (dense rows, any row stride), statistics per (image,
+    level, group), any C % groups == 0, activation "none" / "relu" / "silu" / "gelu", then dropout (elements numbered over rows x
+    C).  Unlike gn_rows its parameter gradients do not depend on the order in which blocks finish."""
+    from . import ops as P
+    if x.dim() != 2 or x.shape[0] != lv.rows:
+        raise ValueError("gn_act_rows: x %s for a pyramid of %d rows" % (tuple(x.shape), lv.rows))
+    if len(lv) > _lib.SM_MAX_LEVELS:
+        raise ValueError("gn_act_rows: at most %d levels" % _lib.SM_MAX_LEVELS)
+    act, thr = P._gn_act_args(x, x.shape[1], gamma, beta, groups, eps, activation, dropout_p, "gn_act_rows")
+    return P.GroupNormActFunction.apply(H.dense_rows(x, x.shape[1]), gamma, beta, lv, groups, eps, act, thr, seed, offset, True)
 
 
 class DeformConvRowsFunction(Function):
