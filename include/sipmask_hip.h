@@ -806,16 +806,21 @@ int sm_dropout(int dtype, const void* x, const void* residual, void* y, int64_t 
                const int64_t* offset_dev, sm_stream_t stream);
 
 /* ---------------------------------------------------------------- 8-bit (e4m3) products, one power-of-two scale per block of 128
- * A quantised matrix of rows x cols: codes (OCP e4m3) uint8 [rows][sm_fp8_cols_padded(cols)], 16-byte aligned, zero codes behind the
- * last column; scales (E8M0: 2^(byte - 127)) uint8 [rows / block_rows rounded up][sm_fp8_scale_cols(cols)], 4-byte aligned, one per
- * block of block_rows x 128, 127 behind the last block.  scale = smallest power of two >= 2^-127 with max |x| / scale <= 448 (1 for a
- * block of zeros), code = x / scale rounded to nearest even; Inf and NaN become the NaN code and leave the block's scale alone. */
-int64_t sm_fp8_cols_padded(int64_t cols); /* up to a multiple of 128 */
-int64_t sm_fp8_scale_cols(int64_t cols);  /* blocks of 128, up to a multiple of 4 */
-/* x [rows][cols] (row stride x_stride) -> q / scale; block_rows 1 or 128; transpose: q is the transpose (cols x rows, blocks along
- * the rows of x) -- with block_rows 128 the same codes and scales, transposed. */
-int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, int transpose, void* q,
-                    void* scale, sm_stream_t stream);
+ * A quantised matrix of rows x cols: codes (OCP e4m3) uint8 [ceil(cols / 128)][rows][128], 16-byte aligned, zero codes behind the last
+ * column; scales (E8M0: 2^(byte - 127)) uint8 [ceil(cols / 512)][ceil(rows / block_rows)][4], 4-byte aligned: the byte of K block kb and
+ * row block r is [kb / 4][r][kb % 4], 127 behind the last block.  scale = smallest power of two >= 2^-127 with max |x| / scale <= 448
+ * over the block of block_rows x 128 (1 for a block of zeros), code = x / scale rounded to nearest even; Inf and NaN become the NaN
+ * code and leave the block's scale alone. */
+int64_t sm_fp8_codes_bytes(int64_t rows, int64_t cols);
+int64_t sm_fp8_scales_bytes(int64_t rows, int64_t cols, int block_rows);
+/* x [rows][cols] (row stride x_stride) -> any of: q / scale, its codes; q_t / scale_t, the codes of the transpose (cols x rows, blocks
+ * along the rows of x; with block_rows 128 the same codes, transposed); col_sum f32 [cols], the sums over the rows (deterministic).
+ * gate (may be NULL, same dtype, row stride gate_stride): values whose gate is not > 0 count as 0.  workspace:
+ * sm_fp8_quantize_workspace(rows, cols, col_sum != NULL) bytes, 16-byte aligned (may be NULL without col_sum). */
+int64_t sm_fp8_quantize_workspace(int64_t rows, int64_t cols, int col_sum);
+int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, const void* gate,
+                    int64_t gate_stride, void* q, void* scale, void* q_t, void* scale_t, float* col_sum, void* workspace,
+                    int64_t workspace_bytes, sm_stream_t stream);
 
 /* y [m][n] = a [m][k] . b [n][k]^T [+ bias f32 [n]] [+ residual [m][n]] [ReLU], f32 accumulation, one rounding to out_dtype
  * (sm_dtype; also the residual's).  workspace: sm_fp8_matmul_workspace(d) bytes, 16-byte aligned.  residual may be y. */
@@ -830,10 +835,11 @@ int64_t sm_fp8_matmul_workspace(const sm_fp8_matmul_desc* d);
 int sm_fp8_matmul(const sm_fp8_matmul_desc* d, const void* a, const void* a_scale, const void* b, const void* b_scale,
                   const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, sm_stream_t stream);
 
-/* out f32 [cols] = column sums of x [rows][cols] (row stride x_stride); deterministic */
-int64_t sm_col_sum_workspace(int64_t rows, int cols);
-int sm_col_sum(int dtype, const void* x, int64_t rows, int cols, int64_t x_stride, float* out, void* workspace,
-               int64_t workspace_bytes, sm_stream_t stream);
+/* the same on x [m][k] (x_dtype, row stride x_stride), quantised in 1 x 128 blocks on the way; d->a_block_rows = 1.  workspace:
+ * sm_fp8_linear_workspace(d).  With few rows this is one launch. */
+int64_t sm_fp8_linear_workspace(const sm_fp8_matmul_desc* d);
+int sm_fp8_linear(const sm_fp8_matmul_desc* d, int x_dtype, const void* x, int64_t x_stride, const void* b, const void* b_scale,
+                  const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, sm_stream_t stream);
 
 #ifdef __cplusplus
 }

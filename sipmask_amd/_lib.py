@@ -213,13 +213,14 @@ PROTOTYPES = {
     "sm_group_norm_act_bwd": (_I, [C.POINTER(GnActDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "sm_dropout": (_I, [_I, _P, _P, _P, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _I, C.c_uint64, C.c_uint64, _P,
                         _P]),
-    "sm_fp8_cols_padded": (C.c_int64, [C.c_int64]),
-    "sm_fp8_scale_cols": (C.c_int64, [C.c_int64]),
-    "sm_fp8_quantize": (_I, [_I, _P, C.c_int64, C.c_int64, C.c_int64, _I, _I, _P, _P, _P]),
+    "sm_fp8_codes_bytes": (C.c_int64, [C.c_int64, C.c_int64]),
+    "sm_fp8_scales_bytes": (C.c_int64, [C.c_int64, C.c_int64, _I]),
+    "sm_fp8_quantize_workspace": (C.c_int64, [C.c_int64, C.c_int64, _I]),
+    "sm_fp8_quantize": (_I, [_I, _P, C.c_int64, C.c_int64, C.c_int64, _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "sm_fp8_matmul_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
     "sm_fp8_matmul": (_I, [C.POINTER(Fp8MatmulDesc), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
-    "sm_col_sum_workspace": (C.c_int64, [C.c_int64, _I]),
-    "sm_col_sum": (_I, [_I, _P, C.c_int64, _I, C.c_int64, _P, _P, C.c_int64, _P]),
+    "sm_fp8_linear_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
+    "sm_fp8_linear": (_I, [C.POINTER(Fp8MatmulDesc), _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
 }
 
 _lib = None
@@ -261,10 +262,13 @@ def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_HERE_ALREADY = contextlib.nullcontext()
+
+
 def on_device(t):
     """context in which `t`'s device is the current one (launches, workspaces and stream_ptr() follow the current device)"""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE_ALREADY
     return torch.cuda.device(t.device)
 
 

@@ -14,9 +14,12 @@
 // (one conversion is 8 cycles; 16 of them beside 4 MFMAs measured 161 cycles against 154 for the MFMAs alone), and the bytes moved
 // through HBM and LDS stay 8-bit.
 //
-// Layout of a quantised matrix: codes [rows][Kp] with Kp = K rounded up to 128 (the tail is zero codes), scales
-// [row blocks][Kb4], Kb4 = K blocks rounded up to 4 (a K loop reads four scales of a row as one dword; padding = 127, i.e. 1).
+// Layout of a quantised matrix: codes [K block][row][128] (zero codes behind the last column), scales [K block / 4][row block][4]
+// (127, i.e. 1, behind the last block).  One K step of a tile is then one contiguous piece of memory: with codes [row][K] the rows of a
+// step lie K bytes apart, and for K a multiple of 4 KB they all fall on a few L2 channels (8192 x 4096 x 4096: 280 us with row-major
+// codes, 188 us with the loads left out).  A K loop reads four scales of a row as one dword, neighbouring rows side by side.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "elem.h"
@@ -65,19 +68,15 @@ __device__ __forceinline__ void fp8_load8(const typename Elem<DT>::type* row, lo
   }
 }
 
-// 1 x 128 blocks along the row: 16 threads per block of 128, 8 values each
+// 1 x 128 blocks along the row: a wave takes four neighbouring blocks of a row, 16 lanes each, 8 values per lane
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const typename Elem<DT>::type* __restrict__ x, long long rows, long long cols,
-                                                             long long ldx, int kb4, long long kp, uint8_t* __restrict__ q,
-                                                             uint8_t* __restrict__ scale) {
-  const long long units = rows * kb4;
-  for (long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); u < units; u += (long long)gridDim.x * 16) {
-    const long long r = u / kb4;
-    const int kb = (int)(u - r * kb4), l = threadIdx.x & 15;
-    if ((long long)kb * 128 >= kp) {             // padding of the scale row
-      if (l == 0) scale[u] = 127;
-      continue;
-    }
+                                                             long long ldx, int nkb, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  const int nq = (nkb + 3) >> 2, l = threadIdx.x & 15, sub = (threadIdx.x >> 4) & 3;
+  const long long units = rows * nq;
+  for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (long long)gridDim.x * 4) {
+    const long long r = u / nq;
+    const int kq = (int)(u - r * nq), kb = kq * 4 + sub;
     float f[8];
     fp8_load8<DT, VEC>(x + r * ldx, (long long)kb * 128 + l * 8, cols, f);
     float m = 0.f;
@@ -85,119 +84,150 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const typename Elem
     for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[e]));
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    const int sb = fp8_scale_byte(m);
-    *reinterpret_cast<uint2*>(q + r * kp + (long long)kb * 128 + l * 8) = fp8_pack8(f, fp8_inv_scale(sb));
-    if (l == 0) scale[u] = (uint8_t)sb;
+    const int sb = fp8_scale_byte(m);            // (a block behind the last column: zeros, 127)
+    if (kb < nkb) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + l * 8) = fp8_pack8(f, fp8_inv_scale(sb));
+    const uint32_t w = (uint32_t)__shfl(sb, 0, 64) | ((uint32_t)__shfl(sb, 16, 64) << 8) | ((uint32_t)__shfl(sb, 32, 64) << 16) |
+                       ((uint32_t)__shfl(sb, 48, 64) << 24);
+    if ((threadIdx.x & 63) == 0) *reinterpret_cast<uint32_t*>(scale + ((long long)kq * rows + r) * 4) = w;
   }
 }
 
-// One 128 x 64 piece (rows x columns) per block, 8 columns x 4 rows per thread.
-//   TRANS   codes go to q[column][row], blocks run along the rows: 1 x 128 (SQUARE false) or 128 x 128 (SQUARE true)
-//   !TRANS  codes go to q[row][column], 128 x 128 blocks (SQUARE)
-// A 128 x 128 block is two pieces: each reads the other half once more for its maximum (weights only: megabytes at most).
-template <int DT, bool VEC, bool TRANS, bool SQUARE>
-__global__ __launch_bounds__(256) void fp8_quant_tile_kernel(const typename Elem<DT>::type* __restrict__ x, long long rows, long long cols,
-                                                             long long ldx, int kb4, long long kp, uint8_t* __restrict__ q,
-                                                             uint8_t* __restrict__ scale) {
-  __shared__ float s_max[32][64 + 1];
-  __shared__ int s_byte[64];
-  __shared__ __attribute__((aligned(16))) uint8_t s_q[64][128 + 16];
-  const long long rb = blockIdx.x, r0 = rb * 128, c0 = (long long)blockIdx.y * 64;
-  const int cv = threadIdx.x & 7, rl = threadIdx.x >> 3;
-  float f[4][8], m[8];
+// One 128 x 128 piece of x per block, 8 columns x 8 consecutive rows per thread, read once for everything that is wanted of it:
+//   q / scale    codes in rows: 1 x 128 blocks, or the whole piece as one block (SQUARE)
+//   qt / scalet  codes of the transpose: blocks of 1 column x 128 rows, or the piece (SQUARE)
+//   colsum       f32 [row block][cols] sums over the piece's rows
+// each may be null.  gate (may be null): values whose gate is not > 0 count as 0 (the ReLU of a layer whose output is the gate).
+// Bound by memory: 2 + 1 + 1 bytes per 16-bit value; a training step that made the three from x one by one would read x three times.
+template <int DT, bool VEC, bool SQUARE>
+__global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem<DT>::type* __restrict__ x,
+                                                             const typename Elem<DT>::type* __restrict__ gate, long long rows, long long cols,
+                                                             long long ldx, long long ldg, int nkb, int nkbt, uint8_t* __restrict__ q,
+                                                             uint8_t* __restrict__ scale, uint8_t* __restrict__ qt,
+                                                             uint8_t* __restrict__ scalet, float* __restrict__ colsum) {
+  __shared__ float s_red[16][128];
+  __shared__ float s_wmax[4];
+  __shared__ int s_byte[128];
+  __shared__ __attribute__((aligned(16))) uint8_t s_q[128 * 128];
+  const long long rb = blockIdx.x, r0 = rb * 128, c0 = (long long)blockIdx.y * 128;
+  const int cv = threadIdx.x & 15, rl = threadIdx.x >> 4;
+  float f[8][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m[e] = 0.f;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const long long r = r0 + u * 32 + rl;
+  for (int u = 0; u < 8; ++u) {
+    const long long r = r0 + rl * 8 + u;
     if (r < rows) {
       fp8_load8<DT, VEC>(x + r * ldx, c0 + cv * 8, cols, f[u]);
+      if (gate != nullptr) {
+        float g[8];
+        fp8_load8<DT, VEC>(gate + r * ldg, c0 + cv * 8, cols, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[u][e] = g[e] > 0.f ? f[u][e] : 0.f;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[u][e] = 0.f;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] = fmaxf(m[e], fp8_abs_finite(f[u][e]));
   }
+  // byte of block kb of a scale row; the last block of a row fills the dword up with 127
+  auto put_scale = [](uint8_t* base, long long r, long long nr, int kb, int nb, int byte) {
+    uint8_t* p = base + ((long long)(kb >> 2) * nr + r) * 4;
+    p[kb & 3] = (uint8_t)byte;
+    if (kb == nb - 1)
+      for (int k = (kb & 3) + 1; k < 4; ++k) p[k] = 127;
+  };
+  const int kb = (int)(c0 >> 7), kbt = (int)rb;
+  int block_byte = 127;
   if constexpr (SQUARE) {
-    const long long co = c0 ^ 64;                // the block's other half
+    float m = 0.f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long r = r0 + u * 32 + rl;
+    for (int u = 0; u < 8; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[u][e]));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if ((threadIdx.x & 63) == 0) s_wmax[threadIdx.x >> 6] = m;
+    __syncthreads();
+    block_byte = fp8_scale_byte(fmaxf(fmaxf(s_wmax[0], s_wmax[1]), fmaxf(s_wmax[2], s_wmax[3])));
+    if (threadIdx.x == 0) {
+      if (q != nullptr) put_scale(scale, rb, (rows + 127) >> 7, kb, nkb, block_byte);
+      if (qt != nullptr) put_scale(scalet, kb, (cols + 127) >> 7, kbt, nkbt, block_byte);
+    }
+  }
+  if (q != nullptr) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const long long r = r0 + rl * 8 + u;
+      int sb = block_byte;
+      if constexpr (!SQUARE) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[u][e]));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        sb = fp8_scale_byte(m);
+      }
       if (r < rows) {
-        float g[8];
-        fp8_load8<DT, VEC>(x + r * ldx, co + cv * 8, cols, g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m[e] = fmaxf(m[e], fp8_abs_finite(g[e]));
+        *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + cv * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
+        if (!SQUARE && cv == 0) put_scale(scale, r, rows, kb, nkb, sb);
       }
     }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s_max[rl][cv * 8 + e] = m[e];
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    float t = 0.f;
-    for (int k = 0; k < 32; ++k) t = fmaxf(t, s_max[k][threadIdx.x]);
-    if constexpr (SQUARE) {
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) t = fmaxf(t, __shfl_xor(t, d, 64));
-    }
-    s_byte[threadIdx.x] = fp8_scale_byte(t);
-  }
-  __syncthreads();
-  if constexpr (!TRANS) {
-    const float inv = fp8_inv_scale(s_byte[0]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long r = r0 + u * 32 + rl;
-      if (r < rows && c0 + cv * 8 < kp) *reinterpret_cast<uint2*>(q + r * kp + c0 + cv * 8) = fp8_pack8(f[u], inv);
-    }
-    const int kb = (int)(c0 >> 7);
-    if ((c0 & 64) == 0 && threadIdx.x == 0) scale[rb * kb4 + kb] = (uint8_t)s_byte[0];
-    if (c0 + 128 >= kp && (c0 & 64) == 0 && threadIdx.x < 4 && kb + 1 + (int)threadIdx.x < kb4) scale[rb * kb4 + kb + 1 + threadIdx.x] = 127;
-  } else {
+  if (colsum != nullptr) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float inv = fp8_inv_scale(s_byte[cv * 8 + e]);
+      float t = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        s_q[cv * 8 + e][u * 32 + rl] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_prep(f[u][e], inv), 0.f, 0, false);
+      for (int u = 0; u < 8; ++u) t += f[u][e];
+      s_red[rl][cv * 8 + e] = t;
     }
     __syncthreads();
-    const int kb = (int)rb;
-    const bool last = r0 + 128 >= kp;            // the scale row's padding behind the last block
+    if (threadIdx.x < 128 && c0 + threadIdx.x < cols) {
+      float t = 0.f;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int i = threadIdx.x + 256 * p, c = i >> 3, ch = i & 7;
-      if (c0 + c < cols) *reinterpret_cast<uint4*>(q + (c0 + c) * kp + r0 + ch * 16) = *reinterpret_cast<const uint4*>(&s_q[c][ch * 16]);
+      for (int k = 0; k < 16; ++k) t += s_red[k][threadIdx.x];
+      colsum[rb * cols + c0 + threadIdx.x] = t;
     }
-    if (threadIdx.x < 64 && c0 + threadIdx.x < cols) {
-      const long long srow = SQUARE ? (c0 >> 7) : c0 + threadIdx.x;
-      if (!SQUARE || (threadIdx.x == 0 && (c0 & 64) == 0)) {
-        scale[srow * kb4 + kb] = (uint8_t)s_byte[threadIdx.x];
-        if (last)
-          for (int k = kb + 1; k < kb4; ++k) scale[srow * kb4 + k] = 127;
-      }
+    __syncthreads();
+  }
+  if (qt == nullptr) return;
+  if constexpr (!SQUARE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float m = 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) m = fmaxf(m, fp8_abs_finite(f[u][e]));
+      s_red[rl][cv * 8 + e] = m;
     }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float m = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) m = fmaxf(m, s_red[k][threadIdx.x]);
+      const int sb = fp8_scale_byte(m);
+      s_byte[threadIdx.x] = sb;
+      if (c0 + threadIdx.x < cols) put_scale(scalet, c0 + threadIdx.x, cols, kbt, nkbt, sb);
+    }
+    __syncthreads();
+  }
+  // the transpose goes through LDS: 8 rows of a column = 8 bytes, chunk rl of column c at slot rl ^ (c / 8) (16 columns of a wave's
+  // write then lie in 16 different slots)
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float inv = fp8_inv_scale(SQUARE ? block_byte : s_byte[cv * 8 + e]);
+    const float t[8] = {f[0][e], f[1][e], f[2][e], f[3][e], f[4][e], f[5][e], f[6][e], f[7][e]};
+    *reinterpret_cast<uint2*>(s_q + (cv * 8 + e) * 128 + ((rl ^ cv) * 8)) = fp8_pack8(t, inv);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int i = threadIdx.x + 256 * p, c = i >> 3, ch = i & 7, sw = c >> 3;
+    uint4 v = *reinterpret_cast<const uint4*>(s_q + c * 128 + ((ch ^ (sw >> 1)) * 16));
+    if (sw & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+    if (c0 + c < cols) *reinterpret_cast<uint4*>(qt + ((long long)kbt * cols + c0 + c) * 128 + ch * 16) = v;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ column sums
-// out[c] = sum over the rows, two launches, a fixed order: part[row block][c], then f64 over the row blocks
-constexpr int CS_ROWS = 512;
-template <int DT>
-__global__ __launch_bounds__(256) void col_sum_kernel(const typename Elem<DT>::type* __restrict__ x, long long rows, int cols, long long ldx,
-                                                      float* __restrict__ part) {
-  __shared__ float sh[4][64];
-  const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = blockIdx.x * 64 + cl;
-  const long long r0 = (long long)blockIdx.y * CS_ROWS, r1 = r0 + CS_ROWS < rows ? r0 + CS_ROWS : rows;
-  float s = 0.f;
-  if (c < cols)
-    for (long long r = r0 + rl; r < r1; r += 4) s += Elem<DT>::load(x + r * ldx + c);
-  sh[rl][cl] = s;
-  __syncthreads();
-  if (rl == 0 && c < cols) part[(long long)blockIdx.y * cols + c] = (sh[0][cl] + sh[1][cl]) + (sh[2][cl] + sh[3][cl]);
-}
+// out[c] = sum over the row blocks of part[block][c], f64, a fixed order
 __global__ __launch_bounds__(256) void col_sum_finish_kernel(const float* __restrict__ part, int nb, int cols, float* __restrict__ out) {
   __shared__ double sh[8][32];
   const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
@@ -214,15 +244,16 @@ __global__ __launch_bounds__(256) void col_sum_finish_kernel(const float* __rest
 
 // ------------------------------------------------------------------------------------------------ product
 struct MmArgs {
-  const uint8_t *a, *b, *sa, *sb;    // activations [m][kp], weights [n][kp] and their scales
+  const uint8_t *a, *b, *sa, *sb;    // activations, weights and their scales
   const float* bias;
   const void* res;
   void* y;
   float* part;                       // [ksplit][m][n] when ksplit > 1
-  long long m, ldy, ldr, kp;
-  int n, nkb, kb4, sha, shb;         // sha / shb: row >> sh = row of the scale matrix
-  int ksplit, relu, out, vec4;       // vec4: four consecutive n of y / residual are one aligned access
-  int tm, tn;                        // tiles
+  long long m, ldy, ldr, nsa;        // nsa / nsb: rows of the scale matrices
+  int n, nkb, nsb, sha, shb;         // sha / shb: row >> sh = row of the scale matrix
+  int ksplit, relu, out, vec;        // vec: eight consecutive n of y / residual are 16-byte aligned accesses
+  long long tm;                      // tiles
+  int tn;
 };
 
 __device__ __forceinline__ float mm_load(const void* p, int dt, long long i) {
@@ -249,23 +280,28 @@ __device__ __forceinline__ bf16x8 fp8_widen8(int lo, int hi, float scale) {
   return __builtin_shufflevector(ab, cd, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// bias, residual, ReLU and the store of four consecutive n (n0 a multiple of 4) of row m
-__device__ __forceinline__ void mm_finish4(const MmArgs& a, long long m, int n0, float (&v)[4]) {
-  if (a.vec4 && n0 + 4 <= a.n) {
+// bias, residual, ReLU and the store of V = 4 or 8 consecutive n (n0 a multiple of V) of row m
+template <int V>
+__device__ __forceinline__ void mm_finish(const MmArgs& a, long long m, int n0, float (&v)[V]) {
+  if (a.vec && n0 + V <= a.n) {
     if (a.bias != nullptr) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += a.bias[n0 + e];
+      for (int e = 0; e < V; ++e) v[e] += a.bias[n0 + e];
     }
     if (a.res != nullptr) {
       const long long o = m * a.ldr + n0;
       if (a.out == SM_DT_F32) {
-        const float4 r = *reinterpret_cast<const float4*>((const float*)a.res + o);
-        v[0] += r.x, v[1] += r.y, v[2] += r.z, v[3] += r.w;
-      } else {
-        const uint2 r = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + o);
-        const uint32_t w[2] = {r.x, r.y};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int q = 0; q < V / 4; ++q) {
+          const float4 r = *reinterpret_cast<const float4*>((const float*)a.res + o + 4 * q);
+          v[4 * q] += r.x, v[4 * q + 1] += r.y, v[4 * q + 2] += r.z, v[4 * q + 3] += r.w;
+        }
+      } else {
+        uint32_t w[V / 2];
+        if constexpr (V == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>((const uint16_t*)a.res + o);
+        else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>((const uint16_t*)a.res + o);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
           const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
           v[e] += a.out == SM_DT_BF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
         }
@@ -273,22 +309,31 @@ __device__ __forceinline__ void mm_finish4(const MmArgs& a, long long m, int n0,
     }
     if (a.relu) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+      for (int e = 0; e < V; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
     }
     const long long o = m * a.ldy + n0;
     if (a.out == SM_DT_F32) {
-      *reinterpret_cast<float4*>((float*)a.y + o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if (a.out == SM_DT_BF16) {
-      *reinterpret_cast<uint2*>((uint16_t*)a.y + o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    } else {
-      uint32_t h[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(uint16_t, (_Float16)v[e]);
-      *reinterpret_cast<uint2*>((uint16_t*)a.y + o) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+      for (int q = 0; q < V / 4; ++q)
+        *reinterpret_cast<float4*>((float*)a.y + o + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      return;
     }
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int q = 0; q < V / 2; ++q) {
+      if (a.out == SM_DT_BF16)
+        w[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
+      else
+        w[q] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * q]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * q + 1]) << 16);
+    }
+    if constexpr (V == 8) *reinterpret_cast<uint4*>((uint16_t*)a.y + o) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>((uint16_t*)a.y + o) = make_uint2(w[0], w[1]);
     return;
   }
-  for (int e = 0; e < 4 && n0 + e < a.n; ++e) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (n0 + e >= a.n) break;
     float t = v[e];
     if (a.bias != nullptr) t += a.bias[n0 + e];
     if (a.res != nullptr) t += mm_load(a.res, a.out, m * a.ldr + n0 + e);
@@ -297,23 +342,64 @@ __device__ __forceinline__ void mm_finish4(const MmArgs& a, long long m, int n0,
   }
 }
 
+// the f32 partial of a K split instead
+template <int V>
+__device__ __forceinline__ void mm_partial(const MmArgs& a, int ks, long long m, int n0, const float (&v)[V]) {
+  float* p = a.part + ((long long)ks * a.m + m) * a.n + n0;
+  if ((a.n & 3) == 0) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q)
+      if (n0 + 4 * q < a.n) *reinterpret_cast<float4*>(p + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (n0 + e < a.n) p[e] = v[e];
+  }
+}
+
+// f(0), ..., f(N - 1) with compile-time indices
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void mm_for(const F& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    mm_for<N, I + 1>(f);
+  }
+}
+
+// blockIdx.x -> tile.  The hardware hands consecutive blocks to the 8 XCDs in turn; tile numbers are laid out so that one XCD gets a
+// run of consecutive tiles (its own L2 then holds the operand panels they share).  Tiles run n-fastest inside bands of GM rows of tiles.
+__device__ __forceinline__ void mm_tile(const MmArgs& a, long long& tm, int& tn) {
+  const long long nt = (long long)a.tm * a.tn, b = blockIdx.x;
+  const long long q = nt >> 3, r = nt & 7, x = b & 7, i = b >> 3;
+  const long long t = x * q + (x < r ? x : r) + i;
+  constexpr int GM = 4;
+  const long long band = (long long)GM * a.tn, bi = t / band, o = t - bi * band;
+  const long long h = a.tm - bi * GM < GM ? a.tm - bi * GM : GM;
+  tn = (int)(o / h);
+  tm = bi * GM + (o - (long long)tn * h);
+}
+
 // Tile of BN weights x BM activations, waves of WN x WM, K steps of one block of 128 through two LDS stages filled by direct
 // global -> LDS loads.  A row of a stage is the 128 codes of one K block = 8 chunks of 16 bytes; chunk c of row r lies at slot
 // c ^ (r & 7), so the 32 rows that one fragment read touches spread over all banks.  The weights are the MFMA's first operand: a lane
-// of the accumulator then holds four consecutive n of one m.
+// of the accumulator then holds four consecutive n of one m.  The results leave through LDS (the stages are free by then), 64 x 64
+// at a time per wave, so that a store instruction writes whole 128-byte lines of a few rows instead of 16 bytes of 32 rows.
 template <int BN, int BM, int WN, int WM>
 __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(const MmArgs a) {
   constexpr int WAVES = (BN / WN) * (BM / WM), TN = WN / 32, TM = WM / 32;
   constexpr int STAGE = (BN + BM) * 128, PIECES = (BN + BM) / 8, PW = PIECES / WAVES;
   static_assert(PIECES % WAVES == 0, "whole pieces per wave");
+  static_assert(WN % 64 == 0 && WM % 64 == 0 && 2 * STAGE >= WAVES * 16384, "64 x 64 floats per wave in the epilogue");
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   typedef __attribute__((address_space(3))) void lds_void;
   typedef const __attribute__((address_space(1))) void glb_void;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * STAGE];
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];      // 2 * STAGE
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const long long tile = blockIdx.x;
-  const int n0 = (int)(tile % a.tn) * BN;
-  const long long m0 = (tile / a.tn) * BM;
+  long long tm;
+  int tn;
+  mm_tile(a, tm, tn);
+  const int n0 = tn * BN;
+  const long long m0 = tm * BM;
   const int ks = blockIdx.y;
   const int kb0 = (int)((long long)ks * a.nkb / a.ksplit), kb1 = (int)((long long)(ks + 1) * a.nkb / a.ksplit);
 
@@ -325,29 +411,32 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
     const int row = (wave * PW + i) * 8 + (lane >> 3), ch = (lane & 7) ^ (row & 7);
     if (row < BN) {
       const int r = n0 + row < a.n ? n0 + row : a.n - 1;
-      src[i] = a.b + (long long)r * a.kp + ch * 16;
+      src[i] = a.b + ((long long)kb0 * a.n + r) * 128 + ch * 16;
     } else {
       const long long r = m0 + row - BN < a.m ? m0 + row - BN : a.m - 1;
-      src[i] = a.a + r * a.kp + ch * 16;
+      src[i] = a.a + ((long long)kb0 * a.m + r) * 128 + ch * 16;
     }
   }
-  auto dma = [&](int kb, int buf) {
+  static_assert(BN % (8 * PW) == 0, "a wave's pieces are all weights or all activations");
+  const long long kstep = (wave * PW * 8 < BN ? (long long)a.n : a.m) * 128;
+  auto dma = [&](int buf) {                      // the next K block
 #pragma unroll
-    for (int i = 0; i < PW; ++i)
-      __builtin_amdgcn_global_load_lds((glb_void*)(src[i] + (long long)kb * 128),
-                                       (lds_void*)((lds_u8*)smem + buf * STAGE + (wave * PW + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < PW; ++i) {
+      __builtin_amdgcn_global_load_lds((glb_void*)src[i], (lds_void*)((lds_u8*)smem + buf * STAGE + (wave * PW + i) * 1024), 16, 0, 0);
+      src[i] += kstep;
+    }
   };
   const int wn = (wave % (BN / WN)) * WN, wm = (wave / (BN / WN)) * WM, l31 = lane & 31, kh = lane >> 5;
   const uint8_t *ps_n[TN], *ps_m[TM];
 #pragma unroll
   for (int i = 0; i < TN; ++i) {
     const int r = std::min(n0 + wn + i * 32 + l31, a.n - 1);
-    ps_n[i] = a.sb + (long long)(r >> a.shb) * a.kb4;
+    ps_n[i] = a.sb + (long long)(r >> a.shb) * 4;
   }
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const long long r = std::min<long long>(m0 + wm + j * 32 + l31, a.m - 1);
-    ps_m[j] = a.sa + (r >> a.sha) * a.kb4;
+    ps_m[j] = a.sa + (r >> a.sha) * 4;
   }
   f32x16 acc[TN][TM];
 #pragma unroll
@@ -358,20 +447,41 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   // 16 codes of a row: chunk c = 2 step + lane / 32 of the K block (the order of k inside a block is free as long as both operands
   // share it), two MFMA operands of 8 values
-  auto frag = [&](int buf, int row, int step) -> i32x4 {
-    return *reinterpret_cast<const i32x4*>(smem + buf * STAGE + row * 128 + (((step * 2 + kh) ^ (row & 7)) * 16));
+  const int rsw = l31 & 7;                       // every fragment row is l31 plus a multiple of 32
+  const uint8_t* const fbase_n = smem + (wn + l31) * 128;
+  const uint8_t* const fbase_m = smem + (BN + wm + l31) * 128;
+  // scales of the four K blocks at hand and of the next four: requested four steps before their use, so that no step waits for a load
+  // (the memory counter is in order: a wait for a scale is a wait for the whole stage in flight)
+  uint32_t dn[TN], dm[TM], en[TN], em[TM];
+  const int qlast = (a.nkb - 1) >> 2;
+  auto scales = [&](int quad, uint32_t (&n_)[TN], uint32_t (&m_)[TM]) {
+    const long long q4 = (long long)std::min(quad, qlast) * 4;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) n_[i] = *reinterpret_cast<const uint32_t*>(ps_n[i] + q4 * a.nsb);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) m_[j] = *reinterpret_cast<const uint32_t*>(ps_m[j] + q4 * a.nsa);
   };
-  uint32_t dn[TN], dm[TM];
-  if (kb0 < kb1) dma(kb0, 0);
+  scales(kb0 >> 2, dn, dm);
+  scales((kb0 >> 2) + 1, en, em);
+  i32x4 fn[2][TN], fm[2][TM];
+  auto read = [&](int set, int buf, int step) {
+    const int o = buf * STAGE + ((step * 2 + kh) ^ rsw) * 16;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) fn[set][i] = *reinterpret_cast<const i32x4*>(fbase_n + o + i * 32 * 128);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fm[set][j] = *reinterpret_cast<const i32x4*>(fbase_m + o + j * 32 * 128);
+  };
+  if (kb0 < kb1) dma(0);
   __syncthreads();
   for (int kb = kb0; kb < kb1; ++kb) {
     const int buf = (kb - kb0) & 1;
-    if (kb + 1 < kb1) dma(kb + 1, buf ^ 1);
-    if (kb == kb0 || (kb & 3) == 0) {
+    if (kb + 1 < kb1) dma(buf ^ 1);
+    if ((kb & 3) == 0 && kb != kb0) {
 #pragma unroll
-      for (int i = 0; i < TN; ++i) dn[i] = *reinterpret_cast<const uint32_t*>(ps_n[i] + (kb & ~3));
+      for (int i = 0; i < TN; ++i) dn[i] = en[i];
 #pragma unroll
-      for (int j = 0; j < TM; ++j) dm[j] = *reinterpret_cast<const uint32_t*>(ps_m[j] + (kb & ~3));
+      for (int j = 0; j < TM; ++j) dm[j] = em[j];
+      scales((kb >> 2) + 1, en, em);
     }
     const int sh = (kb & 3) * 8;
     float sn[TN], sm[TM];
@@ -379,20 +489,18 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
     for (int i = 0; i < TN; ++i) sn[i] = fp8_scale_float(dn[i] >> sh);
 #pragma unroll
     for (int j = 0; j < TM; ++j) sm[j] = fp8_scale_float(dm[j] >> sh);
+    read(0, buf, 0);
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      i32x4 fn[TN], fm[TM];
-#pragma unroll
-      for (int i = 0; i < TN; ++i) fn[i] = frag(buf, wn + i * 32 + l31, step);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) fm[j] = frag(buf, BN + wm + j * 32 + l31, step);
+      const int set = step & 1;
+      if (step < 3) read(set ^ 1, buf, step + 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         bf16x8 on[TN], om[TM];
 #pragma unroll
-        for (int i = 0; i < TN; ++i) on[i] = fp8_widen8(fn[i][2 * h], fn[i][2 * h + 1], sn[i]);
+        for (int i = 0; i < TN; ++i) on[i] = fp8_widen8(fn[set][i][2 * h], fn[set][i][2 * h + 1], sn[i]);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) om[j] = fp8_widen8(fm[j][2 * h], fm[j][2 * h + 1], sm[j]);
+        for (int j = 0; j < TM; ++j) om[j] = fp8_widen8(fm[set][j][2 * h], fm[set][j][2 * h + 1], sm[j]);
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -401,28 +509,109 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
     }
     __syncthreads();
   }
-  // accumulator e of a lane: n = 8 (e / 4) + 4 (lane / 32) + e % 4, m = lane % 32
+  // accumulator e of a lane: n = 8 (e / 4) + 4 (lane / 32) + e % 4, m = lane % 32.  64 m x 64 n floats of this wave's own LDS, the
+  // 16-byte chunk n / 4 of row m at slot (n / 4) ^ (m & 15); the reads follow the writes of the same wave in order
+  float* const E = reinterpret_cast<float*>(smem) + wave * 4096;
+  mm_for<TN / 2 * (TM / 2)>([&](auto IP) {       // (an unrolled loop of this size leaves acc indexed at run time, in scratch)
+    constexpr int ip = decltype(IP)::value % (TN / 2), jp = decltype(IP)::value / (TN / 2);
 #pragma unroll
-  for (int j = 0; j < TM; ++j) {
-    const long long m = m0 + wm + j * 32 + l31;
-    if (m >= a.m) continue;
+    for (int i2 = 0; i2 < 2; ++i2)
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn + i * 32 + g * 8 + kh * 4;
-        float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        if (a.ksplit > 1) {
-          float* p = a.part + ((long long)ks * a.m + m) * a.n + n;
-          if ((a.n & 3) == 0) {
-            if (n < a.n) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-          } else {
-            for (int e = 0; e < 4 && n + e < a.n; ++e) p[e] = v[e];
-          }
-        } else if (n < a.n) {
-          mm_finish4(a, m, n, v);
+        for (int g = 0; g < 4; ++g) {
+          const int m = j * 32 + l31, c = i2 * 8 + g * 2 + kh;
+          const f32x16 t = acc[ip * 2 + i2][jp * 2 + j];
+          *reinterpret_cast<float4*>(E + m * 64 + ((c ^ (m & 15)) * 4)) = make_float4(t[4 * g], t[4 * g + 1], t[4 * g + 2], t[4 * g + 3]);
+        }
+    __builtin_amdgcn_wave_barrier();
+    const int cl = (lane & 7) * 2, n = n0 + wn + ip * 64 + cl * 4;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int ml = r * 8 + (lane >> 3);
+      const long long m = m0 + wm + jp * 64 + ml;
+      const float4 p = *reinterpret_cast<const float4*>(E + ml * 64 + ((cl ^ (ml & 15)) * 4));
+      const float4 q = *reinterpret_cast<const float4*>(E + ml * 64 + (((cl + 1) ^ (ml & 15)) * 4));
+      float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+      if (m < a.m && n < a.n) {
+        if (a.ksplit > 1) mm_partial(a, ks, m, n, v);
+        else mm_finish(a, m, n, v);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  });
+}
+
+// A handful of activation rows (16 MT per block): the weights are what has to be read, and they are read once, straight into registers.
+// A block takes 16 weight rows, its 16 waves every 16th K block; a lane holds 32 neighbouring codes of one row (the four MFMAs of a
+// block share that order of k for both operands).  SRC: sm_dtype of x, which is then quantised on the way -- no launch and no buffer
+// for it -- or 3 for codes.  The waves' sums meet in LDS in wave order.
+template <int SRC, bool VEC, int MT>
+__global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const void* __restrict__ xv, long long ldx, long long cols) {
+  constexpr int WAVES = 16;
+  __shared__ __attribute__((aligned(16))) float s_acc[WAVES][MT][64][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const long long m0 = (long long)blockIdx.y * (16 * MT);
+  const int n = std::min(n0 + r, a.n - 1);
+  long long row[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) row[t] = std::min<long long>(m0 + t * 16 + r, a.m - 1);
+  f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+  for (int kb = wave; kb < a.nkb; kb += WAVES) {
+    const i32x4* pw = reinterpret_cast<const i32x4*>(a.b + ((long long)kb * a.n + n) * 128 + g * 32);
+    const i32x4 w0 = pw[0], w1 = pw[1];
+    const float sw = fp8_scale_float(a.sb[((long long)(kb >> 2) * a.nsb + (n >> a.shb)) * 4 + (kb & 3)]);
+    const bf16x8 on[4] = {fp8_widen8(w0[0], w0[1], sw), fp8_widen8(w0[2], w0[3], sw), fp8_widen8(w1[0], w1[1], sw), fp8_widen8(w1[2], w1[3], sw)};
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      bf16x8 om[4];
+      if constexpr (SRC == 3) {
+        const i32x4* pa = reinterpret_cast<const i32x4*>(a.a + ((long long)kb * a.m + row[t]) * 128 + g * 32);
+        const i32x4 a0 = pa[0], a1 = pa[1];
+        const float sm = fp8_scale_float(a.sa[((long long)(kb >> 2) * a.nsa + (row[t] >> a.sha)) * 4 + (kb & 3)]);
+        om[0] = fp8_widen8(a0[0], a0[1], sm), om[1] = fp8_widen8(a0[2], a0[3], sm);
+        om[2] = fp8_widen8(a1[0], a1[1], sm), om[3] = fp8_widen8(a1[2], a1[3], sm);
+      } else {
+        typedef typename Elem<SRC>::type T;
+        const T* px = (const T*)xv + row[t] * ldx;
+        float f[4][8], m = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          fp8_load8<SRC, VEC>(px, (long long)kb * 128 + g * 32 + q * 8, cols, f[q]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[q][e]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const int sb = fp8_scale_byte(m);
+        const float inv = fp8_inv_scale(sb), sm = fp8_scale_float((uint32_t)sb);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint2 c = fp8_pack8(f[q], inv);
+          om[q] = fp8_widen8((int)c.x, (int)c.y, sm);
         }
       }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(on[q], om[q], acc[t], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4*>(&s_acc[wave][t][lane][0]) = acc[t];
+  __syncthreads();
+  // accumulator e of a lane: n = 4 (lane / 16) + e, m = lane % 16
+  if (threadIdx.x < MT * 64) {
+    const int t = threadIdx.x >> 6;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v += *reinterpret_cast<const f32x4*>(&s_acc[w][t][lane][0]);
+    float o[4] = {v[0], v[1], v[2], v[3]};
+    const long long m = m0 + t * 16 + r;
+    if (m < a.m && n0 + 4 * g < a.n) mm_finish(a, m, n0 + 4 * g, o);
   }
 }
 
@@ -443,18 +632,22 @@ __global__ __launch_bounds__(256) void fp8_mm_finish_kernel(const MmArgs a) {
         for (int e = 0; e < 4 && n + e < a.n; ++e) v[e] += p[e];
       }
     }
-    mm_finish4(a, m, n, v);
+    mm_finish(a, m, n, v);
   }
 }
 
 struct MmPlan {
-  int bm, bn, ksplit;
+  int few, big, ksplit;              // few: fp8_mm_few_kernel; big: 256 x 256 tiles
   long long tm;
   int tn;
   long long ws;
 };
 
-// 128 x 128 tiles; K is split while there are fewer than two tiles per CU and every split keeps four blocks of 128
+// MM_FEW rows or fewer: fp8_mm_few_kernel.
+// 256 x 256 tiles (a wave widens 3 pairs of codes per MFMA, one block fills a CU and nothing covers its epilogue) when they fill the chip
+// and K is long, 128 x 128 (4 pairs per MFMA, two blocks per CU) else: 230 against 245 us at 8192 x 4096 x 4096, but 91 against 74 us at
+// 67200 x 512 x 768.  K is split while there are fewer than two small tiles per CU and every split keeps four blocks of 128.
+constexpr int MM_FEW = 64;
 int mm_plan(const sm_fp8_matmul_desc* d, MmPlan* p) {
   if (d == nullptr) return SM_ERR_BAD_ARG;
   if (d->m < 0 || d->n < 1 || d->k < 1) return SM_ERR_BAD_SHAPE;
@@ -462,98 +655,103 @@ int mm_plan(const sm_fp8_matmul_desc* d, MmPlan* p) {
       d->out_dtype < SM_DT_BF16 || d->out_dtype > SM_DT_F32)
     return SM_ERR_BAD_ARG;
   if (d->y_stride < d->n || d->n > 0x7fffff00 || d->k > 0x7fffff00) return SM_ERR_BAD_SHAPE;
-  p->bm = p->bn = 128;
-  p->tm = (d->m + 127) / 128;
-  p->tn = sm_cdiv(d->n, 128);
+  const long long big = ((d->m + 255) / 256) * sm_cdiv(d->n, 256);
+  p->few = d->m <= MM_FEW;
+  p->big = big >= 256 && d->k >= 2048;
+  const int t = p->big ? 256 : 128;
+  p->tm = (d->m + t - 1) / t;
+  p->tn = sm_cdiv(d->n, t);
   const int nkb = sm_cdiv(d->k, 128);
   const long long tiles = p->tm * p->tn;
   if (tiles > 0xfff000) return SM_ERR_UNSUPPORTED;
-  p->ksplit = tiles == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>(512 / tiles, nkb / 4));
+  p->ksplit = tiles == 0 || p->big || p->few ? 1 : (int)std::max<long long>(1, std::min<long long>(512 / tiles, nkb / 4));
   p->ws = p->ksplit > 1 ? (long long)p->ksplit * d->m * d->n * 4 : 0;
   return SM_OK;
 }
 
 }  // namespace
 
-extern "C" int64_t sm_fp8_cols_padded(int64_t cols) { return (cols + 127) / 128 * 128; }
-extern "C" int64_t sm_fp8_scale_cols(int64_t cols) { return ((cols + 127) / 128 + 3) / 4 * 4; }
+extern "C" int64_t sm_fp8_codes_bytes(int64_t rows, int64_t cols) {
+  return rows < 0 || cols < 0 ? SM_ERR_BAD_SHAPE : (cols + 127) / 128 * rows * 128;
+}
+extern "C" int64_t sm_fp8_scales_bytes(int64_t rows, int64_t cols, int block_rows) {
+  if (block_rows != 1 && block_rows != 128) return SM_ERR_BAD_ARG;
+  return rows < 0 || cols < 0 ? SM_ERR_BAD_SHAPE : (cols + 511) / 512 * ((rows + block_rows - 1) / block_rows) * 4;
+}
 
 namespace {
+struct QuantArgs {
+  const void *x, *gate;
+  long long rows, cols, ldx, ldg;
+  int square;
+  uint8_t *q, *scale, *qt, *scalet;
+  float* colsum;
+};
 template <int DT>
-int fp8_quant_launch(const void* xv, long long rows, long long cols, long long ldx, int block_rows, int transpose, void* qv, void* sv,
-                     hipStream_t s) {
+int fp8_quant_launch(const QuantArgs& a, hipStream_t s) {
   typedef typename Elem<DT>::type T;
-  const T* x = (const T*)xv;
-  uint8_t *q = (uint8_t*)qv, *sc = (uint8_t*)sv;
-  const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (16 / sm_dtype_bytes(DT)) == 0;
-  const long long along = transpose ? rows : cols;
-  const long long kp = sm_fp8_cols_padded(along);
-  const int kb4 = (int)sm_fp8_scale_cols(along);
-  if (!transpose && block_rows == 1) {
-    const unsigned blocks = (unsigned)std::min<long long>((rows * kb4 + 15) / 16, 256 * 32);
-    if (vec) hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, x, rows, cols, ldx, kb4, kp, q, sc);
-    else hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, x, rows, cols, ldx, kb4, kp, q, sc);
+  const int per16 = 16 / sm_dtype_bytes(DT);
+  const bool vec = ((uintptr_t)a.x & 15) == 0 && a.ldx % per16 == 0 && (!a.gate || (((uintptr_t)a.gate & 15) == 0 && a.ldg % per16 == 0));
+  const int nkb = sm_cdiv(a.cols, 128);
+  if (!a.square && !a.qt && !a.colsum && !a.gate) {    // rows alone: no tile, no LDS
+    const unsigned blocks = (unsigned)std::min<long long>((a.rows * ((nkb + 3) / 4) + 3) / 4, 256 * 32);
+    if (vec) hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, (const T*)a.x, a.rows, a.cols, a.ldx, nkb, a.q, a.scale);
+    else hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, (const T*)a.x, a.rows, a.cols, a.ldx, nkb, a.q, a.scale);
     SM_LAUNCH_CHECK();
     return SM_OK;
   }
-  const long long rb = (rows + 127) / 128, cb = transpose ? (cols + 63) / 64 : kp / 64;
-  if (cb > 65535 || rb > 0xfff000) return SM_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)rb, (unsigned)cb);
-#define SM_Q(V, T_, S_) hipLaunchKernelGGL((fp8_quant_tile_kernel<DT, V, T_, S_>), grid, dim3(256), 0, s, x, rows, cols, ldx, kb4, kp, q, sc)
-  if (!transpose) {
-    if (vec) SM_Q(true, false, true);
-    else SM_Q(false, false, true);
-  } else if (block_rows == 128) {
-    if (vec) SM_Q(true, true, true);
-    else SM_Q(false, true, true);
+  const long long rb = (a.rows + 127) / 128;
+  if (nkb > 65535 || rb > 0xfff000) return SM_ERR_UNSUPPORTED;
+#define SM_Q(V, S_)                                                                                                               \
+  hipLaunchKernelGGL((fp8_quant_pair_kernel<DT, V, S_>), dim3((unsigned)rb, nkb), dim3(256), 0, s, (const T*)a.x, (const T*)a.gate, \
+                     a.rows, a.cols, a.ldx, a.ldg, nkb, (int)rb, a.q, a.scale, a.qt, a.scalet, a.colsum)
+  if (a.square) {
+    if (vec) SM_Q(true, true);
+    else SM_Q(false, true);
   } else {
-    if (vec) SM_Q(true, true, false);
-    else SM_Q(false, true, false);
+    if (vec) SM_Q(true, false);
+    else SM_Q(false, false);
   }
 #undef SM_Q
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
+int fp8_quant_run(int dtype, const QuantArgs& a, hipStream_t s) {
+  if (dtype == SM_DT_BF16) return fp8_quant_launch<SM_DT_BF16>(a, s);
+  if (dtype == SM_DT_F16) return fp8_quant_launch<SM_DT_F16>(a, s);
+  return fp8_quant_launch<SM_DT_F32>(a, s);
+}
+bool fp8_out_ok(const void* q, const void* scale) {
+  return (q == nullptr) == (scale == nullptr) && ((uintptr_t)q & 15) == 0 && ((uintptr_t)scale & 3) == 0;
+}
 }  // namespace
 
-extern "C" int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, int transpose,
-                               void* q, void* scale, sm_stream_t stream) {
+extern "C" int64_t sm_fp8_quantize_workspace(int64_t rows, int64_t cols, int col_sum) {
+  if (rows < 0 || cols < 1) return SM_ERR_BAD_SHAPE;
+  return col_sum ? std::max<int64_t>(16, (rows + 127) / 128 * cols * 4) : 16;
+}
+
+extern "C" int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, const void* gate,
+                               int64_t gate_stride, void* q, void* scale, void* q_t, void* scale_t, float* col_sum, void* workspace,
+                               int64_t workspace_bytes, sm_stream_t stream) {
   if (dtype < SM_DT_BF16 || dtype > SM_DT_F32 || (block_rows != 1 && block_rows != 128)) return SM_ERR_BAD_ARG;
   if (rows < 0 || cols < 1 || x_stride < cols || cols > 0x7fffff00 || rows > (int64_t)1 << 40) return SM_ERR_BAD_SHAPE;
-  if (rows == 0) return transpose ? SM_ERR_BAD_SHAPE : SM_OK;
-  if (transpose && rows > 0x7fffff00) return SM_ERR_BAD_SHAPE;
-  if (!x || !q || !scale || ((uintptr_t)q & 15) != 0 || ((uintptr_t)scale & 3) != 0) return SM_ERR_BAD_ARG;
+  if (q_t && (rows < 1 || rows > 0x7fffff00)) return SM_ERR_BAD_SHAPE;     // (the transpose sums over the rows)
+  if (gate && gate_stride < cols) return SM_ERR_BAD_SHAPE;
+  if (!fp8_out_ok(q, scale) || !fp8_out_ok(q_t, scale_t) || (!q && !q_t && !col_sum)) return SM_ERR_BAD_ARG;
   hipStream_t s = sm_hip_stream(stream);
-  if (dtype == SM_DT_BF16) return fp8_quant_launch<SM_DT_BF16>(x, rows, cols, x_stride, block_rows, transpose, q, scale, s);
-  if (dtype == SM_DT_F16) return fp8_quant_launch<SM_DT_F16>(x, rows, cols, x_stride, block_rows, transpose, q, scale, s);
-  return fp8_quant_launch<SM_DT_F32>(x, rows, cols, x_stride, block_rows, transpose, q, scale, s);
-}
-
-extern "C" int64_t sm_col_sum_workspace(int64_t rows, int cols) {
-  if (rows < 0 || cols < 1) return SM_ERR_BAD_SHAPE;
-  return std::max<int64_t>(16, (rows + CS_ROWS - 1) / CS_ROWS * cols * 4);
-}
-
-extern "C" int sm_col_sum(int dtype, const void* x, int64_t rows, int cols, int64_t x_stride, float* out, void* workspace,
-                          int64_t workspace_bytes, sm_stream_t stream) {
-  if (dtype < SM_DT_BF16 || dtype > SM_DT_F32) return SM_ERR_BAD_ARG;
-  if (rows < 0 || cols < 1 || x_stride < cols) return SM_ERR_BAD_SHAPE;
-  if (!out || !workspace || (rows > 0 && !x)) return SM_ERR_BAD_ARG;
-  if (workspace_bytes < sm_col_sum_workspace(rows, cols)) return SM_ERR_WORKSPACE;
-  const long long nb = (rows + CS_ROWS - 1) / CS_ROWS;
-  if (nb > 65535) return SM_ERR_UNSUPPORTED;
-  hipStream_t s = sm_hip_stream(stream);
-  float* part = (float*)workspace;
-  if (nb > 0) {
-    const dim3 grid(sm_cdiv(cols, 64), (unsigned)nb);
-    if (dtype == SM_DT_BF16)
-      hipLaunchKernelGGL((col_sum_kernel<SM_DT_BF16>), grid, dim3(256), 0, s, (const uint16_t*)x, (long long)rows, cols, (long long)x_stride, part);
-    else if (dtype == SM_DT_F16)
-      hipLaunchKernelGGL((col_sum_kernel<SM_DT_F16>), grid, dim3(256), 0, s, (const _Float16*)x, (long long)rows, cols, (long long)x_stride, part);
-    else
-      hipLaunchKernelGGL((col_sum_kernel<SM_DT_F32>), grid, dim3(256), 0, s, (const float*)x, (long long)rows, cols, (long long)x_stride, part);
+  if (rows == 0) {
+    if (col_sum && sm_zero_async(col_sum, sizeof(float) * cols, s) != hipSuccess) return SM_ERR_LAUNCH;
+    return SM_OK;
   }
-  hipLaunchKernelGGL(col_sum_finish_kernel, dim3(sm_cdiv(cols, 32)), dim3(256), 0, s, part, (int)nb, cols, out);
+  if (!x) return SM_ERR_BAD_ARG;
+  if (col_sum && (!workspace || ((uintptr_t)workspace & 15) != 0)) return SM_ERR_BAD_ARG;
+  if (col_sum && workspace_bytes < sm_fp8_quantize_workspace(rows, cols, 1)) return SM_ERR_WORKSPACE;
+  const QuantArgs a = {x, gate, rows, cols, x_stride, gate_stride, block_rows == 128, (uint8_t*)q, (uint8_t*)scale, (uint8_t*)q_t,
+                       (uint8_t*)scale_t, col_sum ? (float*)workspace : nullptr};
+  const int st = fp8_quant_run(dtype, a, s);
+  if (st != SM_OK || !col_sum) return st;
+  hipLaunchKernelGGL(col_sum_finish_kernel, dim3(sm_cdiv(cols, 32)), dim3(256), 0, s, (const float*)workspace, sm_cdiv(rows, 128), (int)cols, col_sum);
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
@@ -565,34 +763,110 @@ extern "C" int64_t sm_fp8_matmul_workspace(const sm_fp8_matmul_desc* d) {
   return std::max<int64_t>(16, p.ws);
 }
 
-extern "C" int sm_fp8_matmul(const sm_fp8_matmul_desc* d, const void* a, const void* a_scale, const void* b, const void* b_scale,
-                             const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes,
-                             sm_stream_t stream) {
-  MmPlan p;
-  const int st = mm_plan(d, &p);
-  if (st != SM_OK) return st;
-  if (d->m == 0) return SM_OK;
-  if (!a || !a_scale || !b || !b_scale || !y) return SM_ERR_BAD_ARG;
-  if (residual && d->res_stride < d->n) return SM_ERR_BAD_SHAPE;
-  if ((((uintptr_t)a | (uintptr_t)b) & 15) != 0 || (((uintptr_t)a_scale | (uintptr_t)b_scale) & 3) != 0) return SM_ERR_BAD_ARG;
-  if (p.ws > 0 && (!workspace || ((uintptr_t)workspace & 15) != 0)) return SM_ERR_BAD_ARG;
-  if (workspace_bytes < p.ws) return SM_ERR_WORKSPACE;
+namespace {
+template <int SRC, bool VEC>
+void mm_few_launch(const MmArgs& k, const void* x, long long ldx, long long cols, hipStream_t s) {
+  if (k.m <= 16)
+    hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 1>), dim3(sm_cdiv(k.n, 16), 1), dim3(1024), 0, s, k, x, ldx, cols);
+  else
+    hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 4>), dim3(sm_cdiv(k.n, 16), sm_cdiv(k.m, 64)), dim3(1024), 0, s, k, x, ldx, cols);
+}
+
+// the product behind its checks.  x != null: a is quantised from it (x_dtype, row stride ldx) -- by the few-rows kernel itself, else into
+// the workspace behind the K splits' partials
+int mm_run(const sm_fp8_matmul_desc* d, const MmPlan& p, const void* a, const void* a_scale, const void* b, const void* b_scale,
+           const float* bias, const void* residual, void* y, void* workspace, int x_dtype, const void* x, long long ldx, hipStream_t s) {
   MmArgs k;
   k.a = (const uint8_t*)a, k.b = (const uint8_t*)b, k.sa = (const uint8_t*)a_scale, k.sb = (const uint8_t*)b_scale;
   k.bias = bias, k.res = residual, k.y = y, k.part = (float*)workspace;
   k.m = d->m, k.n = d->n, k.ldy = d->y_stride, k.ldr = residual ? d->res_stride : 0;
-  k.kp = sm_fp8_cols_padded(d->k), k.nkb = sm_cdiv(d->k, 128), k.kb4 = (int)sm_fp8_scale_cols(d->k);
+  k.nkb = sm_cdiv(d->k, 128);
+  k.nsa = (d->m + d->a_block_rows - 1) / d->a_block_rows, k.nsb = (d->n + d->b_block_rows - 1) / d->b_block_rows;
   k.sha = d->a_block_rows == 128 ? 7 : 0, k.shb = d->b_block_rows == 128 ? 7 : 0;
   k.ksplit = p.ksplit, k.relu = d->relu, k.out = d->out_dtype;
-  const uintptr_t al = (uintptr_t)(4 * sm_dtype_bytes(d->out_dtype) - 1);
-  k.vec4 = ((uintptr_t)y & al) == 0 && d->y_stride % 4 == 0 && (!residual || (((uintptr_t)residual & al) == 0 && d->res_stride % 4 == 0));
-  k.tm = (int)p.tm, k.tn = p.tn;
-  hipStream_t s = sm_hip_stream(stream);
-  hipLaunchKernelGGL((fp8_mm_kernel<128, 128, 64, 64>), dim3((unsigned)(p.tm * p.tn), p.ksplit), dim3(256), 0, s, k);
+  const int per16 = 16 / sm_dtype_bytes(d->out_dtype);
+  k.vec = ((uintptr_t)y & 15) == 0 && d->y_stride % per16 == 0 && (!residual || (((uintptr_t)residual & 15) == 0 && d->res_stride % per16 == 0));
+  k.tm = p.tm, k.tn = p.tn;
+  if (p.few) {
+    if (x == nullptr) {
+      mm_few_launch<3, true>(k, nullptr, 0, 0, s);
+    } else {
+      const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (16 / sm_dtype_bytes(x_dtype)) == 0;
+      if (x_dtype == SM_DT_BF16) vec ? mm_few_launch<SM_DT_BF16, true>(k, x, ldx, d->k, s) : mm_few_launch<SM_DT_BF16, false>(k, x, ldx, d->k, s);
+      else if (x_dtype == SM_DT_F16) vec ? mm_few_launch<SM_DT_F16, true>(k, x, ldx, d->k, s) : mm_few_launch<SM_DT_F16, false>(k, x, ldx, d->k, s);
+      else vec ? mm_few_launch<SM_DT_F32, true>(k, x, ldx, d->k, s) : mm_few_launch<SM_DT_F32, false>(k, x, ldx, d->k, s);
+    }
+    SM_LAUNCH_CHECK();
+    return SM_OK;
+  }
+  if (x != nullptr) {
+    uint8_t* q = (uint8_t*)workspace + (p.ws + 15) / 16 * 16;
+    uint8_t* sc = q + sm_fp8_codes_bytes(d->m, d->k);
+    const QuantArgs qa = {x, nullptr, d->m, d->k, ldx, 0, 0, q, sc, nullptr, nullptr, nullptr};
+    const int st = fp8_quant_run(x_dtype, qa, s);
+    if (st != SM_OK) return st;
+    k.a = q, k.sa = sc;
+  }
+  const dim3 grid((unsigned)(p.tm * p.tn), p.ksplit);
+  if (p.big) {
+    const void* kern = (const void*)fp8_mm_kernel<256, 256, 128, 64>;
+    if (sm_lds_optin(kern, 131072) != hipSuccess) return SM_ERR_LAUNCH;
+    hipLaunchKernelGGL((fp8_mm_kernel<256, 256, 128, 64>), grid, dim3(512), 131072, s, k);
+  } else {
+    hipLaunchKernelGGL((fp8_mm_kernel<128, 128, 64, 64>), grid, dim3(256), 65536, s, k);
+  }
   if (p.ksplit > 1) {
     const long long total = k.m * ((k.n + 3) / 4);
     hipLaunchKernelGGL(fp8_mm_finish_kernel, dim3((unsigned)std::min<long long>((total + 255) / 256, 256 * 16)), dim3(256), 0, s, k);
   }
   SM_LAUNCH_CHECK();
   return SM_OK;
+}
+
+int mm_check(const sm_fp8_matmul_desc* d, const void* b, const void* b_scale, const void* residual, const void* y, const void* workspace,
+             int64_t workspace_bytes, int64_t need) {
+  if (!b || !b_scale || !y || ((uintptr_t)b & 15) != 0 || ((uintptr_t)b_scale & 3) != 0) return SM_ERR_BAD_ARG;
+  if (residual && d->res_stride < d->n) return SM_ERR_BAD_SHAPE;
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15) != 0)) return SM_ERR_BAD_ARG;
+  return workspace_bytes < need ? SM_ERR_WORKSPACE : SM_OK;
+}
+
+int64_t linear_ws(const sm_fp8_matmul_desc* d, const MmPlan& p) {
+  return p.few ? 0 : (p.ws + 15) / 16 * 16 + sm_fp8_codes_bytes(d->m, d->k) + sm_fp8_scales_bytes(d->m, d->k, 1);
+}
+}  // namespace
+
+extern "C" int sm_fp8_matmul(const sm_fp8_matmul_desc* d, const void* a, const void* a_scale, const void* b, const void* b_scale,
+                             const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes,
+                             sm_stream_t stream) {
+  MmPlan p;
+  int st = mm_plan(d, &p);
+  if (st != SM_OK) return st;
+  if (d->m == 0) return SM_OK;
+  if (!a || !a_scale || ((uintptr_t)a & 15) != 0 || ((uintptr_t)a_scale & 3) != 0) return SM_ERR_BAD_ARG;
+  st = mm_check(d, b, b_scale, residual, y, workspace, workspace_bytes, p.ws);
+  if (st != SM_OK) return st;
+  return mm_run(d, p, a, a_scale, b, b_scale, bias, residual, y, workspace, 0, nullptr, 0, sm_hip_stream(stream));
+}
+
+extern "C" int64_t sm_fp8_linear_workspace(const sm_fp8_matmul_desc* d) {
+  MmPlan p;
+  const int st = mm_plan(d, &p);
+  if (st != SM_OK) return st;
+  return std::max<int64_t>(16, linear_ws(d, p));
+}
+
+extern "C" int sm_fp8_linear(const sm_fp8_matmul_desc* d, int x_dtype, const void* x, int64_t x_stride, const void* b,
+                             const void* b_scale, const float* bias, const void* residual, void* y, void* workspace,
+                             int64_t workspace_bytes, sm_stream_t stream) {
+  MmPlan p;
+  int st = mm_plan(d, &p);
+  if (st != SM_OK) return st;
+  if (x_dtype < SM_DT_BF16 || x_dtype > SM_DT_F32 || d->a_block_rows != 1) return SM_ERR_BAD_ARG;
+  if (x_stride < d->k) return SM_ERR_BAD_SHAPE;
+  if (d->m == 0) return SM_OK;
+  if (!x) return SM_ERR_BAD_ARG;
+  st = mm_check(d, b, b_scale, residual, y, workspace, workspace_bytes, linear_ws(d, p));
+  if (st != SM_OK) return st;
+  return mm_run(d, p, nullptr, nullptr, b, b_scale, bias, residual, y, workspace, x_dtype, x, x_stride, sm_hip_stream(stream));
 }

@@ -1419,6 +1419,15 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}         # sm
 _MASK64 = (1 << 64) - 1
 
 
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(t):
+    """the current stream of t's device, as the handle the C entry points take"""
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
 def dtype_code(t, what):
     code = DTYPE_CODES.get(t.dtype)
     if code is None:
@@ -1433,6 +1442,8 @@ def row_stride(t):
 
 def dense_rows(t, cols):
     """`t` [..., cols] as a 2-D tensor with dense, non-overlapping rows (copied only where its strides do not allow the view)"""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     rows = 1
     for s in t.shape[:-1]:
         rows *= s
@@ -1491,8 +1502,8 @@ def group_norm_act(d, x, gamma, beta, want_stats):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stats = torch.empty(d.batch * d.nlev * d.groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
     ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 0), x.device, "sm_group_norm_act")
-    _lib.check(lib.sm_group_norm_act(C.byref(d), _lib.ptr(x), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(y), _lib.ptr(stats),
-                                     _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_group_norm_act")
+    _lib.check(lib.sm_group_norm_act(C.byref(d), _p(x), _p(gamma), _p(beta), _p(y), _p(stats),
+                                     _p(ws), ws.numel(), _stream(x)), "sm_group_norm_act")
     return y, stats
 
 
@@ -1502,54 +1513,74 @@ def group_norm_act_bwd(d, x, dy, gamma, beta, stats, need_dx=True, dgamma=None, 
     d.dy_stride = row_stride(dy)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
     ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 1), x.device, "sm_group_norm_act_bwd")
-    _lib.check(lib.sm_group_norm_act_bwd(C.byref(d), _lib.ptr(x), _lib.ptr(dy), _lib.ptr(gamma), _lib.ptr(beta), _lib.ptr(stats),
-                                         _lib.ptr(dx), _lib.ptr(dgamma), _lib.ptr(dbeta), _lib.ptr(ws), ws.numel(),
-                                         _lib.stream_ptr()), "sm_group_norm_act_bwd")
+    _lib.check(lib.sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats),
+                                         _p(dx), _p(dgamma), _p(dbeta), _p(ws), ws.numel(),
+                                         _stream(x)), "sm_group_norm_act_bwd")
     return dx
 
 
-def dropout_rows(x, residual, thr, seed, offset):
-    """x (and residual) [rows, cols] with dense rows -> dense rows"""
+def dropout_rows(x, residual, thr, seed, offset, y):
+    """x (and residual) [rows, cols] with dense rows -> y, contiguous"""
     lib = _lib.load()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     host, dev = offset
-    _lib.check(lib.sm_dropout(dtype_code(x, "dropout"), _lib.ptr(x), _lib.ptr(residual), _lib.ptr(y), x.shape[0], x.shape[1],
+    _lib.check(lib.sm_dropout(dtype_code(x, "dropout"), _p(x), _p(residual), _p(y), x.shape[0], x.shape[1],
                               row_stride(x), 0 if residual is None else row_stride(residual), x.shape[1], thr,
-                              int(seed) & _MASK64, host, _lib.ptr(dev), _lib.stream_ptr()), "sm_dropout")
+                              int(seed) & _MASK64, host, _p(dev), _stream(x)), "sm_dropout")
     return y
 
 
 # ------------------------------------------------------------------------------- 8-bit products
-def fp8_quantize(x, block_rows, transpose):
-    """x [rows, cols] with dense rows -> (codes [r, cols_padded(c)] e4m3, scales uint8 [ceil(r / block_rows), scale_cols(c)]) of
-    (r, c) = (rows, cols), or (cols, rows) with transpose"""
+def _fp8_alloc(r, c, block_rows, device):
+    """(codes e4m3 [ceil(c / 128), r, 128], scales uint8 [ceil(c / 512), ceil(r / block_rows), 4]) of an r x c matrix"""
+    return (torch.empty(-(-c // 128), r, 128, dtype=torch.float8_e4m3fn, device=device),
+            torch.empty(-(-c // 512), -(-r // block_rows), 4, dtype=torch.uint8, device=device))
+
+
+def fp8_quantize(x, block_rows, rows=True, transpose=False, col_sum=False, gate=None):
+    """x (and gate) [r, c] with dense rows, read once -> ((codes, scales) or None, the transpose's (codes, scales) or None, f32 column
+    sums or None); gate: values whose gate is not > 0 count as 0"""
     lib = _lib.load()
-    r, c = (x.shape[1], x.shape[0]) if transpose else (x.shape[0], x.shape[1])
-    q = torch.empty(r, int(lib.sm_fp8_cols_padded(c)), dtype=torch.float8_e4m3fn, device=x.device)
-    s = torch.empty(-(-r // block_rows), int(lib.sm_fp8_scale_cols(c)), dtype=torch.uint8, device=x.device)
-    _lib.check(lib.sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _lib.ptr(x), x.shape[0], x.shape[1], row_stride(x), block_rows,
-                                   int(transpose), _lib.ptr(q), _lib.ptr(s), _lib.stream_ptr()), "sm_fp8_quantize")
-    return q, s
+    r, c = x.shape
+    q, s = _fp8_alloc(r, c, block_rows, x.device) if rows else (None, None)
+    qt, st = _fp8_alloc(c, r, block_rows, x.device) if transpose else (None, None)
+    cs = ws = None
+    if col_sum:
+        cs = torch.empty(c, dtype=torch.float32, device=x.device)
+        ws = _workspace(lib.sm_fp8_quantize_workspace(r, c, 1), x.device, "sm_fp8_quantize")
+    _lib.check(lib.sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _p(x), r, c, row_stride(x), block_rows, _p(gate),
+                                   0 if gate is None else row_stride(gate), _p(q), _p(s), _p(qt), _p(st), _p(cs), _p(ws),
+                                   0 if ws is None else ws.numel(), _stream(x)), "sm_fp8_quantize")
+    return (q, s) if rows else None, (qt, st) if transpose else None, cs
+
+
+def _fp8_desc(m, n, k, a_block_rows, b_block_rows, out_dtype, relu, residual):
+    d = _lib.Fp8MatmulDesc()
+    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows = m, n, k, a_block_rows, b_block_rows
+    d.out_dtype, d.relu, d.y_stride = DTYPE_CODES[out_dtype], int(relu), n
+    d.res_stride = 0 if residual is None else row_stride(residual)
+    return d
 
 
 def fp8_matmul(a, sa, a_block_rows, b, sb, b_block_rows, k, bias, residual, relu, out_dtype):
     lib = _lib.load()
-    d = _lib.Fp8MatmulDesc()
-    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows = a.shape[0], b.shape[0], k, a_block_rows, b_block_rows
-    d.out_dtype, d.relu, d.y_stride = DTYPE_CODES[out_dtype], int(relu), b.shape[0]
-    d.res_stride = 0 if residual is None else row_stride(residual)
-    y = torch.empty(a.shape[0], b.shape[0], dtype=out_dtype, device=a.device)
-    ws = _workspace(lib.sm_fp8_matmul_workspace(C.byref(d)), a.device, "sm_fp8_matmul")
-    _lib.check(lib.sm_fp8_matmul(C.byref(d), _lib.ptr(a), _lib.ptr(sa), _lib.ptr(b), _lib.ptr(sb), _lib.ptr(bias),
-                                 _lib.ptr(residual), _lib.ptr(y), _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_fp8_matmul")
+    m, n = a.shape[1], b.shape[1]
+    d = _fp8_desc(m, n, k, a_block_rows, b_block_rows, out_dtype, relu, residual)
+    y = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    need = lib.sm_fp8_matmul_workspace(C.byref(d))
+    ws = None if 0 <= need <= 16 else _workspace(need, a.device, "sm_fp8_matmul")
+    _lib.check(lib.sm_fp8_matmul(C.byref(d), _p(a), _p(sa), _p(b), _p(sb), _p(bias), _p(residual), _p(y), _p(ws),
+                                 0 if ws is None else need, _stream(a)), "sm_fp8_matmul")
     return y
 
 
-def col_sum(x):
-    """f32 column sums of x [rows, cols] with dense rows"""
+def fp8_linear(x, b, sb, b_block_rows, bias, residual, relu, out_dtype):
+    """x [m, k] with dense rows, quantised on the way, times the codes b"""
     lib = _lib.load()
-    out = torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
-    ws = _workspace(lib.sm_col_sum_workspace(x.shape[0], x.shape[1]), x.device, "sm_col_sum")
-    _lib.check(lib.sm_col_sum(dtype_code(x, "col_sum"), _lib.ptr(x), x.shape[0], x.shape[1], row_stride(x), _lib.ptr(out),
-                              _lib.ptr(ws), ws.numel(), _lib.stream_ptr()), "sm_col_sum")
-    return out
+    (m, k), n = x.shape, b.shape[1]
+    d = _fp8_desc(m, n, k, 1, b_block_rows, out_dtype, relu, residual)
+    y = torch.empty(m, n, dtype=out_dtype, device=x.device)
+    need = lib.sm_fp8_linear_workspace(C.byref(d))
+    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_fp8_linear")
+    _lib.check(lib.sm_fp8_linear(C.byref(d), dtype_code(x, "linear_fp8"), _p(x), row_stride(x), _p(b), _p(sb), _p(bias), _p(residual),
+                                 _p(y), _p(ws), 0 if ws is None else need, _stream(x)), "sm_fp8_linear")
+    return y

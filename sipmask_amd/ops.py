@@ -297,46 +297,52 @@ group_norm = GroupNormFunction.apply
 
 # ------------------------------------------------------------------------------- GroupNorm + activation, dropout
 class GroupNormActFunction(Function):
-    """act(GroupNorm(x)) [dropped out] of rows x [lv.rows, C] (sm_group_norm_act / _bwd).  The backward recomputes the normalised
-    values and the dropout mask; only x, the parameters and (mean, rstd) per (image, level, group) are kept."""
+    """act(GroupNorm(x)) [dropped out] of channels-last values (sm_group_norm_act / _bwd): x [N, C, *] with lv None, or pyramid rows
+    [lv.rows, C].  The backward recomputes the normalised values and the dropout mask; only x, the parameters and (mean, rstd) per
+    (image, level, group) are kept."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, lv, groups, eps, act, thr, seed, offset, sink):
+    def forward(ctx, x, gamma, beta, lv, groups, eps, act, thr, seed, offset):
         g32 = None if gamma is None else gamma.detach().float().contiguous()
         b32 = None if beta is None else beta.detach().float().contiguous()
         host, dev = H.dropout_offset(offset, x.device)
+        last = x.movedim(1, -1) if lv is None else x
+        rows = H.dense_rows(last, last.shape[-1])
         with _lib.on_device(x):
-            d = H.group_norm_act_desc(x, lv, groups, eps, act, thr, seed, (host, dev))
-            y, stats = H.group_norm_act(d, x, g32, b32, any(ctx.needs_input_grad))
-        ctx.save_for_backward(x, g32, b32, stats, dev)      # (dev: an offset that changed before the backward is an error)
-        ctx.cfg = (lv, groups, eps, act, thr, seed, host, sink, None if gamma is None else gamma.dtype,
-                   None if beta is None else beta.dtype)
-        return y
+            d = H.group_norm_act_desc(rows, lv if lv is not None else H.Levels(x.shape[0], [(rows.shape[0] // max(x.shape[0], 1), 1)]),
+                                      groups, eps, act, thr, seed, (host, dev))
+            y, stats = H.group_norm_act(d, rows, g32, b32, any(ctx.needs_input_grad))
+        if stats is not None:
+            ctx.save_for_backward(x, g32, b32, stats, dev)  # (dev: an offset that changed before the backward is an error)
+            ctx.cfg = (d, lv, None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
+        return y.view(last.shape).movedim(-1, 1) if lv is None else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, g32, b32, stats, dev = ctx.saved_tensors
-        lv, groups, eps, act, thr, seed, host, sink, gdt, bdt = ctx.cfg
+        x, g32, b32, stats, _ = ctx.saved_tensors
+        d, lv, gdt, bdt = ctx.cfg
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
-        dy = H.dense_rows(dy, x.shape[1])
-        tg = H.GRAD_SINK.target(g32) if sink and need_g else None
-        tb = H.GRAD_SINK.target(b32) if sink and need_b else None
-        if (need_g and tg is None) or (need_b and tb is None):
-            tg = tb = None
-        new = lambda: torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+        last, dlast = (x.movedim(1, -1), dy.movedim(1, -1)) if lv is None else (x, dy)
+        c = last.shape[-1]
+        tg = tb = None
+        if lv is not None:                                  # the row graph's parameters may live in all-reduce buckets
+            tg = H.GRAD_SINK.target(g32) if need_g else None
+            tb = H.GRAD_SINK.target(b32) if need_b else None
+        new = lambda: torch.empty(c, dtype=torch.float32, device=x.device)
         dg = None if not need_g else (tg if tg is not None else new())
         db = None if not need_b else (tb if tb is not None else new())
         with _lib.on_device(x):
-            d = H.group_norm_act_desc(x, lv, groups, eps, act, thr, seed, (host, dev))
-            dx = H.group_norm_act_bwd(d, x, dy, g32, b32, stats, need_x, dg, db)
+            dx = H.group_norm_act_bwd(d, H.dense_rows(last, c), H.dense_rows(dlast, c), g32, b32, stats, need_x, dg, db)
+        if dx is not None and lv is None:
+            dx = dx.view(last.shape).movedim(-1, 1)
         if tg is not None:
             H.GRAD_SINK.commit(g32)
             dg = None
         if tb is not None:
             H.GRAD_SINK.commit(b32)
             db = None
-        return (dx, None if dg is None else dg.to(gdt), None if db is None else db.to(bdt)) + (None,) * 8
+        return (dx, None if dg is None else dg.to(gdt), None if db is None else db.to(bdt)) + (None,) * 7
 
 
 def _gn_act_args(x, channels, weight, bias, groups, eps, activation, dropout_p, what):
@@ -367,38 +373,38 @@ def group_norm_act(x, weight, bias, num_groups, eps=1e-5, activation="relu", dro
         raise ValueError("group_norm_act: x is [N, C, *]")
     c = x.shape[1]
     act, thr = _gn_act_args(x, c, weight, bias, num_groups, eps, activation, dropout_p, "group_norm_act")
-    last = x.movedim(1, -1)
-    hw = 1
-    for s in x.shape[2:]:
-        hw *= s
-    y = GroupNormActFunction.apply(H.dense_rows(last, c), weight, bias, H.Levels(x.shape[0], [(hw, 1)]), num_groups, eps, act, thr,
-                                   seed, offset, False)
-    return y.view(last.shape).movedim(-1, 1)
+    return GroupNormActFunction.apply(x, weight, bias, None, num_groups, eps, act, thr, seed, offset)
+
+
+def _dropout_rows(x, residual, thr, seed, offset):
+    """any shape and strides -> contiguous"""
+    flat = x.is_contiguous() and (residual is None or residual.is_contiguous())
+    cols = x.shape[-1] if x.dim() else 1
+    rows = lambda t: None if t is None else (t.view(1, -1) if flat else H.dense_rows(t, cols))
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel():
+        with _lib.on_device(x):
+            H.dropout_rows(rows(x), rows(residual), thr, seed, offset, y)
+    return y
 
 
 class DropoutFunction(Function):
-    """x [rows, cols] with dense rows -> keep * x / (1 - p) [+ residual] (sm_dropout)"""
+    """keep * x / (1 - p) [+ residual] (sm_dropout)"""
 
     @staticmethod
     def forward(ctx, x, residual, thr, seed, offset):
-        host, dev = H.dropout_offset(offset, x.device)
-        with _lib.on_device(x):
-            y = H.dropout_rows(x, residual, thr, seed, (host, dev))
-        ctx.save_for_backward(dev)
-        ctx.cfg = (thr, seed, host)
-        return y
+        off = H.dropout_offset(offset, x.device)
+        ctx.save_for_backward(off[1])
+        ctx.cfg = (thr, seed, off[0])
+        return _dropout_rows(x, residual, thr, seed, off)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (dev,) = ctx.saved_tensors
         thr, seed, host = ctx.cfg
-        dx = None
-        if ctx.needs_input_grad[0]:
-            g = H.dense_rows(dy, dy.shape[1])
-            with _lib.on_device(g):
-                dx = H.dropout_rows(g, None, thr, seed, (host, dev))
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        dev, = ctx.saved_tensors
+        return (_dropout_rows(dy, None, thr, seed, (host, dev)) if ctx.needs_input_grad[0] else None,
+                dy if ctx.needs_input_grad[1] else None, None, None, None)
 
 
 def dropout(x, p, seed, offset=0, residual=None, training=True):
@@ -419,17 +425,14 @@ def dropout(x, p, seed, offset=0, residual=None, training=True):
         if residual is None:
             return x
         thr = 0
-    H.dropout_offset(offset, x.device)
-    cols = x.shape[-1] if x.dim() else 1
-    flat = x.is_contiguous() and (residual is None or residual.is_contiguous())
-    rows = lambda t: None if t is None else (t.reshape(1, -1) if flat else H.dense_rows(t, cols))
-    return DropoutFunction.apply(rows(x), rows(residual), thr, seed, offset).view(x.shape)
+    return DropoutFunction.apply(x, residual, thr, seed, offset)
 
 
 # ------------------------------------------------------------------------------- 8-bit products
 class Fp8Blocks:
-    """A matrix [rows, cols] in e4m3 with one power-of-two scale per block of block_rows x 128 (include/sipmask_hip.h has the
-    layout): `codes` float8_e4m3fn [rows, cols padded to 128], `scales` uint8 (2^(byte - 127))."""
+    """A matrix [rows, cols] in e4m3 with one power-of-two scale per block of block_rows x 128, laid out for the product:
+    `codes` float8_e4m3fn [ceil(cols / 128), rows, 128], `scales` uint8 (2^(byte - 127)) [ceil(cols / 512), ceil(rows / block_rows),
+    4].  code_matrix() / scale_matrix() put them back in rows."""
     __slots__ = ("codes", "scales", "rows", "cols", "block_rows")
 
     def __init__(self, codes, scales, rows, cols, block_rows):
@@ -443,12 +446,20 @@ class Fp8Blocks:
     def device(self):
         return self.codes.device
 
+    def code_matrix(self):
+        """codes [rows, cols]"""
+        c = self.codes.view(torch.uint8).transpose(0, 1).reshape(self.rows, -1)[:, :self.cols]
+        return c.contiguous().view(torch.float8_e4m3fn)
+
+    def scale_matrix(self):
+        """scale bytes [ceil(rows / block_rows), ceil(cols / 128)]"""
+        return self.scales.transpose(0, 1).reshape(self.scales.shape[1], -1)[:, :-(-self.cols // 128)].contiguous()
+
     def dequantize(self, dtype=torch.float32):
         """the values the codes stand for (for checks and for code without an 8-bit product)"""
-        nkb = -(-self.cols // 128)
-        s = ((self.scales[:, :nkb].to(torch.int64) + (1023 - 127)) << 52).view(torch.float64)
+        s = ((self.scale_matrix().to(torch.int64) + (1023 - 127)) << 52).view(torch.float64)
         s = s.repeat_interleave(self.block_rows, 0)[:self.rows].repeat_interleave(128, 1)[:, :self.cols]
-        return (self.codes[:, :self.cols].to(torch.float64) * s).to(dtype)
+        return (self.code_matrix().to(torch.float64) * s).to(dtype)
 
 
 def quantize_fp8(x, block_rows=1, transpose=False):
@@ -465,9 +476,10 @@ def quantize_fp8(x, block_rows=1, transpose=False):
         raise ValueError("quantize_fp8: the transpose of 0 rows has no columns")
     x = H.dense_rows(x.detach(), x.shape[1])
     with _lib.on_device(x):
-        q, s = H.fp8_quantize(x, block_rows, transpose)
-    r, c = (x.shape[1], x.shape[0]) if transpose else x.shape
-    return Fp8Blocks(q, s, r, c, block_rows)
+        rows, cols, _ = H.fp8_quantize(x, block_rows, not transpose, transpose)
+    if transpose:
+        return Fp8Blocks(cols[0], cols[1], x.shape[1], x.shape[0], block_rows)
+    return Fp8Blocks(rows[0], rows[1], x.shape[0], x.shape[1], block_rows)
 
 
 def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloat16):
@@ -495,40 +507,53 @@ def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloa
 
 
 class LinearFp8Function(Function):
-    """y = q(x) q(w)^T + bias (ReLU);  dx = q(dy) q(w);  dw = q(dy^T) q(x^T)^T;  dbias = column sums of dy"""
+    """y = q(x) q(w)^T + bias (ReLU);  dx = q(dy) q(w);  dw = q(dy^T) q(x^T)^T;  dbias = column sums of dy.  Everything the backward
+    needs of x and w is made in the pass that quantises them for the forward: the codes of the transposes (one byte a value)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, relu, weight_q):
-        w = None if weight is None else weight.detach().reshape(weight.shape[0], -1)
-        wq = weight_q if weight_q is not None else quantize_fp8(w, 128)
-        y = matmul_fp8(quantize_fp8(x), wq, bias, relu, None, x.dtype)
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, y if relu else None)
-        ctx.cfg = (relu, None if bias is None else bias.dtype, x.dtype)
-        return y
+        need_x, need_w = ctx.needs_input_grad[:2]
+        rows = H.dense_rows(x, x.shape[-1])
+        b32 = None if bias is None else bias.detach().float().contiguous()
+        xt = wt = None
+        with _lib.on_device(x):
+            if weight_q is None or need_x:
+                w = H.dense_rows(weight.flatten(1), rows.shape[1])
+                wq, wt, _ = H.fp8_quantize(w, 128, weight_q is None, need_x)
+            if weight_q is not None:
+                wq = (weight_q.codes, weight_q.scales)
+            if need_w and rows.shape[0] > 0:
+                xq, xt, _ = H.fp8_quantize(rows, 1, True, True)
+                y = H.fp8_matmul(xq[0], xq[1], 1, wq[0], wq[1], 128, rows.shape[1], b32, None, relu, x.dtype)
+            else:
+                y = H.fp8_linear(rows, wq[0], wq[1], 128, b32, None, relu, x.dtype)
+        if any(ctx.needs_input_grad):
+            pair = lambda t: (None, None) if t is None else t
+            ctx.save_for_backward(*pair(xt), *pair(wt), y if relu else None)
+            ctx.cfg = (None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, rows.shape[1],
+                       x.shape[:-1])
+        return y.view(x.shape[:-1] + (y.shape[1],))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, y = ctx.saved_tensors
-        relu, bdt, dt = ctx.cfg
+        xt, sxt, wt, swt, y = ctx.saved_tensors
+        wmeta, bdt, k, shape = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if relu:
-            dy = torch.where(y > 0, dy, torch.zeros((), dtype=dy.dtype, device=dy.device))
-        dy = H.dense_rows(dy, dy.shape[1])
+        dy = H.dense_rows(dy, dy.shape[-1])
+        m, n = dy.shape
         dx = dw = db = None
-        if need_x:
-            wt = quantize_fp8(weight.detach().reshape(weight.shape[0], -1), 128, transpose=True)
-            dx = matmul_fp8(quantize_fp8(dy), wt, out_dtype=dt)
-        if need_w:
-            if dy.shape[0] == 0:
-                dw = torch.zeros_like(weight)
-            else:
-                dw = matmul_fp8(quantize_fp8(dy, transpose=True), quantize_fp8(x, transpose=True), out_dtype=torch.float32)
-                dw = dw.view(weight.shape).to(weight.dtype)
-        if need_b:
-            with _lib.on_device(dy):
-                db = H.col_sum(dy).to(bdt)
-        return dx, dw, db, None, None
+        with _lib.on_device(dy):
+            if m == 0:
+                dw = torch.zeros(wmeta[0], dtype=wmeta[1], device=dy.device) if need_w else None
+                db = torch.zeros(n, dtype=bdt, device=dy.device) if need_b else None
+                return dy.new_empty(shape + (k,)) if need_x else None, dw, db, None, None
+            g, gt, db = H.fp8_quantize(dy, 1, need_x, need_w, need_b, y)
+            if need_x:
+                dx = H.fp8_matmul(g[0], g[1], 1, wt, swt, 128, n, None, None, False, dy.dtype).view(shape + (k,))
+            if need_w:
+                dw = H.fp8_matmul(gt[0], gt[1], 1, xt, sxt, 1, m, None, None, False, torch.float32).view(wmeta[0]).to(wmeta[1])
+        return dx, dw, None if db is None else db.to(bdt), None, None
 
 
 def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
@@ -555,8 +580,7 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
         raise ValueError("linear_fp8: bias is [%d] on %s" % (n, x.device))
     if weight is None and torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("linear_fp8: a gradient of x needs the weight itself, not weight_q alone")
-    y = LinearFp8Function.apply(H.dense_rows(x, k), weight, bias, relu, weight_q)
-    return y.view(x.shape[:-1] + (n,))
+    return LinearFp8Function.apply(x, weight, bias, relu, weight_q)
 
 
 class UpsampleBilinearFunction(Function):

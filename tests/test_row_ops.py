@@ -143,15 +143,18 @@ def test_dropout_bad_arguments():
 def test_fp8_bad_arguments():
     lib = _lib.load()
     one, odd = C.c_void_p(16), C.c_void_p(17)
-    assert [lib.sm_fp8_cols_padded(c) for c in (1, 128, 129)] == [128, 128, 256]
-    assert [lib.sm_fp8_scale_cols(c) for c in (1, 512, 513)] == [4, 4, 8]
+    assert [lib.sm_fp8_codes_bytes(10, c) for c in (1, 128, 129)] == [1280, 1280, 2560] and lib.sm_fp8_codes_bytes(-1, 1) == -1
+    assert [lib.sm_fp8_scales_bytes(200, c, br) for c, br in ((1, 1), (512, 1), (513, 1), (513, 128))] == [800, 800, 1600, 16]
+    assert lib.sm_fp8_scales_bytes(1, 1, 2) == -2
 
-    def q(dt=0, x=one, rows=4, cols=8, ld=8, br=1, tr=0, codes=one, sc=one):
-        return lib.sm_fp8_quantize(dt, x, rows, cols, ld, br, tr, codes, sc, None)
+    def q(dt=0, x=one, rows=4, cols=8, ld=8, br=1, gate=None, ldg=8, codes=one, sc=one, ct=None, st=None, cs=None, ws=None, n=0):
+        return lib.sm_fp8_quantize(dt, x, rows, cols, ld, br, gate, ldg, codes, sc, ct, st, cs, ws, n, None)
     assert q(dt=5) == -2 and q(br=2) == -2 and q(x=None) == -2 and q(codes=None) == -2 and q(sc=None) == -2
-    assert q(codes=odd) == -2 and q(sc=odd) == -2
-    assert q(rows=-1) == -1 and q(cols=0) == -1 and q(ld=7) == -1 and q(rows=0, tr=1) == -1 and q(rows=0) == 0
-    assert q(rows=1 << 33, tr=1) == -1
+    assert q(codes=odd) == -2 and q(sc=odd) == -2 and q(codes=None, sc=None) == -2 and q(ct=one) == -2 and q(ct=odd, st=one) == -2
+    assert q(rows=-1) == -1 and q(cols=0) == -1 and q(ld=7) == -1 and q(rows=0, ct=one, st=one) == -1 and q(rows=0) == 0
+    assert q(rows=1 << 33, ct=one, st=one) == -1 and q(gate=one, ldg=7) == -1
+    assert q(cs=one) == -2 and q(cs=one, ws=one, n=31) == -5 and lib.sm_fp8_quantize_workspace(4, 8, 1) == 32
+    assert lib.sm_fp8_quantize_workspace(-1, 8, 1) == -1 and lib.sm_fp8_quantize_workspace(1, 0, 0) == -1
 
     def mm(ws=1 << 40, res=None, a=one, y=one, wsp=one, **kw):
         d = _lib.Fp8MatmulDesc()
@@ -165,15 +168,19 @@ def test_fp8_bad_arguments():
         assert mm(**bad) == -2, bad
     assert mm(m=0, a=None, y=None) == 0
     d = _lib.Fp8MatmulDesc()
-    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows, d.y_stride = 64, 512, 1 << 16, 1, 1, 512
+    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows, d.y_stride = 100, 512, 1 << 16, 1, 1, 512
     need = lib.sm_fp8_matmul_workspace(C.byref(d))
     assert need > 16                             # few tiles, long sum: split
     assert lib.sm_fp8_matmul(C.byref(d), one, one, one, one, None, None, one, one, need - 1, None) == -5
     assert lib.sm_fp8_matmul(C.byref(d), one, one, one, one, None, None, one, None, need, None) == -2
-    assert lib.sm_col_sum_workspace(-1, 4) == -1 and lib.sm_col_sum_workspace(10, 0) == -1
-    assert lib.sm_col_sum(0, one, 10, 4, 3, one, one, 1 << 30, None) == -1
-    assert lib.sm_col_sum(0, one, 10, 4, 4, one, one, 1, None) == -5
-    assert lib.sm_col_sum(7, one, 10, 4, 4, one, one, 1 << 30, None) == -2
+    d.m = 1000
+    need = lib.sm_fp8_linear_workspace(C.byref(d))
+
+    def lin(dt=0, x=one, ld=1 << 16, y=one, ws=one, n=need):
+        return lib.sm_fp8_linear(C.byref(d), dt, x, ld, one, one, None, None, y, ws, n, None)
+    assert lin(dt=3) == -2 and lin(x=None) == -2 and lin(y=None) == -2 and lin(ws=None) == -2 and lin(ld=10) == -1 and lin(n=need - 1) == -5
+    d.a_block_rows = 128
+    assert lin() == -2
 
 
 # ------------------------------------------------------------------------------------------------ Python entry points
