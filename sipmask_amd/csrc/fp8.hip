@@ -40,20 +40,37 @@ __device__ __forceinline__ int fp8_scale_byte(float amax) {
 // 2^-e of a scale byte: 254 - byte is a normal exponent for every byte the quantiser makes (0 .. 247)
 __device__ __forceinline__ float fp8_inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-// Inf and NaN have no code but NaN: they are left out of the block's maximum and stored as NaN
+// Inf and NaN have no code but NaN and are left out of the block's maximum.  A maximum skips NaN by itself, and the conversion makes
+// NaN of NaN and of Inf; only the maximum of a block that holds an Inf is taken again, over what is finite (rare: one compare per block).
 __device__ __forceinline__ float fp8_abs_finite(float x) {
   const float a = __builtin_fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
-__device__ __forceinline__ float fp8_prep(float x, float inv) {
-  return __builtin_fabsf(x) <= 3.402823466e38f ? x * inv : __uint_as_float(0x7fc00000u);
+template <int N>
+__device__ __forceinline__ float fp8_amax(const float* f) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, __builtin_fabsf(f[e]));
+  if (m > 3.402823466e38f) {
+    m = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = fmaxf(m, fp8_abs_finite(f[e]));
+  }
+  return m;
+}
+// maximum over the 16 lanes of a DPP row, on every lane: quad permutes, then rotations by 4 and 8
+__device__ __forceinline__ float max16(float m) {
+  m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xB1, 0xf, 0xf, true)));    // lane ^ 1
+  m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4E, 0xf, 0xf, true)));    // lane ^ 2
+  m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x124, 0xf, 0xf, true)));   // row_ror:4
+  return fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x128, 0xf, 0xf, true)));   // row_ror:8
 }
 __device__ __forceinline__ uint2 fp8_pack8(const float* f, float inv) {
   int lo = 0, hi = 0;
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_prep(f[0], inv), fp8_prep(f[1], inv), lo, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_prep(f[2], inv), fp8_prep(f[3], inv), lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_prep(f[4], inv), fp8_prep(f[5], inv), hi, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_prep(f[6], inv), fp8_prep(f[7], inv), hi, true);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
   return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
@@ -68,27 +85,34 @@ __device__ __forceinline__ void fp8_load8(const typename Elem<DT>::type* row, lo
   }
 }
 
-// 1 x 128 blocks along the row: a wave takes four neighbouring blocks of a row, 16 lanes each, 8 values per lane
+// 1 x 128 blocks along the row: a wave takes four neighbouring blocks of a row, 16 lanes each, 8 values per lane; four such pieces are in
+// flight
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const typename Elem<DT>::type* __restrict__ x, long long rows, long long cols,
                                                              long long ldx, int nkb, uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  constexpr int U = 4;
   const int nq = (nkb + 3) >> 2, l = threadIdx.x & 15, sub = (threadIdx.x >> 4) & 3;
-  const long long units = rows * nq;
-  for (long long u = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u < units; u += (long long)gridDim.x * 4) {
-    const long long r = u / nq;
-    const int kq = (int)(u - r * nq), kb = kq * 4 + sub;
-    float f[8];
-    fp8_load8<DT, VEC>(x + r * ldx, (long long)kb * 128 + l * 8, cols, f);
-    float m = 0.f;
+  const long long units = rows * nq, step = (long long)gridDim.x * 4;
+  for (long long u0 = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); u0 < units; u0 += U * step) {
+    float f[U][8];
+    long long r[U];
+    int kq[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[e]));
+    for (int p = 0; p < U; ++p) {
+      const long long u = u0 + p * step < units ? u0 + p * step : u0;     // (behind the end: the first piece again)
+      r[p] = u / nq;
+      kq[p] = (int)(u - r[p] * nq);
+      fp8_load8<DT, VEC>(x + r[p] * ldx, (long long)(kq[p] * 4 + sub) * 128 + l * 8, cols, f[p]);
+    }
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    const int sb = fp8_scale_byte(m);            // (a block behind the last column: zeros, 127)
-    if (kb < nkb) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + l * 8) = fp8_pack8(f, fp8_inv_scale(sb));
-    const uint32_t w = (uint32_t)__shfl(sb, 0, 64) | ((uint32_t)__shfl(sb, 16, 64) << 8) | ((uint32_t)__shfl(sb, 32, 64) << 16) |
-                       ((uint32_t)__shfl(sb, 48, 64) << 24);
-    if ((threadIdx.x & 63) == 0) *reinterpret_cast<uint32_t*>(scale + ((long long)kq * rows + r) * 4) = w;
+    for (int p = 0; p < U; ++p) {
+      const int kb = kq[p] * 4 + sub;
+      const int sb = fp8_scale_byte(max16(fp8_amax<8>(f[p])));            // (a block behind the last column: zeros, 127)
+      if (kb < nkb) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r[p]) * 128 + l * 8) = fp8_pack8(f[p], fp8_inv_scale(sb));
+      const uint32_t w = (uint32_t)__shfl(sb, 0, 64) | ((uint32_t)__shfl(sb, 16, 64) << 8) | ((uint32_t)__shfl(sb, 32, 64) << 16) |
+                         ((uint32_t)__shfl(sb, 48, 64) << 24);
+      if ((threadIdx.x & 63) == 0) *reinterpret_cast<uint32_t*>(scale + ((long long)kq[p] * rows + r[p]) * 4) = w;
+    }
   }
 }
 
@@ -137,13 +161,9 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   const int kb = (int)(c0 >> 7), kbt = (int)rb;
   int block_byte = 127;
   if constexpr (SQUARE) {
-    float m = 0.f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[u][e]));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    float m = max16(fp8_amax<64>(&f[0][0]));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
     if ((threadIdx.x & 63) == 0) s_wmax[threadIdx.x >> 6] = m;
     __syncthreads();
     block_byte = fp8_scale_byte(fmaxf(fmaxf(s_wmax[0], s_wmax[1]), fmaxf(s_wmax[2], s_wmax[3])));
@@ -153,23 +173,18 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
     }
   }
   if (q != nullptr) {
+    int mine = 127;                              // lane cv of the 16 that share a row's block stores the scale of row cv of eight
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const long long r = r0 + rl * 8 + u;
       int sb = block_byte;
       if constexpr (!SQUARE) {
-        float m = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[u][e]));
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-        sb = fp8_scale_byte(m);
+        sb = fp8_scale_byte(max16(fp8_amax<8>(f[u])));
+        mine = cv == u ? sb : mine;
       }
-      if (r < rows) {
-        *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + cv * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
-        if (!SQUARE && cv == 0) put_scale(scale, r, rows, kb, nkb, sb);
-      }
+      if (r < rows) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + cv * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
     }
+    if (!SQUARE && cv < 8 && r0 + rl * 8 + cv < rows) put_scale(scale, r0 + rl * 8 + cv, rows, kb, nkb, mine);
   }
   if (colsum != nullptr) {
 #pragma unroll
@@ -192,10 +207,8 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   if constexpr (!SQUARE) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float m = 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) m = fmaxf(m, fp8_abs_finite(f[u][e]));
-      s_red[rl][cv * 8 + e] = m;
+      const float t[8] = {f[0][e], f[1][e], f[2][e], f[3][e], f[4][e], f[5][e], f[6][e], f[7][e]};
+      s_red[rl][cv * 8 + e] = fp8_amax<8>(t);
     }
     __syncthreads();
     if (threadIdx.x < 128) {
@@ -228,16 +241,16 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
 
 // ------------------------------------------------------------------------------------------------ column sums
 // out[c] = sum over the row blocks of part[block][c], f64, a fixed order
-__global__ __launch_bounds__(256) void col_sum_finish_kernel(const float* __restrict__ part, int nb, int cols, float* __restrict__ out) {
-  __shared__ double sh[8][32];
+__global__ __launch_bounds__(1024) void col_sum_finish_kernel(const float* __restrict__ part, int nb, int cols, float* __restrict__ out) {
+  __shared__ double sh[32][33];
   const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   double s = 0.0;
   if (c < cols)
-    for (int i = sl; i < nb; i += 8) s += (double)part[(long long)i * cols + c];
+    for (int i = sl; i < nb; i += 32) s += (double)part[(long long)i * cols + c];
   sh[sl][cl] = s;
   __syncthreads();
   if (sl == 0 && c < cols) {
-    for (int k = 1; k < 8; ++k) s += sh[k][cl];
+    for (int k = 1; k < 32; ++k) s += sh[k][cl];
     out[c] = (float)s;
   }
 }
@@ -542,7 +555,7 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
   });
 }
 
-// A handful of activation rows (16 MT per block): the weights are what has to be read, and they are read once, straight into registers.
+// A handful of activation rows (16 MT at most): the weights are what has to be read, and they are read once, straight into registers.
 // A block takes 16 weight rows, its 16 waves every 16th K block; a lane holds 32 neighbouring codes of one row (the four MFMAs of a
 // block share that order of k for both operands).  SRC: sm_dtype of x, which is then quantised on the way -- no launch and no buffer
 // for it -- or 3 for codes.  The waves' sums meet in LDS in wave order.
@@ -552,7 +565,7 @@ __global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const 
   __shared__ __attribute__((aligned(16))) float s_acc[WAVES][MT][64][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
-  const long long m0 = (long long)blockIdx.y * (16 * MT);
+  constexpr long long m0 = 0;
   const int n = std::min(n0 + r, a.n - 1);
   long long row[MT];
 #pragma unroll
@@ -579,13 +592,10 @@ __global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const 
       } else {
         typedef typename Elem<SRC>::type T;
         const T* px = (const T*)xv + row[t] * ldx;
-        float f[4][8], m = 0.f;
+        float f[4][8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          fp8_load8<SRC, VEC>(px, (long long)kb * 128 + g * 32 + q * 8, cols, f[q]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) m = fmaxf(m, fp8_abs_finite(f[q][e]));
-        }
+        for (int q = 0; q < 4; ++q) fp8_load8<SRC, VEC>(px, (long long)kb * 128 + g * 32 + q * 8, cols, f[q]);
+        float m = fp8_amax<32>(&f[0][0]);
         m = fmaxf(m, __shfl_xor(m, 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const int sb = fp8_scale_byte(m);
@@ -647,7 +657,9 @@ struct MmPlan {
 // 256 x 256 tiles (a wave widens 3 pairs of codes per MFMA, one block fills a CU and nothing covers its epilogue) when they fill the chip
 // and K is long, 128 x 128 (4 pairs per MFMA, two blocks per CU) else: 230 against 245 us at 8192 x 4096 x 4096, but 91 against 74 us at
 // 67200 x 512 x 768.  K is split while there are fewer than two small tiles per CU and every split keeps four blocks of 128.
-constexpr int MM_FEW = 64;
+// Up to MM_FEW_QUANT rows the few-rows kernel quantises x itself, in every block again (15 us a call of 7 x 4096 x 4096 either way on
+// the host, but one launch instead of two); with 64 rows that repeated work took 28 us against 10 behind a quantiser launch.
+constexpr int MM_FEW = 64, MM_FEW_QUANT = 16;
 int mm_plan(const sm_fp8_matmul_desc* d, MmPlan* p) {
   if (d == nullptr) return SM_ERR_BAD_ARG;
   if (d->m < 0 || d->n < 1 || d->k < 1) return SM_ERR_BAD_SHAPE;
@@ -694,7 +706,7 @@ int fp8_quant_launch(const QuantArgs& a, hipStream_t s) {
   const bool vec = ((uintptr_t)a.x & 15) == 0 && a.ldx % per16 == 0 && (!a.gate || (((uintptr_t)a.gate & 15) == 0 && a.ldg % per16 == 0));
   const int nkb = sm_cdiv(a.cols, 128);
   if (!a.square && !a.qt && !a.colsum && !a.gate) {    // rows alone: no tile, no LDS
-    const unsigned blocks = (unsigned)std::min<long long>((a.rows * ((nkb + 3) / 4) + 3) / 4, 256 * 32);
+    const unsigned blocks = (unsigned)std::min<long long>((a.rows * ((nkb + 3) / 4) + 3) / 4, 256 * 8);
     if (vec) hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, (const T*)a.x, a.rows, a.cols, a.ldx, nkb, a.q, a.scale);
     else hipLaunchKernelGGL((fp8_quant_rows_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, (const T*)a.x, a.rows, a.cols, a.ldx, nkb, a.q, a.scale);
     SM_LAUNCH_CHECK();
@@ -751,7 +763,7 @@ extern "C" int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t c
                        (uint8_t*)scale_t, col_sum ? (float*)workspace : nullptr};
   const int st = fp8_quant_run(dtype, a, s);
   if (st != SM_OK || !col_sum) return st;
-  hipLaunchKernelGGL(col_sum_finish_kernel, dim3(sm_cdiv(cols, 32)), dim3(256), 0, s, (const float*)workspace, sm_cdiv(rows, 128), (int)cols, col_sum);
+  hipLaunchKernelGGL(col_sum_finish_kernel, dim3(sm_cdiv(cols, 32)), dim3(1024), 0, s, (const float*)workspace, sm_cdiv(rows, 128), (int)cols, col_sum);
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
@@ -766,10 +778,7 @@ extern "C" int64_t sm_fp8_matmul_workspace(const sm_fp8_matmul_desc* d) {
 namespace {
 template <int SRC, bool VEC>
 void mm_few_launch(const MmArgs& k, const void* x, long long ldx, long long cols, hipStream_t s) {
-  if (k.m <= 16)
-    hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 1>), dim3(sm_cdiv(k.n, 16), 1), dim3(1024), 0, s, k, x, ldx, cols);
-  else
-    hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 4>), dim3(sm_cdiv(k.n, 16), sm_cdiv(k.m, 64)), dim3(1024), 0, s, k, x, ldx, cols);
+  hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 1>), dim3(sm_cdiv(k.n, 16)), dim3(1024), 0, s, k, x, ldx, cols);
 }
 
 // the product behind its checks.  x != null: a is quantised from it (x_dtype, row stride ldx) -- by the few-rows kernel itself, else into
@@ -787,9 +796,19 @@ int mm_run(const sm_fp8_matmul_desc* d, const MmPlan& p, const void* a, const vo
   const int per16 = 16 / sm_dtype_bytes(d->out_dtype);
   k.vec = ((uintptr_t)y & 15) == 0 && d->y_stride % per16 == 0 && (!residual || (((uintptr_t)residual & 15) == 0 && d->res_stride % per16 == 0));
   k.tm = p.tm, k.tn = p.tn;
+  const bool on_the_way = x != nullptr && d->m <= MM_FEW_QUANT;
+  if (x != nullptr && !on_the_way) {
+    uint8_t* q = (uint8_t*)workspace + (p.ws + 15) / 16 * 16;
+    uint8_t* sc = q + sm_fp8_codes_bytes(d->m, d->k);
+    const QuantArgs qa = {x, nullptr, d->m, d->k, ldx, 0, 0, q, sc, nullptr, nullptr, nullptr};
+    const int st = fp8_quant_run(x_dtype, qa, s);
+    if (st != SM_OK) return st;
+    k.a = q, k.sa = sc;
+  }
   if (p.few) {
-    if (x == nullptr) {
-      mm_few_launch<3, true>(k, nullptr, 0, 0, s);
+    if (!on_the_way) {
+      if (k.m <= 16) mm_few_launch<3, true>(k, nullptr, 0, 0, s);
+      else hipLaunchKernelGGL((fp8_mm_few_kernel<3, true, 4>), dim3(sm_cdiv(k.n, 16)), dim3(1024), 0, s, k, nullptr, 0LL, 0LL);
     } else {
       const bool vec = ((uintptr_t)x & 15) == 0 && ldx % (16 / sm_dtype_bytes(x_dtype)) == 0;
       if (x_dtype == SM_DT_BF16) vec ? mm_few_launch<SM_DT_BF16, true>(k, x, ldx, d->k, s) : mm_few_launch<SM_DT_BF16, false>(k, x, ldx, d->k, s);
@@ -798,14 +817,6 @@ int mm_run(const sm_fp8_matmul_desc* d, const MmPlan& p, const void* a, const vo
     }
     SM_LAUNCH_CHECK();
     return SM_OK;
-  }
-  if (x != nullptr) {
-    uint8_t* q = (uint8_t*)workspace + (p.ws + 15) / 16 * 16;
-    uint8_t* sc = q + sm_fp8_codes_bytes(d->m, d->k);
-    const QuantArgs qa = {x, nullptr, d->m, d->k, ldx, 0, 0, q, sc, nullptr, nullptr, nullptr};
-    const int st = fp8_quant_run(x_dtype, qa, s);
-    if (st != SM_OK) return st;
-    k.a = q, k.sa = sc;
   }
   const dim3 grid((unsigned)(p.tm * p.tn), p.ksplit);
   if (p.big) {
@@ -832,7 +843,7 @@ int mm_check(const sm_fp8_matmul_desc* d, const void* b, const void* b_scale, co
 }
 
 int64_t linear_ws(const sm_fp8_matmul_desc* d, const MmPlan& p) {
-  return p.few ? 0 : (p.ws + 15) / 16 * 16 + sm_fp8_codes_bytes(d->m, d->k) + sm_fp8_scales_bytes(d->m, d->k, 1);
+  return d->m <= MM_FEW_QUANT ? 0 : (p.ws + 15) / 16 * 16 + sm_fp8_codes_bytes(d->m, d->k) + sm_fp8_scales_bytes(d->m, d->k, 1);
 }
 }  // namespace
 

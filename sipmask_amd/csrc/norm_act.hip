@@ -11,6 +11,9 @@
 // level).  The blocks leave partial sums in the workspace and the next launch adds them in a fixed order: no atomics, so the result
 // does not depend on which block came first, and there is nothing to clear between the replays of a captured graph.
 //
+// Maps of a few hundred rows take one launch instead (ga_small_*): a block holds all rows of its columns in registers, reads x (and dy)
+// once and needs no partials -- there the launches, not the bytes, are the time.
+//
 // The sums are held in f64: x and x^2 add exactly enough that E[x^2] - m^2 keeps its digits for |m| >> sqrt(v) (1e4 standard deviations
 // cost 1e-8), and three f64 operations per element stay under the memory time for 16-bit rows.
 #include <algorithm>
@@ -24,16 +27,13 @@ namespace {
 constexpr int GA_THREADS = 256;
 constexpr int GA_TILE = 32;         // column vectors per block: 512-byte row segments for 16-bit types
 constexpr int GA_TILE1 = 64;        // columns per block of the any-alignment path
-constexpr int GA_COMBINE = 2048;    // partial entries a block of the second launch may add up (32 KB out of L2)
-constexpr int GA_GPT = 256;         // groups that a column tile can touch (32 vectors of 8 channels, one channel per group)
 
 struct GaArgs {
   int nlev, batch, C, G, cpg, act;
   int cols, ct, lanes, ntile;       // column vectors, per block, row lanes of a block, column tiles
   long long hw[SM_MAX_LEVELS], row0[SM_MAX_LEVELS];
-  int sblk0[SM_MAX_LEVELS + 1];     // first split of each level (per image); partials of a level are hw / srpb apart
-  int ablk0[SM_MAX_LEVELS + 1];     // the same for the element-wise launch
-  int srpb[SM_MAX_LEVELS], arpb;    // rows per block
+  int blk0[SM_MAX_LEVELS + 1];      // first row block of each level (per image)
+  int rpb;                          // rows per block
   long long ldx, ldy, lddx;         // row strides in elements: x and dy, y, dx
   long long lddy;
   float eps;
@@ -66,7 +66,7 @@ __device__ __forceinline__ void lane_tree(V (*sh)[GA_THREADS], V (&v)[NV], int l
   }
 }
 
-// launch 1, forward: part[image][split][tile][group - first group of the tile] = (sum x, sum x^2)
+// launch 1, forward: part[image][row block][tile][group - first group of the tile] = (sum x, sum x^2)
 // WHOLE: a vector lies in one group (cpg % VEC == 0), so a thread needs two sums instead of 2 * VEC
 template <int DT, int VEC, bool WHOLE>
 __global__ __launch_bounds__(GA_THREADS) void ga_stats_kernel(const typename Elem<DT>::type* __restrict__ x, double2* __restrict__ part,
@@ -74,10 +74,10 @@ __global__ __launch_bounds__(GA_THREADS) void ga_stats_kernel(const typename Ele
   typedef RowVec<DT, VEC> RV;
   constexpr int NS = WHOLE ? 1 : VEC;
   __shared__ double sh[2 * NS][GA_THREADS];
-  const int nsplit = a.sblk0[a.nlev];
-  const int n = blockIdx.x / nsplit, b = blockIdx.x - n * nsplit, tile = blockIdx.y;
-  const int lev = ga_level(a.sblk0, a.nlev, b);
-  const long long rb = (long long)(b - a.sblk0[lev]) * a.srpb[lev], re = min(rb + (long long)a.srpb[lev], a.hw[lev]);
+  const int nblk = a.blk0[a.nlev];
+  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
+  const int lev = ga_level(a.blk0, a.nlev, b);
+  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
   const bool live = lane < a.lanes && col < a.cols;
   double v[2 * NS];
@@ -122,77 +122,87 @@ __global__ __launch_bounds__(GA_THREADS) void ga_stats_kernel(const typename Ele
   }
 }
 
-// (mean, rstd) of every group of this block's column tile from the partials, into LDS; the block that owns a (level, first row
-// block) also writes them out for the backward pass.  Threads share a group's entries and join in a fixed order.
-template <int VEC>
-__device__ __forceinline__ void ga_combine(const double2* __restrict__ part, double2* __restrict__ stats, double2* s_stat, double2* s_red,
-                                           const GaArgs& a, int gpt, int n, int lev, int tile, bool publish) {
-  const int tc = a.ct * VEC;
-  const int c0 = tile * tc, c1 = min(c0 + tc, a.C);
-  const int g0 = c0 / a.cpg, ng = (c1 - 1) / a.cpg - g0 + 1;
-  const int nsplit = a.sblk0[a.nlev], s0 = a.sblk0[lev], ns = a.sblk0[lev + 1] - s0;
-  int tpg = 1;                                   // threads per group, a power of two
-  while (tpg * 2 * ng <= GA_THREADS) tpg <<= 1;
-  const int gi = threadIdx.x / tpg, ti = threadIdx.x - gi * tpg;
+// launch 2, forward: one wave per (image, level, group) adds the group's partials: stats = (mean, rstd)
+__device__ __forceinline__ double2 ga_mean_rstd(double s, double ss, double cnt, float eps) {
+  const double m = s / cnt;
+  double var = ss / cnt - m * m;
+  var = var < 0.0 ? 0.0 : var;                   // (NaN stays NaN)
+  return make_double2(m, 1.0 / sqrt(var + (double)eps));
+}
+__global__ __launch_bounds__(GA_THREADS) void ga_combine_kernel(const double2* __restrict__ part, double2* __restrict__ stats, const GaArgs a,
+                                                                int gpt, int tc) {
+  const long long i = (long long)blockIdx.x * (GA_THREADS / 64) + (threadIdx.x >> 6);
+  if (i >= (long long)a.batch * a.nlev * a.G) return;
+  const int lane = threadIdx.x & 63;
+  const int g = (int)(i % a.G), lev = (int)(i / a.G % a.nlev);
+  const long long n = i / ((long long)a.G * a.nlev);
+  const int b0 = a.blk0[lev], nb = a.blk0[lev + 1] - b0;
   double s = 0.0, ss = 0.0;
-  if (gi < ng) {
-    const int g = g0 + gi;
-    const int t0 = g * a.cpg / tc, t1 = ((g + 1) * a.cpg - 1) / tc;
-    for (int t = t0; t <= t1; ++t) {
-      const int slot = g - t * tc / a.cpg;
-      const double2* q = part + (((long long)n * nsplit + s0) * a.ntile + t) * gpt + slot;
-      for (int i = ti; i < ns; i += tpg) {
-        const double2 e = q[(long long)i * a.ntile * gpt];
-        s += e.x, ss += e.y;
-      }
-    }
-  }
-  s_red[threadIdx.x] = make_double2(s, ss);
-  __syncthreads();
-  if (gi < ng && ti == 0) {
-    for (int k = 1; k < tpg; ++k) {
-      const double2 e = s_red[threadIdx.x + k];
+  for (int t = g * a.cpg / tc; t <= ((g + 1) * a.cpg - 1) / tc; ++t) {
+    const double2* q = part + ((n * a.blk0[a.nlev] + b0) * a.ntile + t) * gpt + (g - t * tc / a.cpg);
+    for (int k = lane; k < nb; k += 64) {
+      const double2 e = q[(long long)k * a.ntile * gpt];
       s += e.x, ss += e.y;
     }
-    const double cnt = (double)a.hw[lev] * (double)a.cpg, m = s / cnt;
-    double var = ss / cnt - m * m;
-    var = var < 0.0 ? 0.0 : var;                 // (NaN stays NaN)
-    const double2 st = make_double2(m, 1.0 / sqrt(var + (double)a.eps));
-    s_stat[gi] = st;
-    const int g = g0 + gi;
-    if (publish && g * a.cpg >= c0) stats[((long long)n * a.nlev + lev) * a.G + g] = st;   // (the tile that a group starts in)
   }
-  __syncthreads();
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64), ss += __shfl_xor(ss, d, 64);
+  if (lane == 0) stats[i] = ga_mean_rstd(s, ss, (double)a.hw[lev] * (double)a.cpg, a.eps);
 }
 
-// launch 2, forward
-template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
-__global__ __launch_bounds__(GA_THREADS) void ga_apply_kernel(const typename Elem<DT>::type* __restrict__ x,
-                                                              typename Elem<DT>::type* __restrict__ y, const float* __restrict__ gamma,
-                                                              const float* __restrict__ beta, const double2* __restrict__ part,
-                                                              double2* __restrict__ stats, const GaArgs a, int gpt) {
-  typedef RowVec<DT, VEC> RV;
-  __shared__ double2 s_stat[GA_GPT], s_red[GA_THREADS];
-  const int nblk = a.ablk0[a.nlev];
-  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.ablk0, a.nlev, b);
-  ga_combine<VEC>(part, stats, s_stat, s_red, a, gpt, n, lev, tile, b == a.ablk0[lev] && stats != nullptr);
-  const long long rb = (long long)(b - a.ablk0[lev]) * a.arpb, re = min(rb + (long long)a.arpb, a.hw[lev]);
-  const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
-  if (lane >= a.lanes || col >= a.cols) return;
-  const int g0 = tile * a.ct * VEC / a.cpg;
-  constexpr int NS = WHOLE ? 1 : VEC;
-  float mh[NS], ml[NS], ga[VEC], be[VEC];     // the mean as a sum of two floats: x - m keeps its digits for |m| >> sqrt(v)
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const int c = col * VEC + e;
-    const double2 st = s_stat[c / a.cpg - g0];
+// what a thread of the forward element pass needs of its channels.  The mean is a sum of two floats: x - m keeps its digits for
+// |m| >> sqrt(v)
+template <int VEC, bool WHOLE>
+struct GaNorm {
+  static constexpr int NS = WHOLE ? 1 : VEC;
+  float mh[NS], ml[NS], ga[VEC], be[VEC];
+  __device__ __forceinline__ void set(int e, double2 st, float gamma, float beta) {
     if (!WHOLE || e == 0) {
       mh[WHOLE ? 0 : e] = (float)st.x;
       ml[WHOLE ? 0 : e] = (float)(st.x - (double)(float)st.x);
     }
-    ga[e] = (float)(st.y * (gamma != nullptr ? (double)gamma[c] : 1.0));
-    be[e] = beta != nullptr ? beta[c] : 0.f;
+    ga[e] = (float)(st.y * (double)gamma);
+    be[e] = beta;
+  }
+  template <int ACT, bool DROP>
+  __device__ __forceinline__ void apply(float (&f)[VEC], uint32_t keep, float scale) const {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int k = WHOLE ? 0 : e;
+      f[e] = act_fwd<ACT>(__builtin_fmaf((f[e] - mh[k]) - ml[k], ga[e], be[e]));
+      if constexpr (DROP) f[e] = (keep >> e) & 1u ? f[e] * scale : 0.f;
+    }
+  }
+};
+
+// keep bits of the VEC channels from column vector `col` of row `row`
+template <int VEC, bool DROP>
+__device__ __forceinline__ uint32_t ga_keep(const GaArgs& a, unsigned long long off, long long row, int col) {
+  if constexpr (!DROP) return 0xffu;
+  const unsigned long long i = (unsigned long long)row * a.C + (unsigned long long)col * VEC;
+  const uint32_t keep = drop_keep8(i >> 3, off, a.drop.seed, a.drop.thr);
+  return VEC == 1 ? keep >> (int)(i & 7) : keep;
+}
+
+// launch 3, forward
+template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
+__global__ __launch_bounds__(GA_THREADS) void ga_apply_kernel(const typename Elem<DT>::type* __restrict__ x,
+                                                              typename Elem<DT>::type* __restrict__ y, const float* __restrict__ gamma,
+                                                              const float* __restrict__ beta, const double2* __restrict__ stats,
+                                                              const GaArgs a) {
+  typedef RowVec<DT, VEC> RV;
+  const int nblk = a.blk0[a.nlev];
+  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
+  const int lev = ga_level(a.blk0, a.nlev, b);
+  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
+  const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
+  if (lane >= a.lanes || col >= a.cols) return;
+  GaNorm<VEC, WHOLE> nm;
+  const double2* st = stats + ((long long)n * a.nlev + lev) * a.G;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const int c = col * VEC + e;
+    nm.set(e, st[c / a.cpg], gamma != nullptr ? gamma[c] : 1.f, beta != nullptr ? beta[c] : 0.f);
   }
   const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
   const long long row_base = a.row0[lev] + (long long)n * a.hw[lev];
@@ -201,18 +211,7 @@ __global__ __launch_bounds__(GA_THREADS) void ga_apply_kernel(const typename Ele
   auto one = [&](const typename RV::raw& q, long long r) {
     float f[VEC];
     RV::unpack(q, f);
-    uint32_t keep = 0xffu;
-    if constexpr (DROP) {
-      const unsigned long long i = (unsigned long long)(row_base + r) * a.C + (unsigned long long)col * VEC;
-      keep = drop_keep8(i >> 3, off, a.drop.seed, a.drop.thr);
-      if constexpr (VEC == 1) keep >>= (int)(i & 7);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int k = WHOLE ? 0 : e;
-      f[e] = act_fwd<ACT>(__builtin_fmaf((f[e] - mh[k]) - ml[k], ga[e], be[e]));
-      if constexpr (DROP) f[e] = (keep >> e) & 1u ? f[e] * a.drop.scale : 0.f;
-    }
+    nm.template apply<ACT, DROP>(f, ga_keep<VEC, DROP>(a, off, row_base + r, col), a.drop.scale);
     RV::store(py + r * a.ldy, f);
   };
   long long r = rb + lane;
@@ -248,30 +247,44 @@ struct GaChan {
       be[e] = beta != nullptr ? beta[c] : 0.f;
     }
   }
-  // xhat and d = dy * keep / (1 - p) * act'(t) of one element
+  // xhat and d = dy * keep / (1 - p) * act'(t) of VEC elements
   template <int ACT, bool DROP>
-  __device__ __forceinline__ void grad(float x, float dy, int e, uint32_t keep, float scale, float& xh, float& d) const {
-    const int k = WHOLE ? 0 : e;
-    xh = ((x - mh[k]) - ml[k]) * rs[k];
-    d = dy;
-    if constexpr (DROP) d = (keep >> e) & 1u ? d * scale : 0.f;
-    if constexpr (ACT == SM_ACT_NONE) return;
-    float t = __builtin_fmaf(xh, ga[e], be[e]);
+  __device__ __forceinline__ void grad(const float (&x)[VEC], const float (&dy)[VEC], uint32_t keep, float scale, float (&xh)[VEC],
+                                       float (&d)[VEC]) const {
+    float t[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int k = WHOLE ? 0 : e;
+      xh[e] = ((x[e] - mh[k]) - ml[k]) * rs[k];
+      if constexpr (ACT != SM_ACT_NONE) t[e] = __builtin_fmaf(xh[e], ga[e], be[e]);
+      d[e] = dy[e];
+      if constexpr (DROP) d[e] = (keep >> e) & 1u ? d[e] * scale : 0.f;
+    }
     if constexpr (ACT == SM_ACT_RELU) {
       // the ReLU passes the whole gradient or nothing: within rounding of the border (t = xh * gamma + beta is off by at most
-      // 3 * 2^-24 (|xh gamma| + |beta|), and near 0 the two are alike) t is taken in f64
-      if (__builtin_fabsf(t) <= 1e-6f * __builtin_fabsf(be[e])) {
-        const double t64 = ((double)x - st[k].x) * st[k].y * (double)ga[e] + (double)be[e];
-        t = t64 > 0.0 ? 1.f : (t64 <= 0.0 ? -1.f : t);
+      // 3 * 2^-24 (|xh gamma| + |beta|), and near 0 the two are alike) t is taken in f64.  One test for the vector: its arm is entered
+      // by one in 10^4 and must not cost the others a branch per element.
+      float near = 1.f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) near = fminf(near, __builtin_fmaf(-1e-6f, __builtin_fabsf(be[e]), __builtin_fabsf(t[e])));
+      if (near <= 0.f) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const double2 s = st[WHOLE ? 0 : e];
+          const double t64 = ((double)x[e] - s.x) * s.y * (double)ga[e] + (double)be[e];
+          if (__builtin_fabsf(t[e]) <= 1e-6f * __builtin_fabsf(be[e])) t[e] = t64 > 0.0 ? 1.f : (t64 <= 0.0 ? -1.f : t[e]);
+        }
       }
-      d = t <= 0.f ? 0.f : d;
-    } else {
-      d *= act_grad<ACT>(t);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) d[e] = t[e] <= 0.f ? 0.f : d[e];
+    } else if constexpr (ACT != SM_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) d[e] *= act_grad<ACT>(t[e]);
     }
   }
 };
 
-// launch 1, backward: part[image][split][channel] = (sum d, sum d xhat) of the split's rows
+// launch 1, backward: part[image][row block][channel] = (sum d, sum d xhat) of the block's rows
 template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
 __global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename Elem<DT>::type* __restrict__ x,
                                                                 const typename Elem<DT>::type* __restrict__ dy,
@@ -280,10 +293,10 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename E
                                                                 const GaArgs a) {
   typedef RowVec<DT, VEC> RV;
   __shared__ float sh[2 * VEC][GA_THREADS];
-  const int nsplit = a.sblk0[a.nlev];
-  const int n = blockIdx.x / nsplit, b = blockIdx.x - n * nsplit, tile = blockIdx.y;
-  const int lev = ga_level(a.sblk0, a.nlev, b);
-  const long long rb = (long long)(b - a.sblk0[lev]) * a.srpb[lev], re = min(rb + (long long)a.srpb[lev], a.hw[lev]);
+  const int nblk = a.blk0[a.nlev];
+  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
+  const int lev = ga_level(a.blk0, a.nlev, b);
+  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
   const bool live = lane < a.lanes && col < a.cols;
   float v[2 * VEC];
@@ -300,18 +313,13 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename E
       float fx[VEC], fd[VEC];
       RV::unpack(qx, fx);
       RV::unpack(qd, fd);
-      uint32_t keep = 0xffu;
-      if constexpr (DROP) {
-        const unsigned long long i = (unsigned long long)(row_base + r) * a.C + (unsigned long long)col * VEC;
-        keep = drop_keep8(i >> 3, off, a.drop.seed, a.drop.thr);
-        if constexpr (VEC == 1) keep >>= (int)(i & 7);
-      }
+      const uint32_t keep = ga_keep<VEC, DROP>(a, off, row_base + r, col);
+      float xh[VEC], d[VEC];
+      ch.template grad<ACT, DROP>(fx, fd, keep, a.drop.scale, xh, d);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        float xh, d;
-        ch.template grad<ACT, DROP>(fx[e], fd[e], e, keep, a.drop.scale, xh, d);
-        v[e] += d;
-        v[VEC + e] = __builtin_fmaf(d, xh, v[VEC + e]);
+        v[e] += d[e];
+        v[VEC + e] = __builtin_fmaf(d[e], xh[e], v[VEC + e]);
       }
     };
     long long r = rb + lane;
@@ -331,13 +339,14 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename E
 }
 
 // launch 2, backward: per (image, level) the channel sums chan[c] = (sum d, sum d xhat) and the group means
-// gmean[g] = (mean d gamma, mean d gamma xhat).  A block takes gb whole groups, 32 channels x 8 slices of the splits at a time.
-__global__ __launch_bounds__(GA_THREADS) void ga_bwd_combine_kernel(const float2* __restrict__ part, const float* __restrict__ gamma,
+// gmean[g] = (mean d gamma, mean d gamma xhat).  A block takes gb whole groups, 32 channels x 32 slices of the
+// row blocks at a time.
+__global__ __launch_bounds__(1024) void ga_bwd_combine_kernel(const float2* __restrict__ part, const float* __restrict__ gamma,
                                                                     double2* __restrict__ chan, double2* __restrict__ gmean, const GaArgs a,
                                                                     int gb) {
-  __shared__ double2 sh[8][32];
+  __shared__ double2 sh[32][33];
   const int nl = blockIdx.x, n = nl / a.nlev, lev = nl - n * a.nlev;
-  const int nsplit = a.sblk0[a.nlev], s0 = a.sblk0[lev], ns = a.sblk0[lev + 1] - s0;
+  const int nblk = a.blk0[a.nlev], s0 = a.blk0[lev], ns = a.blk0[lev + 1] - s0;
   const int g0 = blockIdx.y * gb, g1 = min(g0 + gb, a.G);
   const int ci = threadIdx.x & 31, sl = threadIdx.x >> 5;
   const double cnt = (double)a.hw[lev] * (double)a.cpg;
@@ -345,20 +354,20 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_combine_kernel(const float2
     const int c = c0 + ci;
     double s = 0.0, ss = 0.0;
     if (c < g1 * a.cpg)
-      for (int i = sl; i < ns; i += 8) {
-        const float2 e = part[((long long)n * nsplit + s0 + i) * a.C + c];
+      for (int i = sl; i < ns; i += 32) {
+        const float2 e = part[((long long)n * nblk + s0 + i) * a.C + c];
         s += (double)e.x, ss += (double)e.y;
       }
     __syncthreads();
     sh[sl][ci] = make_double2(s, ss);
     __syncthreads();
     if (sl == 0 && c < g1 * a.cpg) {
-      for (int k = 1; k < 8; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
+      for (int k = 1; k < 32; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
       chan[(long long)nl * a.C + c] = make_double2(s, ss);
     }
   }
   __syncthreads();                               // (the block's own global writes are visible to it behind the barrier)
-  for (int g = g0 + threadIdx.x; g < g1; g += GA_THREADS) {
+  for (int g = g0 + threadIdx.x; g < g1; g += 1024) {
     double m1 = 0.0, m2 = 0.0;
     for (int c = g * a.cpg; c < (g + 1) * a.cpg; ++c) {
       const double2 e = chan[(long long)nl * a.C + c];
@@ -367,6 +376,30 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_combine_kernel(const float2
     }
     gmean[(long long)nl * a.G + g] = make_double2(m1 / cnt, m2 / cnt);
   }
+}
+
+// dgamma / dbeta of 32 channels: the channel sums over images and levels, 8 slices joined in order
+__device__ __forceinline__ void ga_param_grads(double2 (*sh)[32], const double2* __restrict__ chan, float* __restrict__ dgamma,
+                                               float* __restrict__ dbeta, const GaArgs& a, int cblock) {
+  const int ci = threadIdx.x & 31, sl = threadIdx.x >> 5, c = cblock * 32 + ci;
+  double s = 0.0, ss = 0.0;
+  if (c < a.C)
+    for (int i = sl; i < a.batch * a.nlev; i += 8) {
+      const double2 e = chan[(long long)i * a.C + c];
+      s += e.x, ss += e.y;
+    }
+  sh[sl][ci] = make_double2(s, ss);
+  __syncthreads();
+  if (sl == 0 && c < a.C) {
+    for (int k = 1; k < 8; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
+    if (dbeta != nullptr) dbeta[c] = (float)s;
+    if (dgamma != nullptr) dgamma[c] = (float)ss;
+  }
+}
+__global__ __launch_bounds__(GA_THREADS) void ga_param_grads_kernel(const double2* __restrict__ chan, float* __restrict__ dgamma,
+                                                                    float* __restrict__ dbeta, const GaArgs a) {
+  __shared__ double2 sh[8][32];
+  ga_param_grads(sh, chan, dgamma, dbeta, a, blockIdx.x);
 }
 
 // launch 3, backward: dx element by element; the blocks behind the last row block add up dgamma / dbeta over images and levels
@@ -381,28 +414,13 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_apply_kernel(const typename
   typedef RowVec<DT, VEC> RV;
   __shared__ double2 sh[8][32];
   if ((long long)blockIdx.x >= nrow_blocks) {
-    if (blockIdx.y != 0) return;
-    const int ci = threadIdx.x & 31, sl = threadIdx.x >> 5;
-    const int c = (int)(blockIdx.x - nrow_blocks) * 32 + ci;
-    double s = 0.0, ss = 0.0;
-    if (c < a.C)
-      for (int i = sl; i < a.batch * a.nlev; i += 8) {
-        const double2 e = chan[(long long)i * a.C + c];
-        s += e.x, ss += e.y;
-      }
-    sh[sl][ci] = make_double2(s, ss);
-    __syncthreads();
-    if (sl == 0 && c < a.C) {
-      for (int k = 1; k < 8; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
-      if (dbeta != nullptr) dbeta[c] = (float)s;
-      if (dgamma != nullptr) dgamma[c] = (float)ss;
-    }
+    if (blockIdx.y == 0) ga_param_grads(sh, chan, dgamma, dbeta, a, (int)(blockIdx.x - nrow_blocks));
     return;
   }
-  const int nblk = a.ablk0[a.nlev];
+  const int nblk = a.blk0[a.nlev];
   const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.ablk0, a.nlev, b);
-  const long long rb = (long long)(b - a.ablk0[lev]) * a.arpb, re = min(rb + (long long)a.arpb, a.hw[lev]);
+  const int lev = ga_level(a.blk0, a.nlev, b);
+  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
   if (lane >= a.lanes || col >= a.cols) return;
   GaChan<VEC, WHOLE> ch;
@@ -424,18 +442,13 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_apply_kernel(const typename
     float fx[VEC], fd[VEC];
     RV::unpack(qx, fx);
     RV::unpack(qd, fd);
-    uint32_t keep = 0xffu;
-    if constexpr (DROP) {
-      const unsigned long long i = (unsigned long long)(row_base + r) * a.C + (unsigned long long)col * VEC;
-      keep = drop_keep8(i >> 3, off, a.drop.seed, a.drop.thr);
-      if constexpr (VEC == 1) keep >>= (int)(i & 7);
-    }
+    const uint32_t keep = ga_keep<VEC, DROP>(a, off, row_base + r, col);
+    float xh[VEC], d[VEC];
+    ch.template grad<ACT, DROP>(fx, fd, keep, a.drop.scale, xh, d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const int k = WHOLE ? 0 : e;
-      float xh, d;
-      ch.template grad<ACT, DROP>(fx[e], fd[e], e, keep, a.drop.scale, xh, d);
-      fx[e] = ch.rs[k] * (__builtin_fmaf(d, ch.ga[e], -m1[k]) - xh * m2[k]);
+      fx[e] = ch.rs[k] * (__builtin_fmaf(d[e], ch.ga[e], -m1[k]) - xh[e] * m2[k]);
     }
     RV::store(po + r * a.lddx, fx);
   };
@@ -450,12 +463,213 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_apply_kernel(const typename
   for (; r < re; r += a.lanes) one(RV::load(px + r * a.ldx), RV::load(pd + r * a.lddy), r);
 }
 
+// ------------------------------------------------------------------------------------------------ small maps: one launch
+constexpr int GA_SMALL = 1024;                   // threads
+// rows per thread that are kept in registers: 16 (f32: 32) bytes each; 1024 threads have 128 registers
+template <int DT>
+constexpr int ga_small_rows = DT == SM_DT_F32 ? 2 : 4;
+
+// channel sums sh[0 / 1][channel] of a block that owns whole groups -> weighted group sums
+template <int VEC, typename F>
+__device__ __forceinline__ void ga_small_groups(double (*sh)[GA_SMALL / 4], double2* s_grp, int c0, int nc, int cpg, const F& weight) {
+  for (int g = threadIdx.x; g * cpg < nc; g += GA_SMALL) {
+    double s = 0.0, ss = 0.0;
+    for (int c = g * cpg; c < (g + 1) * cpg; ++c) {
+      const double w = weight(c0 + c);
+      s += w * sh[0][c], ss += w * sh[1][c];
+    }
+    s_grp[g] = make_double2(s, ss);
+  }
+  __syncthreads();
+}
+
+// sum over the row lanes of the block: NV values per thread of each of VEC channels -> out[k][channel of the tile].  Waves first (the
+// lanes of a wave that share a column), then the waves in order.
+template <int VEC, typename V>
+__device__ __forceinline__ void ga_small_reduce(V (*red)[32 * VEC], double (*out)[GA_SMALL / 4], V (&a0)[VEC], V (&a1)[VEC], int ct) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    V(&v)[VEC] = q == 0 ? a0 : a1;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      for (int d = ct; d < 64; d <<= 1) v[e] += __shfl_xor(v[e], d, 64);
+    __syncthreads();                             // (the loop before this one has read red)
+    if (lane < ct) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) red[wave][lane * VEC + e] = v[e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < ct * VEC; c += GA_SMALL) {
+      double t = 0.0;
+#pragma unroll
+      for (int w = 0; w < GA_SMALL / 64; ++w) t += (double)red[w][c];
+      out[q][c] = t;
+    }
+  }
+  __syncthreads();
+}
+
+// grid (image, level) x column tile of whole groups, groups of whole vectors; ct (columns per tile) is a power of two of at most 32
+template <int DT, int ACT, bool DROP>
+__global__ __launch_bounds__(GA_SMALL) void ga_small_kernel(const typename Elem<DT>::type* __restrict__ x, typename Elem<DT>::type* __restrict__ y,
+                                                            const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                            double2* __restrict__ stats, const GaArgs a, int ct) {
+  typedef RowVec<DT, 8> RV;
+  constexpr int NR = ga_small_rows<DT>;
+  __shared__ double2 s_red[GA_SMALL / 64][32], s_grp[32];
+  const int lev = blockIdx.x % a.nlev, n = blockIdx.x / a.nlev, hw = (int)a.hw[lev];
+  if (hw == 0) return;
+  const int cl = threadIdx.x & (ct - 1), lane = threadIdx.x / ct, lanes = GA_SMALL / ct, col = blockIdx.y * ct + cl;
+  const int c0 = blockIdx.y * ct * 8, nc = min(ct * 8, a.C - c0);
+  const bool live = col < a.cols;
+  const long long row_base = a.row0[lev] + (long long)n * hw;
+  const typename Elem<DT>::type* px = x + row_base * a.ldx + (long long)col * 8;
+  typename RV::raw q[NR];
+  double s = 0.0, ss = 0.0;                      // (a vector lies in one group)
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    if (live && r < hw) q[u] = RV::load(px + (long long)r * a.ldx);
+  }
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    if (live && r < hw) {
+      float f[8];
+      RV::unpack(q[u], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double d = (double)f[e];
+        s += d, ss = __builtin_fma(d, d, ss);
+      }
+    }
+  }
+  // the row lanes of a wave, then waves x columns of the group, in order
+  for (int d = ct; d < 64; d <<= 1) s += __shfl_xor(s, d, 64), ss += __shfl_xor(ss, d, 64);
+  if ((threadIdx.x & 63) < ct) s_red[threadIdx.x >> 6][threadIdx.x & 63] = make_double2(s, ss);
+  __syncthreads();
+  const int gcols = a.cpg / 8;
+  for (int g = threadIdx.x; g * a.cpg < nc; g += GA_SMALL) {
+    double t = 0.0, tt = 0.0;
+    for (int k = g * gcols; k < (g + 1) * gcols; ++k)
+#pragma unroll
+      for (int w = 0; w < GA_SMALL / 64; ++w) t += s_red[w][k].x, tt += s_red[w][k].y;
+    const double2 st = ga_mean_rstd(t, tt, (double)hw * (double)a.cpg, a.eps);
+    s_grp[g] = st;
+    if (stats != nullptr) stats[(long long)blockIdx.x * a.G + c0 / a.cpg + g] = st;
+  }
+  __syncthreads();
+  if (!live) return;
+  GaNorm<8, true> nm;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int c = col * 8 + e;
+    nm.set(e, s_grp[(c - c0) / a.cpg], gamma != nullptr ? gamma[c] : 1.f, beta != nullptr ? beta[c] : 0.f);
+  }
+  const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
+  typename Elem<DT>::type* py = y + row_base * a.ldy + (long long)col * 8;
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    if (r < hw) {
+      float f[8];
+      RV::unpack(q[u], f);
+      nm.template apply<ACT, DROP>(f, ga_keep<8, DROP>(a, off, row_base + r, col), a.drop.scale);
+      RV::store(py + (long long)r * a.ldy, f);
+    }
+  }
+}
+
+// backward: dx (may be null) and the channel sums chan[image, level][channel] = (sum d, sum d xhat); of one (image, level) the sums are
+// the parameters' gradients themselves
+template <int DT, int ACT, bool DROP>
+__global__ __launch_bounds__(GA_SMALL) void ga_small_bwd_kernel(const typename Elem<DT>::type* __restrict__ x,
+                                                                const typename Elem<DT>::type* __restrict__ dy,
+                                                                const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                const double2* __restrict__ stats, typename Elem<DT>::type* __restrict__ dx,
+                                                                double2* __restrict__ chan, float* __restrict__ dgamma,
+                                                                float* __restrict__ dbeta, const GaArgs a, int ct) {
+  typedef RowVec<DT, 8> RV;
+  constexpr int NR = ga_small_rows<DT>;
+  __shared__ float s_red[GA_SMALL / 64][32 * 8];
+  __shared__ double s_chan[2][GA_SMALL / 4];
+  __shared__ double2 s_grp[GA_SMALL / 4];
+  const int lev = blockIdx.x % a.nlev, n = blockIdx.x / a.nlev, hw = (int)a.hw[lev];
+  const int cl = threadIdx.x & (ct - 1), lane = threadIdx.x / ct, lanes = GA_SMALL / ct, col = blockIdx.y * ct + cl;
+  const int c0 = blockIdx.y * ct * 8, nc = min(ct * 8, a.C - c0);
+  if (hw == 0) {                                 // an empty level adds nothing to the parameters' gradients
+    if (chan != nullptr)
+      for (int c = threadIdx.x; c < nc; c += GA_SMALL) chan[(long long)blockIdx.x * a.C + c0 + c] = make_double2(0.0, 0.0);
+    return;
+  }
+  const bool live = col < a.cols;
+  const long long row_base = a.row0[lev] + (long long)n * hw;
+  const typename Elem<DT>::type* px = x + row_base * a.ldx + (long long)col * 8;
+  const typename Elem<DT>::type* pd = dy + row_base * a.lddy + (long long)col * 8;
+  typename RV::raw qx[NR], qd[NR];
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    if (live && r < hw) qx[u] = RV::load(px + (long long)r * a.ldx), qd[u] = RV::load(pd + (long long)r * a.lddy);
+  }
+  GaChan<8, true> ch;
+  if (live) ch.fill(a, stats, gamma, beta, (long long)blockIdx.x * a.G, col);
+  const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
+  uint32_t keep[NR];
+  float s[8], ss[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.f, ss[e] = 0.f;
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    keep[u] = 0xffu;
+    if (live && r < hw) {
+      keep[u] = ga_keep<8, DROP>(a, off, row_base + r, col);
+      float fx[8], fd[8];
+      RV::unpack(qx[u], fx);
+      RV::unpack(qd[u], fd);
+      float xh[8], d[8];
+      ch.template grad<ACT, DROP>(fx, fd, keep[u], a.drop.scale, xh, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += d[e], ss[e] = __builtin_fmaf(d[e], xh[e], ss[e]);
+    }
+  }
+  ga_small_reduce<8>(s_red, s_chan, s, ss, ct);
+  for (int c = threadIdx.x; c < nc; c += GA_SMALL) {
+    if (chan != nullptr) chan[(long long)blockIdx.x * a.C + c0 + c] = make_double2(s_chan[0][c], s_chan[1][c]);
+    if (dbeta != nullptr) dbeta[c0 + c] = (float)s_chan[0][c];
+    if (dgamma != nullptr) dgamma[c0 + c] = (float)s_chan[1][c];
+  }
+  if (dx == nullptr) return;
+  ga_small_groups<8>(s_chan, s_grp, c0, nc, a.cpg, [&](int c) { return gamma != nullptr ? (double)gamma[c] : 1.0; });
+  if (!live) return;
+  const double cnt = (double)hw * (double)a.cpg;
+  const double2 gs = s_grp[(col * 8 - c0) / a.cpg];
+  const float m1 = (float)(gs.x / cnt), m2 = (float)(gs.y / cnt);
+  typename Elem<DT>::type* po = dx + row_base * a.lddx + (long long)col * 8;
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    const int r = lane + u * lanes;
+    if (r < hw) {
+      float fx[8], fd[8];
+      RV::unpack(qx[u], fx);
+      RV::unpack(qd[u], fd);
+      float xh[8], d[8];
+      ch.template grad<ACT, DROP>(fx, fd, keep[u], a.drop.scale, xh, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) fx[e] = ch.rs[0] * (__builtin_fmaf(d[e], ch.ga[e], -m1) - xh[e] * m2);
+      RV::store(po + (long long)r * a.lddx, fx);
+    }
+  }
+}
+
 struct GaPlan {
   GaArgs a;
   bool vec, whole;
+  int small_ct;                     // > 0: the one-launch kernels, that many column vectors per block
   int gpt;                          // groups per column tile (slots of a partial)
-  long long items;                  // batch * splits of all levels
-  long long ablocks;                // row blocks of the element-wise launch
+  long long items;                  // batch * row blocks of all levels
   long long fwd_ws, bwd_ws;         // bytes
 };
 
@@ -483,44 +697,61 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, GaPlan* p) {
   a.ntile = sm_cdiv(a.cols, a.ct);
   if (a.ntile > 65535 || a.G > 65535 * 32) return SM_ERR_UNSUPPORTED;
   const int tc = a.ct * vec;
-  p->gpt = std::min(a.G, (tc - 1) / a.cpg + 2);
-  if (p->gpt > tc) p->gpt = tc;
-  // rows per block.  The second launch adds splits x tiles-of-a-group x groups-of-a-tile partials: at most GA_COMBINE of them
-  const long long tiles_per_group = (a.cpg - 1) / tc + 2;
-  const long long smax = std::max<long long>(4, std::min<long long>(256, GA_COMBINE / (tiles_per_group * p->gpt)));
-  long long sb = 0, ab = 0, hw_sum = 0;
-  for (int l = 0; l < d->nlev; ++l) hw_sum += d->hw[l] > 0 ? d->hw[l] : 0;
-  // element-wise blocks: about 2048 of them over the chip, between 8 and 32 rows per row lane
-  const long long want = hw_sum * (long long)a.batch * a.ntile / 2048;
-  a.arpb = (int)std::max<long long>(8 * a.lanes, std::min<long long>(32 * a.lanes, want));
+  p->gpt = std::min(std::min(a.G, (tc - 1) / a.cpg + 2), tc);
+  long long rows = 0, hw_max = 0;
   for (int l = 0; l < d->nlev; ++l) {
     if (d->hw[l] < 0 || d->row0[l] < 0) return SM_ERR_BAD_SHAPE;
     a.hw[l] = d->hw[l], a.row0[l] = d->row0[l];
-    const long long rpb = std::max<long long>((d->hw[l] + smax - 1) / smax, 4 * a.lanes);
-    if (rpb > 0x3fffffff) return SM_ERR_UNSUPPORTED;
-    a.srpb[l] = (int)rpb;
-    a.sblk0[l] = (int)sb, a.ablk0[l] = (int)ab;
-    sb += (d->hw[l] + rpb - 1) / rpb;
-    ab += (d->hw[l] + a.arpb - 1) / a.arpb;
-    if (ab > 0x7fffffff) return SM_ERR_UNSUPPORTED;
+    rows += d->hw[l], hw_max = std::max<long long>(hw_max, d->hw[l]);
   }
-  for (int l = d->nlev; l <= SM_MAX_LEVELS; ++l) a.sblk0[l] = (int)sb, a.ablk0[l] = (int)ab;
-  p->items = sb * a.batch, p->ablocks = ab * a.batch;
-  // (256 threads a block: a launch dimension holds fewer than 2^32 threads)
-  if (p->items > 0xfff000 || p->ablocks > 0xff0000 || (long long)a.batch * a.nlev > 0xfff000) return SM_ERR_UNSUPPORTED;
-  p->fwd_ws = p->items * a.ntile * p->gpt * 16;
+  // about 2048 blocks (8 per CU) of at least 4 rows per row lane
+  const long long rpb = std::max<long long>(4 * a.lanes, rows * a.batch / 2048 * a.ntile);
+  if (rpb > 0x3fffffff) return SM_ERR_UNSUPPORTED;
+  a.rpb = (int)rpb;
+  long long nb = 0;
+  for (int l = 0; l < d->nlev; ++l) {
+    a.blk0[l] = (int)nb;
+    nb += (d->hw[l] + rpb - 1) / rpb;
+    if (nb > 0x7fffffff) return SM_ERR_UNSUPPORTED;
+  }
+  for (int l = d->nlev; l <= SM_MAX_LEVELS; ++l) a.blk0[l] = (int)nb;
+  p->items = nb * a.batch;
   const long long nl = (long long)a.batch * a.nlev;
-  p->bwd_ws = (p->items * a.C * 8 + 15) / 16 * 16 + nl * a.C * 16 + nl * a.G * 16;
+  // (256 threads a block: a launch dimension holds fewer than 2^32 threads)
+  if (p->items > 0xfff000 || nl > 0x3ff000 || nl * a.G > 0x3ffc000) return SM_ERR_UNSUPPORTED;
+  // One launch when a block can hold every row of its columns: the columns of whole groups, 8 (128 bytes of a row for 16-bit types) or
+  // the next power of two that is a multiple of the group
+  p->small_ct = 0;
+  if (p->vec && p->whole) {
+    int ct = 8;
+    while (ct <= 32 && (ct * 8) % a.cpg != 0 && ct * 8 < a.C) ct <<= 1;
+    const int nr = d->dtype == SM_DT_F32 ? ga_small_rows<SM_DT_F32> : ga_small_rows<SM_DT_BF16>;
+    if (ct <= 32 && hw_max <= (long long)nr * (GA_SMALL / ct)) p->small_ct = ct;
+  }
+  p->fwd_ws = p->small_ct ? 0 : (p->items * a.ntile * p->gpt + nl * a.G) * 16;
+  p->bwd_ws = p->small_ct ? nl * a.C * 16 : (p->items * a.C * 8 + 15) / 16 * 16 + nl * a.C * 16 + nl * a.G * 16;
   return SM_OK;
 }
 
 template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
 int ga_fwd_launch(const GaPlan& p, const void* x, const float* gamma, const float* beta, void* y, void* stats, void* ws, hipStream_t s) {
   typedef typename Elem<DT>::type T;
-  hipLaunchKernelGGL((ga_stats_kernel<DT, VEC, WHOLE>), dim3((unsigned)p.items, p.a.ntile), dim3(GA_THREADS), 0, s, (const T*)x,
-                     (double2*)ws, p.a, p.gpt);
-  hipLaunchKernelGGL((ga_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.ablocks, p.a.ntile), dim3(GA_THREADS), 0, s,
-                     (const T*)x, (T*)y, gamma, beta, (const double2*)ws, (double2*)stats, p.a, p.gpt);
+  const GaArgs& a = p.a;
+  const long long nl = (long long)a.batch * a.nlev;
+  if constexpr (VEC == 8 && WHOLE) {
+    if (p.small_ct > 0) {
+      hipLaunchKernelGGL((ga_small_kernel<DT, ACT, DROP>), dim3((unsigned)nl, sm_cdiv(a.cols, p.small_ct)), dim3(GA_SMALL), 0, s,
+                         (const T*)x, (T*)y, gamma, beta, (double2*)stats, a, p.small_ct);
+      SM_LAUNCH_CHECK();
+      return SM_OK;
+    }
+  }
+  double2* part = (double2*)ws;
+  double2* st = stats != nullptr ? (double2*)stats : part + p.items * a.ntile * p.gpt;
+  hipLaunchKernelGGL((ga_stats_kernel<DT, VEC, WHOLE>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s, (const T*)x, part, a, p.gpt);
+  hipLaunchKernelGGL(ga_combine_kernel, dim3((unsigned)((nl * a.G + 3) / 4)), dim3(GA_THREADS), 0, s, part, st, a, p.gpt, a.ct * VEC);
+  hipLaunchKernelGGL((ga_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s, (const T*)x,
+                     (T*)y, gamma, beta, st, a);
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
@@ -531,14 +762,26 @@ int ga_bwd_launch(const GaPlan& p, const void* x, const void* dy, const float* g
   typedef typename Elem<DT>::type T;
   const GaArgs& a = p.a;
   const long long nl = (long long)a.batch * a.nlev;
+  const bool params = dgamma != nullptr || dbeta != nullptr;
+  if constexpr (VEC == 8 && WHOLE) {
+    if (p.small_ct > 0) {
+      double2* chan = nl > 1 && params ? (double2*)ws : nullptr;
+      hipLaunchKernelGGL((ga_small_bwd_kernel<DT, ACT, DROP>), dim3((unsigned)nl, sm_cdiv(a.cols, p.small_ct)), dim3(GA_SMALL), 0, s,
+                         (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, (T*)dx, chan, chan ? nullptr : dgamma,
+                         chan ? nullptr : dbeta, a, p.small_ct);
+      if (chan) hipLaunchKernelGGL(ga_param_grads_kernel, dim3(sm_cdiv(a.C, 32)), dim3(GA_THREADS), 0, s, chan, dgamma, dbeta, a);
+      SM_LAUNCH_CHECK();
+      return SM_OK;
+    }
+  }
   float2* part = (float2*)ws;
   double2* chan = (double2*)((char*)ws + (p.items * a.C * 8 + 15) / 16 * 16);
   double2* gmean = chan + nl * a.C;
   hipLaunchKernelGGL((ga_bwd_sum_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s,
                      (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, part, a);
   const int gb = std::max(1, 32 / a.cpg);
-  hipLaunchKernelGGL(ga_bwd_combine_kernel, dim3((unsigned)nl, sm_cdiv(a.G, gb)), dim3(GA_THREADS), 0, s, part, gamma, chan, gmean, a, gb);
-  const long long rowb = dx != nullptr ? p.ablocks : 0, chb = dgamma != nullptr || dbeta != nullptr ? sm_cdiv(a.C, 32) : 0;
+  hipLaunchKernelGGL(ga_bwd_combine_kernel, dim3((unsigned)nl, sm_cdiv(a.G, gb)), dim3(1024), 0, s, part, gamma, chan, gmean, a, gb);
+  const long long rowb = dx != nullptr ? p.items : 0, chb = params ? sm_cdiv(a.C, 32) : 0;
   if (rowb + chb > 0)
     hipLaunchKernelGGL((ga_bwd_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)(rowb + chb), a.ntile), dim3(GA_THREADS), 0, s,
                        (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, (const double2*)chan, (const double2*)gmean,
@@ -617,7 +860,7 @@ extern "C" int sm_group_norm_act(const sm_gn_act_desc* d, const void* x, const f
   const int st = ga_plan(d, al16(x) && al16(y), &p);
   if (st != SM_OK) return st;
   if (p.items == 0) return SM_OK;
-  if (!x || !y || !workspace || !al16(workspace) || (stats != nullptr && !al16(stats))) return SM_ERR_BAD_ARG;
+  if (!x || !y || (p.fwd_ws > 0 && !workspace) || !al16(workspace) || (stats != nullptr && !al16(stats))) return SM_ERR_BAD_ARG;
   if (workspace_bytes < p.fwd_ws) return SM_ERR_WORKSPACE;
   return ga_pick(p, d->dtype, GaFwd{p, x, gamma, beta, y, stats, workspace, sm_hip_stream(stream)});
 }
@@ -634,7 +877,7 @@ extern "C" int sm_group_norm_act_bwd(const sm_gn_act_desc* d, const void* x, con
     if (dbeta && sm_zero_async(dbeta, sizeof(float) * d->channels, s) != hipSuccess) return SM_ERR_LAUNCH;
     return SM_OK;
   }
-  if (!x || !dy || !stats || !al16(stats) || !workspace || !al16(workspace)) return SM_ERR_BAD_ARG;
+  if (!x || !dy || !stats || !al16(stats) || (p.bwd_ws > 0 && !workspace) || !al16(workspace)) return SM_ERR_BAD_ARG;
   if (workspace_bytes < p.bwd_ws) return SM_ERR_WORKSPACE;
   return ga_pick(p, d->dtype, GaBwd{p, x, dy, gamma, beta, stats, dx, dgamma, dbeta, workspace, s});
 }

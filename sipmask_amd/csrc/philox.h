@@ -27,7 +27,8 @@ __device__ __forceinline__ void philox10(unsigned long long idx8, unsigned long 
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const unsigned long long p0 = (unsigned long long)c[0] * 0xD2511F53u, p1 = (unsigned long long)c[2] * 0xCD9E8D57u;
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c[1] ^ k0, n2 = (uint32_t)(p0 >> 32) ^ c[3] ^ k1;
+    const uint32_t n0 = __builtin_amdgcn_bitop3_b32((uint32_t)(p1 >> 32), c[1], k0, 0x96);   // a ^ b ^ c in one instruction
+    const uint32_t n2 = __builtin_amdgcn_bitop3_b32((uint32_t)(p0 >> 32), c[3], k1, 0x96);
     c[1] = (uint32_t)p1, c[3] = (uint32_t)p0, c[0] = n0, c[2] = n2;
     k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
   }

@@ -1501,9 +1501,10 @@ def group_norm_act(d, x, gamma, beta, want_stats):
     lib = _lib.load()
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stats = torch.empty(d.batch * d.nlev * d.groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
-    ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 0), x.device, "sm_group_norm_act")
+    need = lib.sm_group_norm_act_workspace(C.byref(d), 0)
+    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_group_norm_act")
     _lib.check(lib.sm_group_norm_act(C.byref(d), _p(x), _p(gamma), _p(beta), _p(y), _p(stats),
-                                     _p(ws), ws.numel(), _stream(x)), "sm_group_norm_act")
+                                     _p(ws), 0 if ws is None else need, _stream(x)), "sm_group_norm_act")
     return y, stats
 
 
@@ -1512,10 +1513,11 @@ def group_norm_act_bwd(d, x, dy, gamma, beta, stats, need_dx=True, dgamma=None, 
     lib = _lib.load()
     d.dy_stride = row_stride(dy)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    ws = _workspace(lib.sm_group_norm_act_workspace(C.byref(d), 1), x.device, "sm_group_norm_act_bwd")
+    need = lib.sm_group_norm_act_workspace(C.byref(d), 1)
+    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_group_norm_act_bwd")
     _lib.check(lib.sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats),
-                                         _p(dx), _p(dgamma), _p(dbeta), _p(ws), ws.numel(),
-                                         _stream(x)), "sm_group_norm_act_bwd")
+                                         _p(dx), _p(dgamma), _p(dbeta), _p(ws), 0 if ws is None else need, _stream(x)),
+               "sm_group_norm_act_bwd")
     return dx
 
 

@@ -296,6 +296,28 @@ group_norm = GroupNormFunction.apply
 
 
 # ------------------------------------------------------------------------------- GroupNorm + activation, dropout
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _gn_act_forward(x, gamma, beta, lv, groups, eps, act, thr, seed, offset, want_stats):
+    """-> (y, descriptor, f32 gamma, f32 beta, stats, device offset)"""
+    g32 = None if gamma is None else gamma.detach().float().contiguous()
+    b32 = None if beta is None else beta.detach().float().contiguous()
+    off = H.dropout_offset(offset, x.device)
+    last = x.movedim(1, -1) if lv is None else x
+    rows = H.dense_rows(last, last.shape[-1])
+    if lv is None:
+        lv = H.Levels(x.shape[0], [(rows.shape[0] // max(x.shape[0], 1), 1)])
+        back = lambda y: y.view(last.shape).movedim(-1, 1)
+    else:
+        back = lambda y: y
+    with _lib.on_device(x):
+        d = H.group_norm_act_desc(rows, lv, groups, eps, act, thr, seed, off)
+        y, stats = H.group_norm_act(d, rows, g32, b32, want_stats)
+    return back(y), d, g32, b32, stats, off[1]
+
+
 class GroupNormActFunction(Function):
     """act(GroupNorm(x)) [dropped out] of channels-last values (sm_group_norm_act / _bwd): x [N, C, *] with lv None, or pyramid rows
     [lv.rows, C].  The backward recomputes the normalised values and the dropout mask; only x, the parameters and (mean, rstd) per
@@ -303,19 +325,10 @@ class GroupNormActFunction(Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, lv, groups, eps, act, thr, seed, offset):
-        g32 = None if gamma is None else gamma.detach().float().contiguous()
-        b32 = None if beta is None else beta.detach().float().contiguous()
-        host, dev = H.dropout_offset(offset, x.device)
-        last = x.movedim(1, -1) if lv is None else x
-        rows = H.dense_rows(last, last.shape[-1])
-        with _lib.on_device(x):
-            d = H.group_norm_act_desc(rows, lv if lv is not None else H.Levels(x.shape[0], [(rows.shape[0] // max(x.shape[0], 1), 1)]),
-                                      groups, eps, act, thr, seed, (host, dev))
-            y, stats = H.group_norm_act(d, rows, g32, b32, any(ctx.needs_input_grad))
-        if stats is not None:
-            ctx.save_for_backward(x, g32, b32, stats, dev)  # (dev: an offset that changed before the backward is an error)
-            ctx.cfg = (d, lv, None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
-        return y.view(last.shape).movedim(-1, 1) if lv is None else y
+        y, d, g32, b32, stats, dev = _gn_act_forward(x, gamma, beta, lv, groups, eps, act, thr, seed, offset, True)
+        ctx.save_for_backward(x, g32, b32, stats, dev)      # (dev: an offset that changed before the backward is an error)
+        ctx.cfg = (d, lv, None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -361,6 +374,12 @@ def _gn_act_args(x, channels, weight, bias, groups, eps, activation, dropout_p, 
     return H.ACTIVATIONS[activation], H.dropout_threshold(dropout_p)
 
 
+def _gn_act(x, gamma, beta, *args):
+    if not _wants_grad(x, gamma, beta):
+        return _gn_act_forward(x, gamma, beta, *args, False)[0]
+    return GroupNormActFunction.apply(x, gamma, beta, *args)
+
+
 def group_norm_act(x, weight, bias, num_groups, eps=1e-5, activation="relu", dropout_p=0.0, seed=0, offset=0):
     """act(F.group_norm(x, num_groups, weight, bias, eps)) on channels-last memory, optionally dropped out; differentiable in
     x, weight and bias.
@@ -373,7 +392,7 @@ def group_norm_act(x, weight, bias, num_groups, eps=1e-5, activation="relu", dro
         raise ValueError("group_norm_act: x is [N, C, *]")
     c = x.shape[1]
     act, thr = _gn_act_args(x, c, weight, bias, num_groups, eps, activation, dropout_p, "group_norm_act")
-    return GroupNormActFunction.apply(x, weight, bias, None, num_groups, eps, act, thr, seed, offset)
+    return _gn_act(x, weight, bias, None, num_groups, eps, act, thr, seed, offset)
 
 
 def _dropout_rows(x, residual, thr, seed, offset):
@@ -425,6 +444,8 @@ def dropout(x, p, seed, offset=0, residual=None, training=True):
         if residual is None:
             return x
         thr = 0
+    if not _wants_grad(x, residual):
+        return _dropout_rows(x, residual, thr, seed, H.dropout_offset(offset, x.device))
     return DropoutFunction.apply(x, residual, thr, seed, offset)
 
 
@@ -580,7 +601,13 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
         raise ValueError("linear_fp8: bias is [%d] on %s" % (n, x.device))
     if weight is None and torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("linear_fp8: a gradient of x needs the weight itself, not weight_q alone")
-    return LinearFp8Function.apply(x, weight, bias, relu, weight_q)
+    if _wants_grad(x, weight, bias):
+        return LinearFp8Function.apply(x, weight, bias, relu, weight_q)
+    rows = H.dense_rows(x, k)
+    with _lib.on_device(x):
+        wq = (weight_q.codes, weight_q.scales) if weight_q is not None else H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128)[0]
+        y = H.fp8_linear(rows, wq[0], wq[1], 128, None if bias is None else bias.detach().float().contiguous(), None, relu, x.dtype)
+    return y.view(x.shape[:-1] + (n,))
 
 
 class UpsampleBilinearFunction(Function):

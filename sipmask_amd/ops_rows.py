@@ -228,7 +228,7 @@ def gn_act_rows(x, lv, gamma, beta, groups=32, eps=1e-5, activation="relu", drop
     if len(lv) > _lib.SM_MAX_LEVELS:
         raise ValueError("gn_act_rows: at most %d levels" % _lib.SM_MAX_LEVELS)
     act, thr = P._gn_act_args(x, x.shape[1], gamma, beta, groups, eps, activation, dropout_p, "gn_act_rows")
-    return P.GroupNormActFunction.apply(x, gamma, beta, lv, groups, eps, act, thr, seed, offset)
+    return P._gn_act(x, gamma, beta, lv, groups, eps, act, thr, seed, offset)
 
 
 class DeformConvRowsFunction(Function):
