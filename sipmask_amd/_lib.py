@@ -220,7 +220,7 @@ PROTOTYPES = {
     "sm_fp8_matmul_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
     "sm_fp8_matmul": (_I, [C.POINTER(Fp8MatmulDesc), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "sm_fp8_linear_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
-    "sm_fp8_linear": (_I, [C.POINTER(Fp8MatmulDesc), _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_fp8_linear": (_I, [_P, _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
 }
 
 _lib = None

@@ -5,6 +5,7 @@ lives here so the error messages mirror the reference's Python-side checks
 (M/mmdet/ops/dcn/deform_conv.py:27-30,47,50-51; M/mmdet/ops/crop/src/crop_split_cuda.cpp:17).
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -1419,12 +1420,17 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}         # sm
 _MASK64 = (1 << 64) - 1
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
 def _stream(t):
     """the current stream of t's device, as the handle the C entry points take"""
+    if _raw_stream is not None:                  # (a stream object per call costs 2 us of host time, 12 in autograd's thread)
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -1475,114 +1481,123 @@ def dropout_offset(offset, device):
     return int(offset) & _MASK64, None
 
 
-def group_norm_act_desc(x, lv, groups, eps, act, thr, seed, offset):
-    """sm_gn_act_desc of rows x [lv.rows, C]; y, dy and dx are dense rows unless the caller sets their strides"""
+@functools.lru_cache(maxsize=512)
+def _gn_act_plan(batch, hw, channels, groups, dtype, act, eps, thr):
+    """(sm_gn_act_desc as bytes, forward and backward workspace) of a geometry; level l holds batch * hw[l] rows"""
+    lib = _lib.load()
     d = _lib.GnActDesc()
-    c = x.shape[1]
-    d.nlev, d.batch, d.channels, d.groups = len(lv), lv.batch, c, groups
-    d.dtype, d.act, d.eps, d.drop_threshold = dtype_code(x, "group_norm_act"), act, eps, thr
-    for l, (h, w) in enumerate(lv.sizes):
-        d.hw[l], d.row0[l] = h * w, lv.row0[l]
-    d.x_stride, d.y_stride, d.dy_stride, d.dx_stride = row_stride(x), c, c, c
-    host, dev = offset
-    d.drop_seed, d.drop_offset = int(seed) & _MASK64, host
-    d.drop_offset_dev = None if dev is None else dev.data_ptr()
-    return d
+    d.nlev, d.batch, d.channels, d.groups = len(hw), batch, channels, groups
+    d.dtype, d.act, d.eps, d.drop_threshold = dtype, act, eps, thr
+    r = 0
+    for l, n in enumerate(hw):
+        d.hw[l], d.row0[l] = n, r
+        r += batch * n
+    d.x_stride = d.y_stride = d.dy_stride = d.dx_stride = channels
+    need = [lib.sm_group_norm_act_workspace(C.byref(d), b) for b in (0, 1)]
+    if min(need) < 0:
+        _lib.check(int(min(need)), "sm_group_norm_act")
+    return bytes(d), need[0], need[1]
 
 
-def _workspace(need, device, what):
-    if need < 0:
-        _lib.check(int(need), what)
-    return torch.empty(need, dtype=torch.uint8, device=device)
+def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, seed, offset, gamma, beta, want_stats):
+    """x: channels-last values, rows x_stride elements apart; y: contiguous rows.  -> (descriptor, backward workspace bytes, stats f64
+    [batch * nlev * groups, 2] or None)"""
+    plan, need, bwd_need = _gn_act_plan(batch, hw, channels, groups, dtype_code(x, "group_norm_act"), act, eps, thr)
+    d = _lib.GnActDesc.from_buffer_copy(plan)
+    d.x_stride = x_stride
+    if thr:
+        d.drop_seed, d.drop_offset = int(seed) & _MASK64, offset[0]
+        d.drop_offset_dev = None if offset[1] is None else offset[1].data_ptr()
+    stats = torch.empty(batch * len(hw) * groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    _lib.check(_lib.load().sm_group_norm_act(C.byref(d), _p(x), _p(gamma), _p(beta), _p(y), _p(stats), _p(ws), need, _stream(x)),
+               "sm_group_norm_act")
+    return d, bwd_need, stats
 
 
-def group_norm_act(d, x, gamma, beta, want_stats):
-    """-> (y dense rows, stats f64 [batch * nlev * groups, 2] or None)"""
-    lib = _lib.load()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(d.batch * d.nlev * d.groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
-    need = lib.sm_group_norm_act_workspace(C.byref(d), 0)
-    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_group_norm_act")
-    _lib.check(lib.sm_group_norm_act(C.byref(d), _p(x), _p(gamma), _p(beta), _p(y), _p(stats),
-                                     _p(ws), 0 if ws is None else need, _stream(x)), "sm_group_norm_act")
-    return y, stats
+def group_norm_act_bwd(d, need, x, dy, dy_stride, dx, gamma, beta, stats, dgamma, dbeta):
+    """dx (contiguous rows) and dgamma / dbeta f32 [C] are written where given"""
+    d.dy_stride = dy_stride
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    _lib.check(_lib.load().sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats), _p(dx), _p(dgamma), _p(dbeta),
+                                                 _p(ws), need, _stream(x)), "sm_group_norm_act_bwd")
 
 
-def group_norm_act_bwd(d, x, dy, gamma, beta, stats, need_dx=True, dgamma=None, dbeta=None):
-    """-> dx dense rows or None; dgamma / dbeta f32 [C] buffers are written when given"""
-    lib = _lib.load()
-    d.dy_stride = row_stride(dy)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    need = lib.sm_group_norm_act_workspace(C.byref(d), 1)
-    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_group_norm_act_bwd")
-    _lib.check(lib.sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats),
-                                         _p(dx), _p(dgamma), _p(dbeta), _p(ws), 0 if ws is None else need, _stream(x)),
-               "sm_group_norm_act_bwd")
-    return dx
-
-
-def dropout_rows(x, residual, thr, seed, offset, y):
-    """x (and residual) [rows, cols] with dense rows -> y, contiguous"""
-    lib = _lib.load()
-    host, dev = offset
-    _lib.check(lib.sm_dropout(dtype_code(x, "dropout"), _p(x), _p(residual), _p(y), x.shape[0], x.shape[1],
-                              row_stride(x), 0 if residual is None else row_stride(residual), x.shape[1], thr,
-                              int(seed) & _MASK64, host, _p(dev), _stream(x)), "sm_dropout")
+def dropout_rows(x, residual, y, rows, cols, x_stride, res_stride, thr, seed, offset):
+    """rows x cols values, rows x_stride / res_stride elements apart -> y, contiguous"""
+    _lib.check(_lib.load().sm_dropout(DTYPE_CODES[x.dtype], _p(x), _p(residual), _p(y), rows, cols, x_stride, res_stride, cols, thr,
+                                      int(seed) & _MASK64, offset[0], _p(offset[1]), _stream(x)), "sm_dropout")
     return y
 
 
 # ------------------------------------------------------------------------------- 8-bit products
-def _fp8_alloc(r, c, block_rows, device):
-    """(codes e4m3 [ceil(c / 128), r, 128], scales uint8 [ceil(c / 512), ceil(r / block_rows), 4]) of an r x c matrix"""
-    return (torch.empty(-(-c // 128), r, 128, dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(-(-c // 512), -(-r // block_rows), 4, dtype=torch.uint8, device=device))
+def fp8_bytes(r, c, block_rows):
+    """bytes of the codes and of the scales of an r x c matrix (sm_fp8_codes_bytes, sm_fp8_scales_bytes)"""
+    return -(-c // 128) * r * 128, -(-c // 512) * -(-r // block_rows) * 4
+
+
+class Fp8Buffer:
+    """codes and scales of an r x c matrix in one uint8 tensor"""
+    __slots__ = ("data", "codes", "scales")
+
+    def __init__(self, r, c, block_rows, device=None, data=None):
+        nc, ns = fp8_bytes(r, c, block_rows)
+        self.data = torch.empty(nc + ns, dtype=torch.uint8, device=device) if data is None else data
+        self.codes = self.data.data_ptr()
+        self.scales = self.codes + nc
 
 
 def fp8_quantize(x, block_rows, rows=True, transpose=False, col_sum=False, gate=None):
-    """x (and gate) [r, c] with dense rows, read once -> ((codes, scales) or None, the transpose's (codes, scales) or None, f32 column
-    sums or None); gate: values whose gate is not > 0 count as 0"""
+    """x (and gate) [r, c] with dense rows, read once -> (Fp8Buffer or None, the transpose's or None, f32 column sums or None); gate:
+    values whose gate is not > 0 count as 0"""
     lib = _lib.load()
     r, c = x.shape
-    q, s = _fp8_alloc(r, c, block_rows, x.device) if rows else (None, None)
-    qt, st = _fp8_alloc(c, r, block_rows, x.device) if transpose else (None, None)
+    q = Fp8Buffer(r, c, block_rows, x.device) if rows else None
+    t = Fp8Buffer(c, r, block_rows, x.device) if transpose else None
     cs = ws = None
+    need = 0
     if col_sum:
         cs = torch.empty(c, dtype=torch.float32, device=x.device)
-        ws = _workspace(lib.sm_fp8_quantize_workspace(r, c, 1), x.device, "sm_fp8_quantize")
+        need = lib.sm_fp8_quantize_workspace(r, c, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.check(lib.sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _p(x), r, c, row_stride(x), block_rows, _p(gate),
-                                   0 if gate is None else row_stride(gate), _p(q), _p(s), _p(qt), _p(st), _p(cs), _p(ws),
-                                   0 if ws is None else ws.numel(), _stream(x)), "sm_fp8_quantize")
-    return (q, s) if rows else None, (qt, st) if transpose else None, cs
+                                   0 if gate is None else row_stride(gate), q and q.codes, q and q.scales, t and t.codes, t and t.scales,
+                                   _p(cs), _p(ws), need, _stream(x)), "sm_fp8_quantize")
+    return q, t, cs
 
 
-def _fp8_desc(m, n, k, a_block_rows, b_block_rows, out_dtype, relu, residual):
+@functools.lru_cache(maxsize=512)
+def _fp8_plan(m, n, k, a_block_rows, b_block_rows, out_dtype, relu):
+    """(sm_fp8_matmul_desc as bytes, workspace of sm_fp8_matmul, of sm_fp8_linear)"""
+    lib = _lib.load()
     d = _lib.Fp8MatmulDesc()
     d.m, d.n, d.k, d.a_block_rows, d.b_block_rows = m, n, k, a_block_rows, b_block_rows
-    d.out_dtype, d.relu, d.y_stride = DTYPE_CODES[out_dtype], int(relu), n
-    d.res_stride = 0 if residual is None else row_stride(residual)
-    return d
+    d.out_dtype, d.relu, d.y_stride = out_dtype, relu, n
+    need = lib.sm_fp8_matmul_workspace(C.byref(d)), lib.sm_fp8_linear_workspace(C.byref(d))
+    if min(need) < 0:
+        _lib.check(int(min(need)), "sm_fp8_matmul")
+    return bytes(d), need[0], need[1]
 
 
-def fp8_matmul(a, sa, a_block_rows, b, sb, b_block_rows, k, bias, residual, relu, out_dtype):
-    lib = _lib.load()
-    m, n = a.shape[1], b.shape[1]
-    d = _fp8_desc(m, n, k, a_block_rows, b_block_rows, out_dtype, relu, residual)
-    y = torch.empty(m, n, dtype=out_dtype, device=a.device)
-    need = lib.sm_fp8_matmul_workspace(C.byref(d))
-    ws = None if 0 <= need <= 16 else _workspace(need, a.device, "sm_fp8_matmul")
-    _lib.check(lib.sm_fp8_matmul(C.byref(d), _p(a), _p(sa), _p(b), _p(sb), _p(bias), _p(residual), _p(y), _p(ws),
-                                 0 if ws is None else need, _stream(a)), "sm_fp8_matmul")
+def fp8_matmul(a, a_block_rows, b, b_block_rows, m, n, k, bias, residual, relu, out_dtype, device):
+    """a, b: codes / scales as Fp8Buffer (or anything with these two addresses)"""
+    plan, need, _ = _fp8_plan(m, n, k, a_block_rows, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
+    d = _lib.Fp8MatmulDesc.from_buffer_copy(plan)
+    if residual is not None:
+        d.res_stride = row_stride(residual)
+    y = torch.empty(m, n, dtype=out_dtype, device=device)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 16 else None
+    _lib.check(_lib.load().sm_fp8_matmul(C.byref(d), a.codes, a.scales, b.codes, b.scales, _p(bias), _p(residual), _p(y), _p(ws), need,
+                                         _stream(y)), "sm_fp8_matmul")
     return y
 
 
-def fp8_linear(x, b, sb, b_block_rows, bias, residual, relu, out_dtype):
+def fp8_linear(x, b, b_block_rows, n, bias, relu, out_dtype):
     """x [m, k] with dense rows, quantised on the way, times the codes b"""
-    lib = _lib.load()
-    (m, k), n = x.shape, b.shape[1]
-    d = _fp8_desc(m, n, k, 1, b_block_rows, out_dtype, relu, residual)
+    m, k = x.shape
+    plan, _, need = _fp8_plan(m, n, k, 1, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
     y = torch.empty(m, n, dtype=out_dtype, device=x.device)
-    need = lib.sm_fp8_linear_workspace(C.byref(d))
-    ws = None if 0 <= need <= 16 else _workspace(need, x.device, "sm_fp8_linear")
-    _lib.check(lib.sm_fp8_linear(C.byref(d), dtype_code(x, "linear_fp8"), _p(x), row_stride(x), _p(b), _p(sb), _p(bias), _p(residual),
-                                 _p(y), _p(ws), 0 if ws is None else need, _stream(x)), "sm_fp8_linear")
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    _lib.check(_lib.load().sm_fp8_linear(plan, dtype_code(x, "linear_fp8"), _p(x), row_stride(x), b.codes, b.scales, _p(bias), None, _p(y),
+                                         _p(ws), need, _stream(x)), "sm_fp8_linear")
     return y

@@ -300,22 +300,45 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _channels_last_rows(t):
+    """[N, C, *] -> (a tensor whose storage starts with the rows, elements between the rows); no copy and no view for channels-last
+    4-D memory"""
+    if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return t, t.shape[1]
+    r = H.dense_rows(t.movedim(1, -1), t.shape[1])
+    return r, H.row_stride(r)
+
+
+def _empty_channels_last(t):
+    """uninitialised tensor of t's shape, channels-last"""
+    if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return torch.empty_like(t)
+    return torch.empty(t.shape[:1] + t.shape[2:] + t.shape[1:2], dtype=t.dtype, device=t.device).movedim(-1, 1)
+
+
+def _f32(t):
+    if t is None:
+        return None
+    t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
 def _gn_act_forward(x, gamma, beta, lv, groups, eps, act, thr, seed, offset, want_stats):
-    """-> (y, descriptor, f32 gamma, f32 beta, stats, device offset)"""
-    g32 = None if gamma is None else gamma.detach().float().contiguous()
-    b32 = None if beta is None else beta.detach().float().contiguous()
+    """-> (y, (descriptor, backward workspace), f32 gamma, f32 beta, stats, device offset)"""
+    g32, b32 = _f32(gamma), _f32(beta)
     off = H.dropout_offset(offset, x.device)
-    last = x.movedim(1, -1) if lv is None else x
-    rows = H.dense_rows(last, last.shape[-1])
     if lv is None:
-        lv = H.Levels(x.shape[0], [(rows.shape[0] // max(x.shape[0], 1), 1)])
-        back = lambda y: y.view(last.shape).movedim(-1, 1)
+        rows, stride = _channels_last_rows(x)
+        y = _empty_channels_last(x)
+        batch = x.shape[0]
+        hw = (x.numel() // (batch * x.shape[1]) if batch else 0,)
     else:
-        back = lambda y: y
+        rows = H.dense_rows(x, x.shape[1])
+        stride, y = H.row_stride(rows), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        batch, hw = lv.batch, tuple(h * w for h, w in lv.sizes)
     with _lib.on_device(x):
-        d = H.group_norm_act_desc(rows, lv, groups, eps, act, thr, seed, off)
-        y, stats = H.group_norm_act(d, rows, g32, b32, want_stats)
-    return back(y), d, g32, b32, stats, off[1]
+        d, bwd_need, stats = H.group_norm_act(rows, stride, y, batch, hw, x.shape[1], groups, eps, act, thr, seed, off, g32, b32, want_stats)
+    return y, (d, bwd_need), g32, b32, stats, off[1]
 
 
 class GroupNormActFunction(Function):
@@ -325,37 +348,43 @@ class GroupNormActFunction(Function):
 
     @staticmethod
     def forward(ctx, x, gamma, beta, lv, groups, eps, act, thr, seed, offset):
-        y, d, g32, b32, stats, dev = _gn_act_forward(x, gamma, beta, lv, groups, eps, act, thr, seed, offset, True)
+        y, plan, g32, b32, stats, dev = _gn_act_forward(x, gamma, beta, lv, groups, eps, act, thr, seed, offset, True)
         ctx.save_for_backward(x, g32, b32, stats, dev)      # (dev: an offset that changed before the backward is an error)
-        ctx.cfg = (d, lv, None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
+        ctx.cfg = (plan, lv is not None, None if gamma is None else gamma.dtype, None if beta is None else beta.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, g32, b32, stats, _ = ctx.saved_tensors
-        d, lv, gdt, bdt = ctx.cfg
+        (d, need), pyramid, gdt, bdt = ctx.cfg
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
-        last, dlast = (x.movedim(1, -1), dy.movedim(1, -1)) if lv is None else (x, dy)
-        c = last.shape[-1]
-        tg = tb = None
-        if lv is not None:                                  # the row graph's parameters may live in all-reduce buckets
+        dx = dg = db = tg = tb = None
+        if pyramid:
+            rows, dyr = H.dense_rows(x, x.shape[1]), H.dense_rows(dy, x.shape[1])
+            dy_stride = H.row_stride(dyr)
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+            # the row graph's parameters may live in all-reduce buckets
             tg = H.GRAD_SINK.target(g32) if need_g else None
             tb = H.GRAD_SINK.target(b32) if need_b else None
-        new = lambda: torch.empty(c, dtype=torch.float32, device=x.device)
-        dg = None if not need_g else (tg if tg is not None else new())
-        db = None if not need_b else (tb if tb is not None else new())
+        else:
+            rows = _channels_last_rows(x)[0]
+            dyr, dy_stride = _channels_last_rows(dy)
+            dx = _empty_channels_last(x) if need_x else None
+        if need_g:
+            dg = tg if tg is not None else torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
+        if need_b:
+            db = tb if tb is not None else torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
         with _lib.on_device(x):
-            dx = H.group_norm_act_bwd(d, H.dense_rows(last, c), H.dense_rows(dlast, c), g32, b32, stats, need_x, dg, db)
-        if dx is not None and lv is None:
-            dx = dx.view(last.shape).movedim(-1, 1)
+            H.group_norm_act_bwd(d, need, rows, dyr, dy_stride, dx, g32, b32, stats, dg, db)
         if tg is not None:
             H.GRAD_SINK.commit(g32)
             dg = None
         if tb is not None:
             H.GRAD_SINK.commit(b32)
             db = None
-        return (dx, None if dg is None else dg.to(gdt), None if db is None else db.to(bdt)) + (None,) * 7
+        return (dx, dg if dg is None or gdt == torch.float32 else dg.to(gdt), db if db is None or bdt == torch.float32 else db.to(bdt),
+                None, None, None, None, None, None, None)
 
 
 def _gn_act_args(x, channels, weight, bias, groups, eps, activation, dropout_p, what):
@@ -397,14 +426,21 @@ def group_norm_act(x, weight, bias, num_groups, eps=1e-5, activation="relu", dro
 
 def _dropout_rows(x, residual, thr, seed, offset):
     """any shape and strides -> contiguous"""
-    flat = x.is_contiguous() and (residual is None or residual.is_contiguous())
-    cols = x.shape[-1] if x.dim() else 1
-    rows = lambda t: None if t is None else (t.view(1, -1) if flat else H.dense_rows(t, cols))
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if y.numel():
-        with _lib.on_device(x):
-            H.dropout_rows(rows(x), rows(residual), thr, seed, offset, y)
-    return y
+    n = y.numel()
+    if n == 0:
+        return y
+    if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        rows, cols, ldx, ldr = 1, n, n, n
+    else:
+        cols = x.shape[-1] if x.dim() else 1
+        x = H.dense_rows(x, cols)
+        rows, ldx, ldr = x.shape[0], H.row_stride(x), 0
+        if residual is not None:
+            residual = H.dense_rows(residual, cols)
+            ldr = H.row_stride(residual)
+    with _lib.on_device(x):
+        return H.dropout_rows(x, residual, y, rows, cols, ldx, ldr, thr, seed, offset)
 
 
 class DropoutFunction(Function):
@@ -498,9 +534,22 @@ def quantize_fp8(x, block_rows=1, transpose=False):
     x = H.dense_rows(x.detach(), x.shape[1])
     with _lib.on_device(x):
         rows, cols, _ = H.fp8_quantize(x, block_rows, not transpose, transpose)
-    if transpose:
-        return Fp8Blocks(cols[0], cols[1], x.shape[1], x.shape[0], block_rows)
-    return Fp8Blocks(rows[0], rows[1], x.shape[0], x.shape[1], block_rows)
+    (r, c), buf = (x.shape, rows) if not transpose else ((x.shape[1], x.shape[0]), cols)
+    nc = H.fp8_bytes(r, c, block_rows)[0]
+    return Fp8Blocks(buf.data[:nc].view(torch.float8_e4m3fn).view(-(-c // 128), r, 128),
+                     buf.data[nc:].view(-(-c // 512), -(-r // block_rows), 4), r, c, block_rows)
+
+
+class _Fp8Operand:
+    """the two addresses of an Fp8Blocks"""
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, t):
+        if t.codes.dtype != torch.float8_e4m3fn or t.scales.dtype != torch.uint8 or not t.codes.is_contiguous() or \
+                not t.scales.is_contiguous() or t.codes.shape != (-(-t.cols // 128), t.rows, 128) or \
+                t.scales.shape != (-(-t.cols // 512), -(-t.rows // t.block_rows), 4) or t.scales.device != t.codes.device:
+            raise ValueError("Fp8Blocks of %s: codes %s, scales %s do not have its layout" % (t.shape, tuple(t.codes.shape), tuple(t.scales.shape)))
+        self.codes, self.scales = t.codes.data_ptr(), t.scales.data_ptr()
 
 
 def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloat16):
@@ -524,7 +573,8 @@ def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloa
             raise ValueError("matmul_fp8: residual is %s %s" % ((a.rows, b.rows), out_dtype))
         residual = H.dense_rows(residual.detach(), b.rows)
     with _lib.on_device(a.codes):
-        return H.fp8_matmul(a.codes, a.scales, a.block_rows, b.codes, b.scales, b.block_rows, a.cols, bias, residual, relu, out_dtype)
+        return H.fp8_matmul(_Fp8Operand(a), a.block_rows, _Fp8Operand(b), b.block_rows, a.rows, b.rows, a.cols, bias, residual, relu, out_dtype,
+                            a.device)
 
 
 class LinearFp8Function(Function):
@@ -535,30 +585,28 @@ class LinearFp8Function(Function):
     def forward(ctx, x, weight, bias, relu, weight_q):
         need_x, need_w = ctx.needs_input_grad[:2]
         rows = H.dense_rows(x, x.shape[-1])
-        b32 = None if bias is None else bias.detach().float().contiguous()
+        m, k = rows.shape
+        n = weight.shape[0] if weight is not None else weight_q.rows
+        b32 = _f32(bias)
         xt = wt = None
         with _lib.on_device(x):
-            if weight_q is None or need_x:
-                w = H.dense_rows(weight.flatten(1), rows.shape[1])
-                wq, wt, _ = H.fp8_quantize(w, 128, weight_q is None, need_x)
-            if weight_q is not None:
-                wq = (weight_q.codes, weight_q.scales)
-            if need_w and rows.shape[0] > 0:
+            wq = None if weight_q is None else _Fp8Operand(weight_q)
+            if wq is None or need_x:
+                made, wt, _ = H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128, wq is None, need_x)
+                wq = made if wq is None else wq
+            if need_w and m > 0:
                 xq, xt, _ = H.fp8_quantize(rows, 1, True, True)
-                y = H.fp8_matmul(xq[0], xq[1], 1, wq[0], wq[1], 128, rows.shape[1], b32, None, relu, x.dtype)
+                y = H.fp8_matmul(xq, 1, wq, 128, m, n, k, b32, None, relu, x.dtype, x.device)
             else:
-                y = H.fp8_linear(rows, wq[0], wq[1], 128, b32, None, relu, x.dtype)
-        if any(ctx.needs_input_grad):
-            pair = lambda t: (None, None) if t is None else t
-            ctx.save_for_backward(*pair(xt), *pair(wt), y if relu else None)
-            ctx.cfg = (None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, rows.shape[1],
-                       x.shape[:-1])
-        return y.view(x.shape[:-1] + (y.shape[1],))
+                y = H.fp8_linear(rows, wq, 128, n, b32, relu, x.dtype)
+        ctx.save_for_backward(None if xt is None else xt.data, None if wt is None else wt.data, y if relu else None)
+        ctx.cfg = (None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, k, x.shape[:-1])
+        return y.view(x.shape[:-1] + (n,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xt, sxt, wt, swt, y = ctx.saved_tensors
+        xt, wt, y = ctx.saved_tensors
         wmeta, bdt, k, shape = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = H.dense_rows(dy, dy.shape[-1])
@@ -571,10 +619,11 @@ class LinearFp8Function(Function):
                 return dy.new_empty(shape + (k,)) if need_x else None, dw, db, None, None
             g, gt, db = H.fp8_quantize(dy, 1, need_x, need_w, need_b, y)
             if need_x:
-                dx = H.fp8_matmul(g[0], g[1], 1, wt, swt, 128, n, None, None, False, dy.dtype).view(shape + (k,))
+                dx = H.fp8_matmul(g, 1, H.Fp8Buffer(k, n, 128, data=wt), 128, m, k, n, None, None, False, dy.dtype, dy.device).view(shape + (k,))
             if need_w:
-                dw = H.fp8_matmul(gt[0], gt[1], 1, xt, sxt, 1, m, None, None, False, torch.float32).view(wmeta[0]).to(wmeta[1])
-        return dx, dw, None if db is None else db.to(bdt), None, None
+                dw = H.fp8_matmul(gt, 1, H.Fp8Buffer(k, m, 1, data=xt), 1, n, k, m, None, None, False, torch.float32, dy.device)
+                dw = dw.view(wmeta[0]) if wmeta[1] == torch.float32 else dw.view(wmeta[0]).to(wmeta[1])
+        return dx, dw, db if db is None or bdt == torch.float32 else db.to(bdt), None, None
 
 
 def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
@@ -605,8 +654,8 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
         return LinearFp8Function.apply(x, weight, bias, relu, weight_q)
     rows = H.dense_rows(x, k)
     with _lib.on_device(x):
-        wq = (weight_q.codes, weight_q.scales) if weight_q is not None else H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128)[0]
-        y = H.fp8_linear(rows, wq[0], wq[1], 128, None if bias is None else bias.detach().float().contiguous(), None, relu, x.dtype)
+        wq = _Fp8Operand(weight_q) if weight_q is not None else H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128)[0]
+        y = H.fp8_linear(rows, wq, 128, n, _f32(bias), relu, x.dtype)
     return y.view(x.shape[:-1] + (n,))
 
 

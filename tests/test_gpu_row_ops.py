@@ -204,8 +204,9 @@ def test_group_norm_act_leaves_other_columns_alone():
     """a C call that writes a channel slice: what lies beside it stays"""
     lib = _lib.load()
     x, out = rnd(30, 16), torch.full((30, 40), 7.0, device=DEV)
-    d = H.group_norm_act_desc(x, H.Levels(2, [(5, 3)]), 4, 1e-5, 0, 0, 0, (0, None))
-    d.y_stride = 40
+    d = _lib.GnActDesc()
+    d.nlev, d.batch, d.channels, d.groups, d.dtype, d.act, d.eps = 1, 2, 16, 4, 2, 0, 1e-5
+    d.hw[0], d.x_stride, d.y_stride, d.dy_stride, d.dx_stride = 15, 16, 40, 16, 16
     ws = torch.empty(lib.sm_group_norm_act_workspace(C.byref(d), 0), dtype=torch.uint8, device=DEV)
     dst = out[:, 8:24]
     _lib.check(lib.sm_group_norm_act(C.byref(d), _lib.ptr(x), None, None, C.c_void_p(dst.data_ptr()), None, _lib.ptr(ws), ws.numel(),
