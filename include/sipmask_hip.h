@@ -789,7 +789,7 @@ typedef struct {
 
 /* y = act(GroupNorm(x) * gamma + beta) [dropped out]; gamma / beta f32 [channels] or NULL (1 / 0).  stats (may be NULL when no
  * backward follows): f64 [batch][nlev][groups][2] = (mean, 1 / sqrt(var + eps)).  workspace: sm_group_norm_act_workspace(d, 0) bytes,
- * 16-byte aligned, contents irrelevant; y may be x.  No atomics: bit-reproducible. */
+ * 16-byte aligned, contents irrelevant (0 bytes: NULL will do, here and below); y may be x.  No atomics: bit-reproducible. */
 int64_t sm_group_norm_act_workspace(const sm_gn_act_desc* d, int backward);
 int sm_group_norm_act(const sm_gn_act_desc* d, const void* x, const float* gamma, const float* beta, void* y, double* stats,
                       void* workspace, int64_t workspace_bytes, sm_stream_t stream);

@@ -740,7 +740,7 @@ bool fp8_out_ok(const void* q, const void* scale) {
 
 extern "C" int64_t sm_fp8_quantize_workspace(int64_t rows, int64_t cols, int col_sum) {
   if (rows < 0 || cols < 1) return SM_ERR_BAD_SHAPE;
-  return col_sum ? std::max<int64_t>(16, (rows + 127) / 128 * cols * 4) : 16;
+  return col_sum ? (rows + 127) / 128 * cols * 4 : 0;
 }
 
 extern "C" int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t cols, int64_t x_stride, int block_rows, const void* gate,
@@ -772,7 +772,7 @@ extern "C" int64_t sm_fp8_matmul_workspace(const sm_fp8_matmul_desc* d) {
   MmPlan p;
   const int st = mm_plan(d, &p);
   if (st != SM_OK) return st;
-  return std::max<int64_t>(16, p.ws);
+  return p.ws;
 }
 
 namespace {
@@ -864,7 +864,7 @@ extern "C" int64_t sm_fp8_linear_workspace(const sm_fp8_matmul_desc* d) {
   MmPlan p;
   const int st = mm_plan(d, &p);
   if (st != SM_OK) return st;
-  return std::max<int64_t>(16, linear_ws(d, p));
+  return linear_ws(d, p);
 }
 
 extern "C" int sm_fp8_linear(const sm_fp8_matmul_desc* d, int x_dtype, const void* x, int64_t x_stride, const void* b,

@@ -24,16 +24,21 @@
 
 namespace {
 
-constexpr int GA_THREADS = 256;
+constexpr int GA_THREADS = 256;     // element-wise launches
+constexpr int GA_STAT = 1024;       // threads of the forward's reduction: few blocks with many waves, so that few partials are left
+constexpr int GA_STAT1 = 256;       // ... where a vector spans groups (16 sums a thread)
+constexpr int GA_SUM = 512;         // threads of the backward's reduction
+constexpr int GA_COMBINE = 2048;    // partials that an element-wise block has to add up (32 KB out of L2), see ga_plan
 constexpr int GA_TILE = 32;         // column vectors per block: 512-byte row segments for 16-bit types
 constexpr int GA_TILE1 = 64;        // columns per block of the any-alignment path
 
 struct GaArgs {
   int nlev, batch, C, G, cpg, act;
-  int cols, ct, lanes, ntile;       // column vectors, per block, row lanes of a block, column tiles
+  int cols, ct, ntile;              // column vectors, per block, column tiles
   long long hw[SM_MAX_LEVELS], row0[SM_MAX_LEVELS];
-  int blk0[SM_MAX_LEVELS + 1];      // first row block of each level (per image)
-  int rpb;                          // rows per block
+  int sblk0[SM_MAX_LEVELS + 1];     // reductions: first row block of each level (per image)
+  int ablk0[SM_MAX_LEVELS + 1];     // element-wise launches
+  int srpb, arpb;                   // rows per block
   long long ldx, ldy, lddx;         // row strides in elements: x and dy, y, dx
   long long lddy;
   float eps;
@@ -48,9 +53,9 @@ __device__ __forceinline__ int ga_level(const int* blk0, int nlev, int b) {
   return lev;
 }
 
-// sum over the block's row lanes of NV values per thread, left on the threads of lane 0 (fixed tree)
-template <int NV, typename V>
-__device__ __forceinline__ void lane_tree(V (*sh)[GA_THREADS], V (&v)[NV], int lane, int ct, int lanes) {
+// sum over the block's row lanes of NV values per thread, left in sh[k][column] (fixed tree)
+template <int NV, int NT, typename V>
+__device__ __forceinline__ void lane_tree(V (*sh)[NT], const V* v, int lane, int ct, int lanes) {
   const int t = threadIdx.x;
 #pragma unroll
   for (int k = 0; k < NV; ++k) sh[k][t] = v[k];
@@ -66,55 +71,68 @@ __device__ __forceinline__ void lane_tree(V (*sh)[GA_THREADS], V (&v)[NV], int l
   }
 }
 
+// what a block works on: image, level and rows [rb, re) of it
+struct GaBlock {
+  int n, b, lev;
+  long long rb, re;
+};
+__device__ __forceinline__ GaBlock ga_block(const GaArgs& a, const int* blk0, int rpb, int block) {
+  GaBlock k;
+  const int nblk = blk0[a.nlev];
+  k.n = block / nblk, k.b = block - k.n * nblk;
+  k.lev = ga_level(blk0, a.nlev, k.b);
+  k.rb = (long long)(k.b - blk0[k.lev]) * rpb;
+  k.re = min(k.rb + (long long)rpb, a.hw[k.lev]);
+  return k;
+}
+
 // launch 1, forward: part[image][row block][tile][group - first group of the tile] = (sum x, sum x^2)
 // WHOLE: a vector lies in one group (cpg % VEC == 0), so a thread needs two sums instead of 2 * VEC
 template <int DT, int VEC, bool WHOLE>
-__global__ __launch_bounds__(GA_THREADS) void ga_stats_kernel(const typename Elem<DT>::type* __restrict__ x, double2* __restrict__ part,
+__global__ __launch_bounds__(WHOLE ? GA_STAT : GA_STAT1) void ga_stats_kernel(const typename Elem<DT>::type* __restrict__ x, double2* __restrict__ part,
                                                               const GaArgs a, int gpt) {
   typedef RowVec<DT, VEC> RV;
-  constexpr int NS = WHOLE ? 1 : VEC;
-  __shared__ double sh[2 * NS][GA_THREADS];
-  const int nblk = a.blk0[a.nlev];
-  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.blk0, a.nlev, b);
-  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
+  constexpr int NS = WHOLE ? 1 : VEC, NT = WHOLE ? GA_STAT : GA_STAT1;
+  __shared__ double sh[2 * NS][NT];
+  const GaBlock k = ga_block(a, a.sblk0, a.srpb, blockIdx.x);
+  const int tile = blockIdx.y, lanes = NT / a.ct;
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
-  const bool live = lane < a.lanes && col < a.cols;
+  const bool live = lane < lanes && col < a.cols;
   double v[2 * NS];
 #pragma unroll
   for (int k = 0; k < 2 * NS; ++k) v[k] = 0.0;
   if (live) {
-    const typename Elem<DT>::type* p = x + (a.row0[lev] + (long long)n * a.hw[lev]) * a.ldx + (long long)col * VEC;
+    const typename Elem<DT>::type* p = x + (a.row0[k.lev] + (long long)k.n * a.hw[k.lev]) * a.ldx + (long long)col * VEC;
     auto add = [&](const typename RV::raw& q) {
       float f[VEC];
       RV::unpack(q, f);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const double d = (double)f[e];
-        const int k = WHOLE ? 0 : e;
-        v[k] += d;
-        v[NS + k] = __builtin_fma(d, d, v[NS + k]);
+        const int w = WHOLE ? 0 : e;
+        v[w] += d;
+        v[NS + w] = __builtin_fma(d, d, v[NS + w]);
       }
     };
-    long long r = rb + lane;
-    for (; r + 3 * a.lanes < re; r += 4 * a.lanes) {     // four loads in flight
+    long long r = k.rb + lane;
+    for (; r + 3 * lanes < k.re; r += 4 * lanes) {     // four loads in flight
       typename RV::raw q[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) q[u] = RV::load(p + (r + u * a.lanes) * a.ldx);
+      for (int u = 0; u < 4; ++u) q[u] = RV::load(p + (r + u * lanes) * a.ldx);
 #pragma unroll
       for (int u = 0; u < 4; ++u) add(q[u]);
     }
-    for (; r < re; r += a.lanes) add(RV::load(p + r * a.ldx));
+    for (; r < k.re; r += lanes) add(RV::load(p + r * a.ldx));
   }
-  lane_tree<2 * NS>(sh, v, lane, a.ct, a.lanes);
+  lane_tree<2 * NS, NT>(sh, v, lane, a.ct, lanes);
   // one thread per group of the tile adds its channels
   const int c0 = tile * a.ct * VEC, c1 = min(c0 + a.ct * VEC, a.C);
   const int g0 = c0 / a.cpg, g1 = (c1 - 1) / a.cpg;
-  for (int g = g0 + threadIdx.x; g <= g1; g += GA_THREADS) {
+  for (int g = g0 + threadIdx.x; g <= g1; g += NT) {
     const int lo = max(g * a.cpg, c0) - c0, hi = min((g + 1) * a.cpg, c1) - c0;
     double s = 0.0, ss = 0.0;
     if constexpr (WHOLE) {
-      for (int k = lo / VEC; k < hi / VEC; ++k) s += sh[0][k], ss += sh[1][k];
+      for (int q = lo / VEC; q < hi / VEC; ++q) s += sh[0][q], ss += sh[1][q];
     } else {
       for (int c = lo; c < hi; ++c) s += sh[c % VEC][c / VEC], ss += sh[NS + c % VEC][c / VEC];
     }
@@ -122,32 +140,42 @@ __global__ __launch_bounds__(GA_THREADS) void ga_stats_kernel(const typename Ele
   }
 }
 
-// launch 2, forward: one wave per (image, level, group) adds the group's partials: stats = (mean, rstd)
 __device__ __forceinline__ double2 ga_mean_rstd(double s, double ss, double cnt, float eps) {
   const double m = s / cnt;
   double var = ss / cnt - m * m;
   var = var < 0.0 ? 0.0 : var;                   // (NaN stays NaN)
   return make_double2(m, 1.0 / sqrt(var + (double)eps));
 }
-__global__ __launch_bounds__(GA_THREADS) void ga_combine_kernel(const double2* __restrict__ part, double2* __restrict__ stats, const GaArgs a,
-                                                                int gpt, int tc) {
-  const long long i = (long long)blockIdx.x * (GA_THREADS / 64) + (threadIdx.x >> 6);
-  if (i >= (long long)a.batch * a.nlev * a.G) return;
-  const int lane = threadIdx.x & 63;
-  const int g = (int)(i % a.G), lev = (int)(i / a.G % a.nlev);
-  const long long n = i / ((long long)a.G * a.nlev);
-  const int b0 = a.blk0[lev], nb = a.blk0[lev + 1] - b0;
+
+// The partials of every group of this block's column tile, added into s_sum[group - first group]: every element-wise block does it for
+// itself (a launch of its own for it cost 6 us, more than these few KB out of L2).  Threads share a group's entries and join in order.
+__device__ __forceinline__ int ga_combine(const double2* __restrict__ part, double2* s_sum, double2* s_red, const GaArgs& a, int gpt, int tc,
+                                          int n, int lev, int tile) {
+  const int c0 = tile * tc, c1 = min(c0 + tc, a.C);
+  const int g0 = c0 / a.cpg, ng = (c1 - 1) / a.cpg - g0 + 1;
+  const int b0 = a.sblk0[lev], nb = a.sblk0[lev + 1] - b0;
+  int tpg = 1;                                   // threads per group, a power of two
+  while (tpg * 2 * ng <= GA_THREADS) tpg <<= 1;
+  const int gi = threadIdx.x / tpg, ti = threadIdx.x - gi * tpg;
   double s = 0.0, ss = 0.0;
-  for (int t = g * a.cpg / tc; t <= ((g + 1) * a.cpg - 1) / tc; ++t) {
-    const double2* q = part + ((n * a.blk0[a.nlev] + b0) * a.ntile + t) * gpt + (g - t * tc / a.cpg);
-    for (int k = lane; k < nb; k += 64) {
-      const double2 e = q[(long long)k * a.ntile * gpt];
-      s += e.x, ss += e.y;
+  if (gi < ng) {
+    const int g = g0 + gi;
+    for (int t = g * a.cpg / tc; t <= ((g + 1) * a.cpg - 1) / tc; ++t) {
+      const double2* q = part + (((long long)n * a.sblk0[a.nlev] + b0) * a.ntile + t) * gpt + (g - t * tc / a.cpg);
+      for (int i = ti; i < nb; i += tpg) {
+        const double2 e = q[(long long)i * a.ntile * gpt];
+        s += e.x, ss += e.y;
+      }
     }
   }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64), ss += __shfl_xor(ss, d, 64);
-  if (lane == 0) stats[i] = ga_mean_rstd(s, ss, (double)a.hw[lev] * (double)a.cpg, a.eps);
+  s_red[threadIdx.x] = make_double2(s, ss);
+  __syncthreads();
+  if (gi < ng && ti == 0) {
+    for (int i = 1; i < tpg; ++i) s += s_red[threadIdx.x + i].x, ss += s_red[threadIdx.x + i].y;
+    s_sum[gi] = make_double2(s, ss);
+  }
+  __syncthreads();
+  return ng;
 }
 
 // what a thread of the forward element pass needs of its channels.  The mean is a sum of two floats: x - m keeps its digits for
@@ -184,28 +212,35 @@ __device__ __forceinline__ uint32_t ga_keep(const GaArgs& a, unsigned long long 
   return VEC == 1 ? keep >> (int)(i & 7) : keep;
 }
 
-// launch 3, forward
+// launch 2, forward; the first row block of a level writes (mean, rstd) out for the backward pass
 template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
 __global__ __launch_bounds__(GA_THREADS) void ga_apply_kernel(const typename Elem<DT>::type* __restrict__ x,
                                                               typename Elem<DT>::type* __restrict__ y, const float* __restrict__ gamma,
-                                                              const float* __restrict__ beta, const double2* __restrict__ stats,
-                                                              const GaArgs a) {
+                                                              const float* __restrict__ beta, const double2* __restrict__ part,
+                                                              double2* __restrict__ stats, const GaArgs a, int gpt) {
   typedef RowVec<DT, VEC> RV;
-  const int nblk = a.blk0[a.nlev];
-  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.blk0, a.nlev, b);
-  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
+  __shared__ double2 s_stat[GA_THREADS], s_red[GA_THREADS];
+  const GaBlock k = ga_block(a, a.ablk0, a.arpb, blockIdx.x);
+  const int tile = blockIdx.y, lanes = GA_THREADS / a.ct, tc = a.ct * VEC, g0 = tile * tc / a.cpg;
+  const int ng = ga_combine(part, s_stat, s_red, a, gpt, tc, k.n, k.lev, tile);
+  for (int g = threadIdx.x; g < ng; g += GA_THREADS) {
+    const double2 st = ga_mean_rstd(s_stat[g].x, s_stat[g].y, (double)a.hw[k.lev] * (double)a.cpg, a.eps);
+    s_stat[g] = st;
+    // (a group is written by the tile that it starts in)
+    if (stats != nullptr && k.b == a.ablk0[k.lev] && (g0 + g) * a.cpg >= tile * tc)
+      stats[((long long)k.n * a.nlev + k.lev) * a.G + g0 + g] = st;
+  }
+  __syncthreads();
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
-  if (lane >= a.lanes || col >= a.cols) return;
+  if (lane >= lanes || col >= a.cols) return;
   GaNorm<VEC, WHOLE> nm;
-  const double2* st = stats + ((long long)n * a.nlev + lev) * a.G;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     const int c = col * VEC + e;
-    nm.set(e, st[c / a.cpg], gamma != nullptr ? gamma[c] : 1.f, beta != nullptr ? beta[c] : 0.f);
+    nm.set(e, s_stat[c / a.cpg - g0], gamma != nullptr ? gamma[c] : 1.f, beta != nullptr ? beta[c] : 0.f);
   }
   const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
-  const long long row_base = a.row0[lev] + (long long)n * a.hw[lev];
+  const long long row_base = a.row0[k.lev] + (long long)k.n * a.hw[k.lev];
   const typename Elem<DT>::type* px = x + row_base * a.ldx + (long long)col * VEC;
   typename Elem<DT>::type* py = y + row_base * a.ldy + (long long)col * VEC;
   auto one = [&](const typename RV::raw& q, long long r) {
@@ -214,15 +249,18 @@ __global__ __launch_bounds__(GA_THREADS) void ga_apply_kernel(const typename Ele
     nm.template apply<ACT, DROP>(f, ga_keep<VEC, DROP>(a, off, row_base + r, col), a.drop.scale);
     RV::store(py + r * a.ldy, f);
   };
-  long long r = rb + lane;
-  for (; r + 3 * a.lanes < re; r += 4 * a.lanes) {
+  long long r = k.rb + lane;
+  for (; r + 3 * lanes < k.re; r += 4 * lanes) {
     typename RV::raw q[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) q[u] = RV::load(px + (r + u * a.lanes) * a.ldx);
+    for (int u = 0; u < 4; ++u) q[u] = RV::load(px + (r + u * lanes) * a.ldx);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) one(q[u], r + u * a.lanes);
+    for (int u = 0; u < 4; ++u) {
+      one(q[u], r + u * lanes);
+      __builtin_amdgcn_sched_barrier(0);         // one row at a time: interleaved, four generator blocks took 30 more registers
+    }
   }
-  for (; r < re; r += a.lanes) one(RV::load(px + r * a.ldx), r);
+  for (; r < k.re; r += lanes) one(RV::load(px + r * a.ldx), r);
 }
 
 // what a thread of the backward launches needs of its channels
@@ -273,6 +311,7 @@ struct GaChan {
           const double2 s = st[WHOLE ? 0 : e];
           const double t64 = ((double)x[e] - s.x) * s.y * (double)ga[e] + (double)be[e];
           if (__builtin_fabsf(t[e]) <= 1e-6f * __builtin_fabsf(be[e])) t[e] = t64 > 0.0 ? 1.f : (t64 <= 0.0 ? -1.f : t[e]);
+          __builtin_amdgcn_sched_barrier(0);     // (one at a time: this arm must not set the kernel's register count)
         }
       }
 #pragma unroll
@@ -284,29 +323,28 @@ struct GaChan {
   }
 };
 
-// launch 1, backward: part[image][row block][channel] = (sum d, sum d xhat) of the block's rows
+// launch 1, backward, over the rows of a block: chan[image][row block][channel] = (sum d, sum d xhat) and, weighted with gamma, the same
+// per group of the column tile: part[image][row block][tile][group - first group of the tile]
 template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
-__global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename Elem<DT>::type* __restrict__ x,
+__global__ __launch_bounds__(GA_SUM, WHOLE ? 4 : 2) void ga_bwd_sum_kernel(const typename Elem<DT>::type* __restrict__ x,
                                                                 const typename Elem<DT>::type* __restrict__ dy,
                                                                 const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                                const double2* __restrict__ stats, float2* __restrict__ part,
-                                                                const GaArgs a) {
+                                                                const double2* __restrict__ stats, float2* __restrict__ chan,
+                                                                double2* __restrict__ part, const GaArgs a, int gpt) {
   typedef RowVec<DT, VEC> RV;
-  __shared__ float sh[2 * VEC][GA_THREADS];
-  const int nblk = a.blk0[a.nlev];
-  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.blk0, a.nlev, b);
-  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
+  __shared__ float sh[VEC][GA_SUM], s_chan[2][GA_THREADS];
+  const GaBlock k = ga_block(a, a.sblk0, a.srpb, blockIdx.x);
+  const int tile = blockIdx.y, lanes = GA_SUM / a.ct;
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
-  const bool live = lane < a.lanes && col < a.cols;
+  const bool live = lane < lanes && col < a.cols;
   float v[2 * VEC];
 #pragma unroll
   for (int k = 0; k < 2 * VEC; ++k) v[k] = 0.f;
   if (live) {
     GaChan<VEC, WHOLE> ch;
-    ch.fill(a, stats, gamma, beta, ((long long)n * a.nlev + lev) * a.G, col);
+    ch.fill(a, stats, gamma, beta, ((long long)k.n * a.nlev + k.lev) * a.G, col);
     const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
-    const long long row_base = a.row0[lev] + (long long)n * a.hw[lev];
+    const long long row_base = a.row0[k.lev] + (long long)k.n * a.hw[k.lev];
     const typename Elem<DT>::type* px = x + row_base * a.ldx + (long long)col * VEC;
     const typename Elem<DT>::type* pd = dy + row_base * a.lddy + (long long)col * VEC;
     auto one = [&](const typename RV::raw& qx, const typename RV::raw& qd, long long r) {
@@ -322,119 +360,99 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_sum_kernel(const typename E
         v[VEC + e] = __builtin_fmaf(d[e], xh[e], v[VEC + e]);
       }
     };
-    long long r = rb + lane;
-    for (; r + a.lanes < re; r += 2 * a.lanes) {
+    long long r = k.rb + lane;
+    for (; r + lanes < k.re; r += 2 * lanes) {
       typename RV::raw qx[2], qd[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) qx[u] = RV::load(px + (r + u * a.lanes) * a.ldx), qd[u] = RV::load(pd + (r + u * a.lanes) * a.lddy);
+      for (int u = 0; u < 2; ++u) qx[u] = RV::load(px + (r + u * lanes) * a.ldx), qd[u] = RV::load(pd + (r + u * lanes) * a.lddy);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) one(qx[u], qd[u], r + u * a.lanes);
-    }
-    for (; r < re; r += a.lanes) one(RV::load(px + r * a.ldx), RV::load(pd + r * a.lddy), r);
-  }
-  lane_tree<2 * VEC>(sh, v, lane, a.ct, a.lanes);
-  const int c0 = tile * a.ct * VEC, nc = min(a.ct * VEC, a.C - c0);
-  for (int c = threadIdx.x; c < nc; c += GA_THREADS)
-    part[(long long)blockIdx.x * a.C + c0 + c] = make_float2(sh[c % VEC][c / VEC], sh[VEC + c % VEC][c / VEC]);
-}
-
-// launch 2, backward: per (image, level) the channel sums chan[c] = (sum d, sum d xhat) and the group means
-// gmean[g] = (mean d gamma, mean d gamma xhat).  A block takes gb whole groups, 32 channels x 32 slices of the
-// row blocks at a time.
-__global__ __launch_bounds__(1024) void ga_bwd_combine_kernel(const float2* __restrict__ part, const float* __restrict__ gamma,
-                                                                    double2* __restrict__ chan, double2* __restrict__ gmean, const GaArgs a,
-                                                                    int gb) {
-  __shared__ double2 sh[32][33];
-  const int nl = blockIdx.x, n = nl / a.nlev, lev = nl - n * a.nlev;
-  const int nblk = a.blk0[a.nlev], s0 = a.blk0[lev], ns = a.blk0[lev + 1] - s0;
-  const int g0 = blockIdx.y * gb, g1 = min(g0 + gb, a.G);
-  const int ci = threadIdx.x & 31, sl = threadIdx.x >> 5;
-  const double cnt = (double)a.hw[lev] * (double)a.cpg;
-  for (int c0 = g0 * a.cpg; c0 < g1 * a.cpg; c0 += 32) {
-    const int c = c0 + ci;
-    double s = 0.0, ss = 0.0;
-    if (c < g1 * a.cpg)
-      for (int i = sl; i < ns; i += 32) {
-        const float2 e = part[((long long)n * nblk + s0 + i) * a.C + c];
-        s += (double)e.x, ss += (double)e.y;
+      for (int u = 0; u < 2; ++u) {
+        one(qx[u], qd[u], r + u * lanes);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    __syncthreads();
-    sh[sl][ci] = make_double2(s, ss);
-    __syncthreads();
-    if (sl == 0 && c < g1 * a.cpg) {
-      for (int k = 1; k < 32; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
-      chan[(long long)nl * a.C + c] = make_double2(s, ss);
     }
+    for (; r < k.re; r += lanes) one(RV::load(px + r * a.ldx), RV::load(pd + r * a.lddy), r);
   }
-  __syncthreads();                               // (the block's own global writes are visible to it behind the barrier)
-  for (int g = g0 + threadIdx.x; g < g1; g += 1024) {
-    double m1 = 0.0, m2 = 0.0;
-    for (int c = g * a.cpg; c < (g + 1) * a.cpg; ++c) {
-      const double2 e = chan[(long long)nl * a.C + c];
-      const double w = gamma != nullptr ? (double)gamma[c] : 1.0;
-      m1 += w * e.x, m2 += w * e.y;
+  const int c0 = tile * a.ct * VEC, nc = min(a.ct * VEC, a.C - c0);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    lane_tree<VEC, GA_SUM>(sh, v + q * VEC, lane, a.ct, lanes);
+    for (int c = threadIdx.x; c < nc; c += GA_SUM) s_chan[q][c] = sh[c % VEC][c / VEC];
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < nc; c += GA_SUM)
+    chan[(long long)blockIdx.x * a.C + c0 + c] = make_float2(s_chan[0][c], s_chan[1][c]);
+  const int g0 = c0 / a.cpg, ng = (c0 + nc - 1) / a.cpg - g0 + 1;
+  for (int g = threadIdx.x; g < ng; g += GA_SUM) {
+    const int lo = max((g0 + g) * a.cpg - c0, 0), hi = min((g0 + g + 1) * a.cpg - c0, nc);
+    double s = 0.0, ss = 0.0;
+    for (int c = lo; c < hi; ++c) {
+      const double w = gamma != nullptr ? (double)gamma[c0 + c] : 1.0;
+      s += w * (double)s_chan[0][c], ss += w * (double)s_chan[1][c];
     }
-    gmean[(long long)nl * a.G + g] = make_double2(m1 / cnt, m2 / cnt);
+    part[((long long)blockIdx.x * a.ntile + tile) * gpt + g] = make_double2(s, ss);
   }
 }
 
-// dgamma / dbeta of 32 channels: the channel sums over images and levels, 8 slices joined in order
-__device__ __forceinline__ void ga_param_grads(double2 (*sh)[32], const double2* __restrict__ chan, float* __restrict__ dgamma,
+// dgamma / dbeta of 32 channels: entries chan[0 .. n)[channel], 8 slices joined in order
+template <typename V2>
+__device__ __forceinline__ void ga_param_grads(double2 (*sh)[32], const V2* __restrict__ chan, long long n, float* __restrict__ dgamma,
                                                float* __restrict__ dbeta, const GaArgs& a, int cblock) {
   const int ci = threadIdx.x & 31, sl = threadIdx.x >> 5, c = cblock * 32 + ci;
   double s = 0.0, ss = 0.0;
-  if (c < a.C)
-    for (int i = sl; i < a.batch * a.nlev; i += 8) {
-      const double2 e = chan[(long long)i * a.C + c];
-      s += e.x, ss += e.y;
+  if (c < a.C) {
+#pragma unroll 4
+    for (long long i = sl; i < n; i += GA_THREADS / 32) {
+      const V2 e = chan[i * a.C + c];
+      s += (double)e.x, ss += (double)e.y;
     }
+  }
   sh[sl][ci] = make_double2(s, ss);
   __syncthreads();
   if (sl == 0 && c < a.C) {
-    for (int k = 1; k < 8; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
+    for (int k = 1; k < GA_THREADS / 32; ++k) s += sh[k][ci].x, ss += sh[k][ci].y;
     if (dbeta != nullptr) dbeta[c] = (float)s;
     if (dgamma != nullptr) dgamma[c] = (float)ss;
   }
 }
-__global__ __launch_bounds__(GA_THREADS) void ga_param_grads_kernel(const double2* __restrict__ chan, float* __restrict__ dgamma,
+__global__ __launch_bounds__(GA_THREADS) void ga_param_grads_kernel(const double2* __restrict__ chan, long long n, float* __restrict__ dgamma,
                                                                     float* __restrict__ dbeta, const GaArgs a) {
-  __shared__ double2 sh[8][32];
-  ga_param_grads(sh, chan, dgamma, dbeta, a, blockIdx.x);
+  __shared__ double2 sh[GA_THREADS / 32][32];
+  ga_param_grads(sh, chan, n, dgamma, dbeta, a, blockIdx.x);
 }
 
-// launch 3, backward: dx element by element; the blocks behind the last row block add up dgamma / dbeta over images and levels
+// launch 2, backward: the first nparam blocks add up dgamma / dbeta (a long walk over few bytes: they start first), the others write dx
 template <int DT, int VEC, bool WHOLE, int ACT, bool DROP>
 __global__ __launch_bounds__(GA_THREADS) void ga_bwd_apply_kernel(const typename Elem<DT>::type* __restrict__ x,
                                                                   const typename Elem<DT>::type* __restrict__ dy,
                                                                   const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                                  const double2* __restrict__ stats, const double2* __restrict__ chan,
-                                                                  const double2* __restrict__ gmean, typename Elem<DT>::type* __restrict__ dx,
-                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta, const GaArgs a,
-                                                                  long long nrow_blocks) {
+                                                                  const double2* __restrict__ stats, const float2* __restrict__ chan,
+                                                                  const double2* __restrict__ part, typename Elem<DT>::type* __restrict__ dx,
+                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta, const GaArgs a, int gpt,
+                                                                  int nparam) {
   typedef RowVec<DT, VEC> RV;
-  __shared__ double2 sh[8][32];
-  if ((long long)blockIdx.x >= nrow_blocks) {
-    if (blockIdx.y == 0) ga_param_grads(sh, chan, dgamma, dbeta, a, (int)(blockIdx.x - nrow_blocks));
+  __shared__ double2 s_sum[GA_THREADS], s_red[GA_THREADS / 32][32];
+  if ((int)blockIdx.x < nparam) {
+    if (blockIdx.y == 0) ga_param_grads(s_red, chan, (long long)a.batch * a.sblk0[a.nlev], dgamma, dbeta, a, blockIdx.x);
     return;
   }
-  const int nblk = a.blk0[a.nlev];
-  const int n = blockIdx.x / nblk, b = blockIdx.x - n * nblk, tile = blockIdx.y;
-  const int lev = ga_level(a.blk0, a.nlev, b);
-  const long long rb = (long long)(b - a.blk0[lev]) * a.rpb, re = min(rb + (long long)a.rpb, a.hw[lev]);
+  const GaBlock k = ga_block(a, a.ablk0, a.arpb, blockIdx.x - nparam);
+  const int tile = blockIdx.y, lanes = GA_THREADS / a.ct, tc = a.ct * VEC, g0 = tile * tc / a.cpg;
+  ga_combine(part, s_sum, &s_red[0][0], a, gpt, tc, k.n, k.lev, tile);
   const int cl = threadIdx.x % a.ct, lane = threadIdx.x / a.ct, col = tile * a.ct + cl;
-  if (lane >= a.lanes || col >= a.cols) return;
+  if (lane >= lanes || col >= a.cols) return;
   GaChan<VEC, WHOLE> ch;
-  const long long sbase = ((long long)n * a.nlev + lev) * a.G;
-  ch.fill(a, stats, gamma, beta, sbase, col);
+  ch.fill(a, stats, gamma, beta, ((long long)k.n * a.nlev + k.lev) * a.G, col);
   constexpr int NS = WHOLE ? 1 : VEC;
-  float m1[NS], m2[NS];
+  const double cnt = (double)a.hw[k.lev] * (double)a.cpg;
+  float m1[NS], m2[NS];                          // means over the group of d gamma and d gamma xhat
 #pragma unroll
-  for (int k = 0; k < NS; ++k) {
-    const double2 e = gmean[sbase + (col * VEC + k) / a.cpg];
-    m1[k] = (float)e.x, m2[k] = (float)e.y;
+  for (int e = 0; e < NS; ++e) {
+    const double2 sum = s_sum[(col * VEC + e) / a.cpg - g0];
+    m1[e] = (float)(sum.x / cnt), m2[e] = (float)(sum.y / cnt);
   }
   const unsigned long long off = DROP ? drop_offset(a.drop) : 0ull;
-  const long long row_base = a.row0[lev] + (long long)n * a.hw[lev];
+  const long long row_base = a.row0[k.lev] + (long long)k.n * a.hw[k.lev];
   const typename Elem<DT>::type* px = x + row_base * a.ldx + (long long)col * VEC;
   const typename Elem<DT>::type* pd = dy + row_base * a.lddy + (long long)col * VEC;
   typename Elem<DT>::type* po = dx + row_base * a.lddx + (long long)col * VEC;
@@ -447,20 +465,23 @@ __global__ __launch_bounds__(GA_THREADS) void ga_bwd_apply_kernel(const typename
     ch.template grad<ACT, DROP>(fx, fd, keep, a.drop.scale, xh, d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int k = WHOLE ? 0 : e;
-      fx[e] = ch.rs[k] * (__builtin_fmaf(d[e], ch.ga[e], -m1[k]) - xh[e] * m2[k]);
+      const int w = WHOLE ? 0 : e;
+      fx[e] = ch.rs[w] * (__builtin_fmaf(d[e], ch.ga[e], -m1[w]) - xh[e] * m2[w]);
     }
     RV::store(po + r * a.lddx, fx);
   };
-  long long r = rb + lane;
-  for (; r + a.lanes < re; r += 2 * a.lanes) {
+  long long r = k.rb + lane;
+  for (; r + lanes < k.re; r += 2 * lanes) {
     typename RV::raw qx[2], qd[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) qx[u] = RV::load(px + (r + u * a.lanes) * a.ldx), qd[u] = RV::load(pd + (r + u * a.lanes) * a.lddy);
+    for (int u = 0; u < 2; ++u) qx[u] = RV::load(px + (r + u * lanes) * a.ldx), qd[u] = RV::load(pd + (r + u * lanes) * a.lddy);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) one(qx[u], qd[u], r + u * a.lanes);
+    for (int u = 0; u < 2; ++u) {
+      one(qx[u], qd[u], r + u * lanes);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
-  for (; r < re; r += a.lanes) one(RV::load(px + r * a.ldx), RV::load(pd + r * a.lddy), r);
+  for (; r < k.re; r += lanes) one(RV::load(px + r * a.ldx), RV::load(pd + r * a.lddy), r);
 }
 
 // ------------------------------------------------------------------------------------------------ small maps: one launch
@@ -669,11 +690,11 @@ struct GaPlan {
   bool vec, whole;
   int small_ct;                     // > 0: the one-launch kernels, that many column vectors per block
   int gpt;                          // groups per column tile (slots of a partial)
-  long long items;                  // batch * row blocks of all levels
+  long long items, ablocks;         // batch * row blocks of all levels: reductions, element-wise launches
   long long fwd_ws, bwd_ws;         // bytes
 };
 
-int ga_plan(const sm_gn_act_desc* d, bool aligned, GaPlan* p) {
+int ga_plan(const sm_gn_act_desc* d, bool aligned, bool backward, GaPlan* p) {
   if (d == nullptr) return SM_ERR_BAD_ARG;
   if (d->nlev < 1 || d->nlev > SM_MAX_LEVELS || d->batch < 0 || d->channels < 1 || d->groups < 1 || d->channels % d->groups != 0)
     return SM_ERR_BAD_SHAPE;
@@ -693,7 +714,6 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, GaPlan* p) {
   p->whole = a.cpg % vec == 0;
   a.cols = a.C / vec;
   a.ct = std::min(a.cols, p->vec ? GA_TILE : GA_TILE1);
-  a.lanes = GA_THREADS / a.ct;
   a.ntile = sm_cdiv(a.cols, a.ct);
   if (a.ntile > 65535 || a.G > 65535 * 32) return SM_ERR_UNSUPPORTED;
   const int tc = a.ct * vec;
@@ -704,21 +724,31 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, GaPlan* p) {
     a.hw[l] = d->hw[l], a.row0[l] = d->row0[l];
     rows += d->hw[l], hw_max = std::max<long long>(hw_max, d->hw[l]);
   }
-  // about 2048 blocks (8 per CU) of at least 4 rows per row lane
-  const long long rpb = std::max<long long>(4 * a.lanes, rows * a.batch / 2048 * a.ntile);
-  if (rpb > 0x3fffffff) return SM_ERR_UNSUPPORTED;
-  a.rpb = (int)rpb;
-  long long nb = 0;
+  // Element-wise: about 1024 blocks (all resident at once) of at least 4 rows per row lane.  Reductions: about 512 blocks of at least
+  // 2 rows per row lane; every element-wise block adds up the partials of its (image, level), so a level has no more row blocks than
+  // fit into GA_COMBINE entries (89 600 x 256 rows of five levels forward: 37 us with 64 row blocks to a level, 41 with 96), twice as
+  // many where the chip would else be empty (one 100 x 168 map backward: 45 us with 64, 36 with 128).
+  const long long total = rows * a.batch * a.ntile;
+  const long long arpb = std::max<long long>(4 * (GA_THREADS / a.ct), total / 1024);
+  const long long tiles_per_group = (a.cpg - 1) / tc + 2;
+  const long long smax = std::max<long long>(4, std::min<long long>(256, GA_COMBINE / (tiles_per_group * p->gpt)));
+  const long long few = (hw_max + smax - 1) / smax, many = (hw_max + 2 * smax - 1) / (2 * smax);
+  const long long srpb = std::max(std::max<long long>(2 * ((backward ? GA_SUM : GA_STAT) / a.ct), total / 512),
+                                  few > 0 && total / few < 256 ? many : few);
+  if (srpb > 0x3fffffff || arpb > 0x3fffffff) return SM_ERR_UNSUPPORTED;
+  a.srpb = (int)srpb, a.arpb = (int)arpb;
+  long long sb = 0, ab = 0;
   for (int l = 0; l < d->nlev; ++l) {
-    a.blk0[l] = (int)nb;
-    nb += (d->hw[l] + rpb - 1) / rpb;
-    if (nb > 0x7fffffff) return SM_ERR_UNSUPPORTED;
+    a.sblk0[l] = (int)sb, a.ablk0[l] = (int)ab;
+    sb += (d->hw[l] + srpb - 1) / srpb;
+    ab += (d->hw[l] + arpb - 1) / arpb;
+    if (ab > 0x7fffffff) return SM_ERR_UNSUPPORTED;
   }
-  for (int l = d->nlev; l <= SM_MAX_LEVELS; ++l) a.blk0[l] = (int)nb;
-  p->items = nb * a.batch;
+  for (int l = d->nlev; l <= SM_MAX_LEVELS; ++l) a.sblk0[l] = (int)sb, a.ablk0[l] = (int)ab;
+  p->items = sb * a.batch, p->ablocks = ab * a.batch;
   const long long nl = (long long)a.batch * a.nlev;
-  // (256 threads a block: a launch dimension holds fewer than 2^32 threads)
-  if (p->items > 0xfff000 || nl > 0x3ff000 || nl * a.G > 0x3ffc000) return SM_ERR_UNSUPPORTED;
+  // (a launch dimension holds fewer than 2^32 threads)
+  if (p->items > 0x3ff000 || p->ablocks + a.C / 32 > 0xfff000 || nl > 0x3ff000 || nl * a.G > 0x3fffffff) return SM_ERR_UNSUPPORTED;
   // One launch when a block can hold every row of its columns: the columns of whole groups, 8 (128 bytes of a row for 16-bit types) or
   // the next power of two that is a multiple of the group
   p->small_ct = 0;
@@ -728,8 +758,8 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, GaPlan* p) {
     const int nr = d->dtype == SM_DT_F32 ? ga_small_rows<SM_DT_F32> : ga_small_rows<SM_DT_BF16>;
     if (ct <= 32 && hw_max <= (long long)nr * (GA_SMALL / ct)) p->small_ct = ct;
   }
-  p->fwd_ws = p->small_ct ? 0 : (p->items * a.ntile * p->gpt + nl * a.G) * 16;
-  p->bwd_ws = p->small_ct ? nl * a.C * 16 : (p->items * a.C * 8 + 15) / 16 * 16 + nl * a.C * 16 + nl * a.G * 16;
+  p->fwd_ws = p->small_ct ? 0 : p->items * a.ntile * p->gpt * 16;
+  p->bwd_ws = p->small_ct ? nl * a.C * 16 : p->items * a.ntile * p->gpt * 16 + p->items * a.C * 8;
   return SM_OK;
 }
 
@@ -747,11 +777,10 @@ int ga_fwd_launch(const GaPlan& p, const void* x, const float* gamma, const floa
     }
   }
   double2* part = (double2*)ws;
-  double2* st = stats != nullptr ? (double2*)stats : part + p.items * a.ntile * p.gpt;
-  hipLaunchKernelGGL((ga_stats_kernel<DT, VEC, WHOLE>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s, (const T*)x, part, a, p.gpt);
-  hipLaunchKernelGGL(ga_combine_kernel, dim3((unsigned)((nl * a.G + 3) / 4)), dim3(GA_THREADS), 0, s, part, st, a, p.gpt, a.ct * VEC);
-  hipLaunchKernelGGL((ga_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s, (const T*)x,
-                     (T*)y, gamma, beta, st, a);
+  hipLaunchKernelGGL((ga_stats_kernel<DT, VEC, WHOLE>), dim3((unsigned)p.items, a.ntile), dim3(WHOLE ? GA_STAT : GA_STAT1), 0, s,
+                     (const T*)x, part, a, p.gpt);
+  hipLaunchKernelGGL((ga_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.ablocks, a.ntile), dim3(GA_THREADS), 0, s, (const T*)x,
+                     (T*)y, gamma, beta, part, (double2*)stats, a, p.gpt);
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
@@ -769,23 +798,19 @@ int ga_bwd_launch(const GaPlan& p, const void* x, const void* dy, const float* g
       hipLaunchKernelGGL((ga_small_bwd_kernel<DT, ACT, DROP>), dim3((unsigned)nl, sm_cdiv(a.cols, p.small_ct)), dim3(GA_SMALL), 0, s,
                          (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, (T*)dx, chan, chan ? nullptr : dgamma,
                          chan ? nullptr : dbeta, a, p.small_ct);
-      if (chan) hipLaunchKernelGGL(ga_param_grads_kernel, dim3(sm_cdiv(a.C, 32)), dim3(GA_THREADS), 0, s, chan, dgamma, dbeta, a);
+      if (chan) hipLaunchKernelGGL(ga_param_grads_kernel, dim3(sm_cdiv(a.C, 32)), dim3(GA_THREADS), 0, s, chan, nl, dgamma, dbeta, a);
       SM_LAUNCH_CHECK();
       return SM_OK;
     }
   }
-  float2* part = (float2*)ws;
-  double2* chan = (double2*)((char*)ws + (p.items * a.C * 8 + 15) / 16 * 16);
-  double2* gmean = chan + nl * a.C;
-  hipLaunchKernelGGL((ga_bwd_sum_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.items, a.ntile), dim3(GA_THREADS), 0, s,
-                     (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, part, a);
-  const int gb = std::max(1, 32 / a.cpg);
-  hipLaunchKernelGGL(ga_bwd_combine_kernel, dim3((unsigned)nl, sm_cdiv(a.G, gb)), dim3(1024), 0, s, part, gamma, chan, gmean, a, gb);
-  const long long rowb = dx != nullptr ? p.items : 0, chb = params ? sm_cdiv(a.C, 32) : 0;
+  double2* part = (double2*)ws;
+  float2* chan = (float2*)(part + p.items * a.ntile * p.gpt);
+  hipLaunchKernelGGL((ga_bwd_sum_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)p.items, a.ntile), dim3(GA_SUM), 0, s, (const T*)x,
+                     (const T*)dy, gamma, beta, (const double2*)stats, chan, part, a, p.gpt);
+  const long long rowb = dx != nullptr ? p.ablocks : 0, chb = params ? sm_cdiv(a.C, 32) : 0;
   if (rowb + chb > 0)
     hipLaunchKernelGGL((ga_bwd_apply_kernel<DT, VEC, WHOLE, ACT, DROP>), dim3((unsigned)(rowb + chb), a.ntile), dim3(GA_THREADS), 0, s,
-                       (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, (const double2*)chan, (const double2*)gmean,
-                       (T*)dx, dgamma, dbeta, a, rowb);
+                       (const T*)x, (const T*)dy, gamma, beta, (const double2*)stats, chan, part, (T*)dx, dgamma, dbeta, a, p.gpt, (int)chb);
   SM_LAUNCH_CHECK();
   return SM_OK;
 }
@@ -844,10 +869,10 @@ inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // a workspace serves either alignment
 extern "C" int64_t sm_group_norm_act_workspace(const sm_gn_act_desc* d, int backward) {
-  int64_t need = 16;
+  int64_t need = 0;
   for (int al = 0; al < 2; ++al) {
     GaPlan p;
-    const int st = ga_plan(d, al != 0, &p);
+    const int st = ga_plan(d, al != 0, backward != 0, &p);
     if (st != SM_OK) return st;
     need = std::max<int64_t>(need, backward ? p.bwd_ws : p.fwd_ws);
   }
@@ -857,7 +882,7 @@ extern "C" int64_t sm_group_norm_act_workspace(const sm_gn_act_desc* d, int back
 extern "C" int sm_group_norm_act(const sm_gn_act_desc* d, const void* x, const float* gamma, const float* beta, void* y, double* stats,
                                  void* workspace, int64_t workspace_bytes, sm_stream_t stream) {
   GaPlan p;
-  const int st = ga_plan(d, al16(x) && al16(y), &p);
+  const int st = ga_plan(d, al16(x) && al16(y), false, &p);
   if (st != SM_OK) return st;
   if (p.items == 0) return SM_OK;
   if (!x || !y || (p.fwd_ws > 0 && !workspace) || !al16(workspace) || (stats != nullptr && !al16(stats))) return SM_ERR_BAD_ARG;
@@ -869,7 +894,7 @@ extern "C" int sm_group_norm_act_bwd(const sm_gn_act_desc* d, const void* x, con
                                      const double* stats, void* dx, float* dgamma, float* dbeta, void* workspace,
                                      int64_t workspace_bytes, sm_stream_t stream) {
   GaPlan p;
-  const int st = ga_plan(d, al16(x) && al16(dy) && al16(dx), &p);
+  const int st = ga_plan(d, al16(x) && al16(dy) && al16(dx), true, &p);
   if (st != SM_OK) return st;
   hipStream_t s = sm_hip_stream(stream);
   if (p.items == 0) {          // no rows: the parameter gradients are sums over nothing

@@ -1509,7 +1509,7 @@ def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, s
         d.drop_seed, d.drop_offset = int(seed) & _MASK64, offset[0]
         d.drop_offset_dev = None if offset[1] is None else offset[1].data_ptr()
     stats = torch.empty(batch * len(hw) * groups, 2, dtype=torch.float64, device=x.device) if want_stats else None
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _lib.check(_lib.load().sm_group_norm_act(C.byref(d), _p(x), _p(gamma), _p(beta), _p(y), _p(stats), _p(ws), need, _stream(x)),
                "sm_group_norm_act")
     return d, bwd_need, stats
@@ -1518,7 +1518,7 @@ def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, s
 def group_norm_act_bwd(d, need, x, dy, dy_stride, dx, gamma, beta, stats, dgamma, dbeta):
     """dx (contiguous rows) and dgamma / dbeta f32 [C] are written where given"""
     d.dy_stride = dy_stride
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _lib.check(_lib.load().sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats), _p(dx), _p(dgamma), _p(dbeta),
                                                  _p(ws), need, _stream(x)), "sm_group_norm_act_bwd")
 
@@ -1586,7 +1586,7 @@ def fp8_matmul(a, a_block_rows, b, b_block_rows, m, n, k, bias, residual, relu, 
     if residual is not None:
         d.res_stride = row_stride(residual)
     y = torch.empty(m, n, dtype=out_dtype, device=device)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 16 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _lib.check(_lib.load().sm_fp8_matmul(C.byref(d), a.codes, a.scales, b.codes, b.scales, _p(bias), _p(residual), _p(y), _p(ws), need,
                                          _stream(y)), "sm_fp8_matmul")
     return y
@@ -1597,7 +1597,7 @@ def fp8_linear(x, b, b_block_rows, n, bias, relu, out_dtype):
     m, k = x.shape
     plan, _, need = _fp8_plan(m, n, k, 1, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
     y = torch.empty(m, n, dtype=out_dtype, device=x.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 16 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _lib.check(_lib.load().sm_fp8_linear(plan, dtype_code(x, "linear_fp8"), _p(x), row_stride(x), b.codes, b.scales, _p(bias), None, _p(y),
                                          _p(ws), need, _stream(x)), "sm_fp8_linear")
     return y

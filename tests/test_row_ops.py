@@ -93,9 +93,9 @@ def _gn_desc(**kw):
 def test_group_norm_workspace_is_host_arithmetic():
     lib = _lib.load()
     for back in (0, 1):
-        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc()), back) > 0
-        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc(batch=0)), back) > 0
-        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc(hw0=0)), back) > 0
+        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc(hw0=1000)), back) > 0
+        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc(batch=0)), back) == 0
+        assert lib.sm_group_norm_act_workspace(C.byref(_gn_desc(hw0=0)), back) >= 0
 
 
 @pytest.mark.parametrize("bad", [dict(nlev=0), dict(nlev=6), dict(batch=-1), dict(channels=0), dict(groups=0), dict(groups=7), dict(dtype=3),
