@@ -806,7 +806,7 @@ int sm_dropout(int dtype, const void* x, const void* residual, void* y, int64_t 
                const int64_t* offset_dev, sm_stream_t stream);
 
 /* ---------------------------------------------------------------- 8-bit (e4m3) products, one power-of-two scale per block of 128
- * A quantised matrix of rows x cols: codes (OCP e4m3) uint8 [ceil(cols / 128)][rows][128], 16-byte aligned, zero codes behind the last
+ * A quantised matrix of rows x cols: codes (OCP e4m3) uint8 [2 ceil(cols / 128)][rows][64], 16-byte aligned, zero codes behind the last
  * column; scales (E8M0: 2^(byte - 127)) uint8 [ceil(cols / 512)][ceil(rows / block_rows)][4], 4-byte aligned: the byte of K block kb and
  * row block r is [kb / 4][r][kb % 4], 127 behind the last block.  scale = smallest power of two >= 2^-127 with max |x| / scale <= 448
  * over the block of block_rows x 128 (1 for a block of zeros), code = x / scale rounded to nearest even; Inf and NaN become the NaN

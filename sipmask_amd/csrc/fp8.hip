@@ -14,10 +14,9 @@
 // (one conversion is 8 cycles; 16 of them beside 4 MFMAs measured 161 cycles against 154 for the MFMAs alone), and the bytes moved
 // through HBM and LDS stay 8-bit.
 //
-// Layout of a quantised matrix: codes [K block][row][128] (zero codes behind the last column), scales [K block / 4][row block][4]
-// (127, i.e. 1, behind the last block).  One K step of a tile is then one contiguous piece of memory: with codes [row][K] the rows of a
-// step lie K bytes apart, and for K a multiple of 4 KB they all fall on a few L2 channels (8192 x 4096 x 4096: 280 us with row-major
-// codes, 188 us with the loads left out).  A K loop reads four scales of a row as one dword, neighbouring rows side by side.
+// Layout of a quantised matrix: codes [K / 64][row][64] (two slabs per block of 128, zero codes behind the last column), scales
+// [K block / 4][row block][4] (127, i.e. 1, behind the last block).  One K step of a tile is then one contiguous piece of memory, and
+// a K loop reads four scales of a row as one dword, neighbouring rows side by side.
 #include <algorithm>
 #include <type_traits>
 
@@ -108,7 +107,8 @@ __global__ __launch_bounds__(256) void fp8_quant_rows_kernel(const typename Elem
     for (int p = 0; p < U; ++p) {
       const int kb = kq[p] * 4 + sub;
       const int sb = fp8_scale_byte(max16(fp8_amax<8>(f[p])));            // (a block behind the last column: zeros, 127)
-      if (kb < nkb) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r[p]) * 128 + l * 8) = fp8_pack8(f[p], fp8_inv_scale(sb));
+      if (kb < nkb)
+        *reinterpret_cast<uint2*>(q + ((long long)(kb * 2 + (l >> 3)) * rows + r[p]) * 64 + (l & 7) * 8) = fp8_pack8(f[p], fp8_inv_scale(sb));
       const uint32_t w = (uint32_t)__shfl(sb, 0, 64) | ((uint32_t)__shfl(sb, 16, 64) << 8) | ((uint32_t)__shfl(sb, 32, 64) << 16) |
                          ((uint32_t)__shfl(sb, 48, 64) << 24);
       if ((threadIdx.x & 63) == 0) *reinterpret_cast<uint32_t*>(scale + ((long long)kq[p] * rows + r[p]) * 4) = w;
@@ -182,7 +182,8 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
         sb = fp8_scale_byte(max16(fp8_amax<8>(f[u])));
         mine = cv == u ? sb : mine;
       }
-      if (r < rows) *reinterpret_cast<uint2*>(q + ((long long)kb * rows + r) * 128 + cv * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
+      if (r < rows)
+        *reinterpret_cast<uint2*>(q + ((long long)(kb * 2 + (cv >> 3)) * rows + r) * 64 + (cv & 7) * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
     }
     if (!SQUARE && cv < 8 && r0 + rl * 8 + cv < rows) put_scale(scale, r0 + rl * 8 + cv, rows, kb, nkb, mine);
   }
@@ -232,10 +233,10 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const int i = threadIdx.x + 256 * p, c = i >> 3, ch = i & 7, sw = c >> 3;
+    const int i = threadIdx.x + 256 * p, c = (i >> 2) & 127, ch = (i >> 9) * 4 + (i & 3), sw = c >> 3;   // slab, column, 16-byte chunk
     uint4 v = *reinterpret_cast<const uint4*>(s_q + c * 128 + ((ch ^ (sw >> 1)) * 16));
     if (sw & 1) v = make_uint4(v.z, v.w, v.x, v.y);
-    if (c0 + c < cols) *reinterpret_cast<uint4*>(qt + ((long long)kbt * cols + c0 + c) * 128 + ch * 16) = v;
+    if (c0 + c < cols) *reinterpret_cast<uint4*>(qt + ((long long)(kbt * 2 + (ch >> 2)) * cols + c0 + c) * 64 + (ch & 3) * 16) = v;
   }
 }
 
@@ -392,21 +393,34 @@ __device__ __forceinline__ void mm_tile(const MmArgs& a, long long& tm, int& tn)
   tm = bi * GM + (o - (long long)tn * h);
 }
 
-// Tile of BN weights x BM activations, waves of WN x WM, K steps of one block of 128 through two LDS stages filled by direct
-// global -> LDS loads.  A row of a stage is the 128 codes of one K block = 8 chunks of 16 bytes; chunk c of row r lies at slot
-// c ^ (r & 7), so the 32 rows that one fragment read touches spread over all banks.  The weights are the MFMA's first operand: a lane
-// of the accumulator then holds four consecutive n of one m.  The results leave through LDS (the stages are free by then), 64 x 64
-// at a time per wave, so that a store instruction writes whole 128-byte lines of a few rows instead of 16 bytes of 32 rows.
-template <int BN, int BM, int WN, int WM>
-__global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(const MmArgs a) {
+// s_waitcnt vmcnt(N) lgkmcnt(0) and a raw barrier: everything but this wave's N youngest loads has landed, nobody reads the stage
+// before any more -- and, unlike __syncthreads(), the younger stages stay in flight
+template <int N>
+__device__ __forceinline__ void mm_stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// LDS of a block: the stages, under which the epilogue's 8 KB per wave lie, and two sets of scales
+constexpr int mm_stage_lds(int bn, int bm, int waves, int nst) {
+  return (bn + bm) * 64 * nst > waves * 8192 ? (bn + bm) * 64 * nst : waves * 8192;
+}
+constexpr int mm_lds(int bn, int bm, int waves, int nst) { return mm_stage_lds(bn, bm, waves, nst) + (bn + bm) * 8; }
+
+// Tile of BN weights x BM activations, waves of WN x WM, K steps of 64 (half a scale block) through NST LDS stages filled by direct
+// global -> LDS loads, NST - 1 of them in flight.  A row of a stage is 64 codes = 4 chunks of 16 bytes; chunk c of row r lies at slot
+// c ^ (r / 2 & 3), so eight neighbouring rows of one chunk cover 128 bytes.  The weights are the MFMA's first operand: a lane of the
+// accumulator then holds four consecutive n of one m.  The results leave through LDS (the stages are free by then), 64 n x 32 m at a
+// time per wave, so that a store instruction writes whole 128-byte lines of a few rows instead of 16 bytes of 32 rows.
+template <int BN, int BM, int WN, int WM, int NST>
+__global__ __launch_bounds__((BN / WN) * (BM / WM) * 64, 4) void fp8_mm_kernel(const MmArgs a) {
   constexpr int WAVES = (BN / WN) * (BM / WM), TN = WN / 32, TM = WM / 32;
-  constexpr int STAGE = (BN + BM) * 128, PIECES = (BN + BM) / 8, PW = PIECES / WAVES;
-  static_assert(PIECES % WAVES == 0, "whole pieces per wave");
-  static_assert(WN % 64 == 0 && WM % 64 == 0 && 2 * STAGE >= WAVES * 16384, "64 x 64 floats per wave in the epilogue");
+  constexpr int STAGE = (BN + BM) * 64, PIECES = (BN + BM) / 16, PW = PIECES / WAVES;
+  static_assert(PIECES % WAVES == 0 && BN % 16 == 0, "whole pieces per wave, each all weights or all activations");
+  static_assert(WN % 64 == 0 && BN % 64 == 0 && BM % 64 == 0 && NST >= 2, "the epilogue takes 64 n x 32 m at a time");
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   typedef __attribute__((address_space(3))) void lds_void;
   typedef const __attribute__((address_space(1))) void glb_void;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];      // 2 * STAGE
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];      // mm_lds(BN, BM, WAVES, NST)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   long long tm;
   int tn;
@@ -415,42 +429,55 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
   const long long m0 = tm * BM;
   const int ks = blockIdx.y;
   const int kb0 = (int)((long long)ks * a.nkb / a.ksplit), kb1 = (int)((long long)(ks + 1) * a.nkb / a.ksplit);
+  const int nst = (kb1 - kb0) * 2;                                    // stages (>= 2: every split has a block)
 
-  // DMA sources: piece p = 8 rows; lane -> row p * 8 + lane / 8, the chunk that belongs into its slot.  Rows behind the end read the
+  // DMA sources: piece p = 16 rows; lane -> row p * 16 + lane / 4, the chunk that belongs into its slot.  Rows behind the end read the
   // last row (their results are not stored).
   const uint8_t* src[PW];
 #pragma unroll
   for (int i = 0; i < PW; ++i) {
-    const int row = (wave * PW + i) * 8 + (lane >> 3), ch = (lane & 7) ^ (row & 7);
+    const int row = (wave * PW + i) * 16 + (lane >> 2), ch = (lane & 3) ^ ((row >> 1) & 3);
     if (row < BN) {
       const int r = n0 + row < a.n ? n0 + row : a.n - 1;
-      src[i] = a.b + ((long long)kb0 * a.n + r) * 128 + ch * 16;
+      src[i] = a.b + ((long long)kb0 * 2 * a.n + r) * 64 + ch * 16;
     } else {
       const long long r = m0 + row - BN < a.m ? m0 + row - BN : a.m - 1;
-      src[i] = a.a + ((long long)kb0 * a.m + r) * 128 + ch * 16;
+      src[i] = a.a + ((long long)kb0 * 2 * a.m + r) * 64 + ch * 16;
     }
   }
-  static_assert(BN % (8 * PW) == 0, "a wave's pieces are all weights or all activations");
-  const long long kstep = (wave * PW * 8 < BN ? (long long)a.n : a.m) * 128;
-  auto dma = [&](int buf) {                      // the next K block
+  const long long kn = (long long)a.n * 64, km = a.m * 64;
+  auto dma = [&](int buf) {                      // the next K step
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       __builtin_amdgcn_global_load_lds((glb_void*)src[i], (lds_void*)((lds_u8*)smem + buf * STAGE + (wave * PW + i) * 1024), 16, 0, 0);
-      src[i] += kstep;
+      src[i] += (wave * PW + i) * 16 < BN ? kn : km;
     }
   };
   const int wn = (wave % (BN / WN)) * WN, wm = (wave / (BN / WN)) * WM, l31 = lane & 31, kh = lane >> 5;
-  const uint8_t *ps_n[TN], *ps_m[TM];
+  // scales: four K blocks of all rows at a time, also by direct loads (a dword per row; as ordinary loads the wait for them, on the same
+  // in-order counter, drained the stages in flight), the next four blocks' while the present four are at work
+  constexpr int SROWS = BN + BM, SOFF = mm_stage_lds(BN, BM, WAVES, NST);
+  uint8_t* const s_scale = smem + SOFF;                        // [2][SROWS][4]
+  const int qlast = (a.nkb - 1) >> 2;
+  auto scales = [&](int quad) {
+    const long long q = std::min(quad, qlast);
 #pragma unroll
-  for (int i = 0; i < TN; ++i) {
-    const int r = std::min(n0 + wn + i * 32 + l31, a.n - 1);
-    ps_n[i] = a.sb + (long long)(r >> a.shb) * 4;
-  }
+    for (int p = 0; p < (SROWS / 64 + WAVES - 1) / WAVES; ++p) {
+      const int piece = wave + p * WAVES;
+      if (piece < SROWS / 64) {                                       // (wave-uniform)
+        const int row = piece * 64 + lane;
+        const uint8_t* g;
+        if (piece * 64 < BN) g = a.sb + (q * a.nsb + (std::min(n0 + row, a.n - 1) >> a.shb)) * 4;
+        else g = a.sa + (q * a.nsa + (std::min<long long>(m0 + row - BN, a.m - 1) >> a.sha)) * 4;
+        __builtin_amdgcn_global_load_lds((glb_void*)g, (lds_void*)((lds_u8*)smem + SOFF + ((quad & 1) * SROWS + piece * 64) * 4), 4, 0, 0);
+      }
+    }
+  };
+  scales(kb0 >> 2);
+  scales((kb0 >> 2) + 1);
 #pragma unroll
-  for (int j = 0; j < TM; ++j) {
-    const long long r = std::min<long long>(m0 + wm + j * 32 + l31, a.m - 1);
-    ps_m[j] = a.sa + (r >> a.sha) * 4;
-  }
+  for (int t = 0; t < NST - 1; ++t)
+    if (t < nst) dma(t);
   f32x16 acc[TN][TM];
 #pragma unroll
   for (int i = 0; i < TN; ++i)
@@ -458,91 +485,76 @@ __global__ __launch_bounds__((BN / WN) * (BM / WM) * 64) void fp8_mm_kernel(cons
     for (int j = 0; j < TM; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  // 16 codes of a row: chunk c = 2 step + lane / 32 of the K block (the order of k inside a block is free as long as both operands
-  // share it), two MFMA operands of 8 values
-  const int rsw = l31 & 7;                       // every fragment row is l31 plus a multiple of 32
-  const uint8_t* const fbase_n = smem + (wn + l31) * 128;
-  const uint8_t* const fbase_m = smem + (BN + wm + l31) * 128;
-  // scales of the four K blocks at hand and of the next four: requested four steps before their use, so that no step waits for a load
-  // (the memory counter is in order: a wait for a scale is a wait for the whole stage in flight)
-  uint32_t dn[TN], dm[TM], en[TN], em[TM];
-  const int qlast = (a.nkb - 1) >> 2;
-  auto scales = [&](int quad, uint32_t (&n_)[TN], uint32_t (&m_)[TM]) {
-    const long long q4 = (long long)std::min(quad, qlast) * 4;
+  // 16 codes of a row: chunk 2 step + lane / 32 of the stage (the order of k inside a block is free as long as both operands share
+  // it), two MFMA operands of 8 values
+  const int rsw = (l31 >> 1) & 3;                // every fragment row is l31 plus a multiple of 32
+  const uint8_t* const fbase_n = smem + (wn + l31) * 64;
+  const uint8_t* const fbase_m = smem + (BN + wm + l31) * 64;
+  float sn[TN], sm[TM];
+  int buf = 0, fill = NST - 1;                   // the stage at hand, the one that the next loads go to
+  for (int t = 0; t < nst; ++t) {
+    // stage t has landed when at most the loads of the NST - 2 stages behind it are outstanding (other loads in between only make
+    // the wait stricter); behind the barrier stage t - 1, which everybody has read, is filled again
+    if (t + NST - 2 < nst) mm_stage_barrier<(NST - 2) * PW>();
+    else mm_stage_barrier<0>();
+    if (t + NST - 1 < nst) dma(fill);
+    const int kb = kb0 + (t >> 1);
+    if ((t & 1) == 0) {
+      if ((kb & 3) == 0 && t != 0) scales((kb >> 2) + 1);             // (into the half that the four blocks before this one used)
+      const uint8_t* const sc = s_scale + ((kb >> 2) & 1) * SROWS * 4 + (kb & 3);
 #pragma unroll
-    for (int i = 0; i < TN; ++i) n_[i] = *reinterpret_cast<const uint32_t*>(ps_n[i] + q4 * a.nsb);
+      for (int i = 0; i < TN; ++i) sn[i] = fp8_scale_float(sc[(wn + i * 32 + l31) * 4]);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) m_[j] = *reinterpret_cast<const uint32_t*>(ps_m[j] + q4 * a.nsa);
-  };
-  scales(kb0 >> 2, dn, dm);
-  scales((kb0 >> 2) + 1, en, em);
-  i32x4 fn[2][TN], fm[2][TM];
-  auto read = [&](int set, int buf, int step) {
-    const int o = buf * STAGE + ((step * 2 + kh) ^ rsw) * 16;
-#pragma unroll
-    for (int i = 0; i < TN; ++i) fn[set][i] = *reinterpret_cast<const i32x4*>(fbase_n + o + i * 32 * 128);
-#pragma unroll
-    for (int j = 0; j < TM; ++j) fm[set][j] = *reinterpret_cast<const i32x4*>(fbase_m + o + j * 32 * 128);
-  };
-  if (kb0 < kb1) dma(0);
-  __syncthreads();
-  for (int kb = kb0; kb < kb1; ++kb) {
-    const int buf = (kb - kb0) & 1;
-    if (kb + 1 < kb1) dma(buf ^ 1);
-    if ((kb & 3) == 0 && kb != kb0) {
-#pragma unroll
-      for (int i = 0; i < TN; ++i) dn[i] = en[i];
-#pragma unroll
-      for (int j = 0; j < TM; ++j) dm[j] = em[j];
-      scales((kb >> 2) + 1, en, em);
+      for (int j = 0; j < TM; ++j) sm[j] = fp8_scale_float(sc[(BN + wm + j * 32 + l31) * 4]);
     }
-    const int sh = (kb & 3) * 8;
-    float sn[TN], sm[TM];
+    i32x4 fn[2][TN], fm[2][TM];
+    auto read = [&](int step) {
+      const int o = buf * STAGE + ((step * 2 + kh) ^ rsw) * 16;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) sn[i] = fp8_scale_float(dn[i] >> sh);
+      for (int i = 0; i < TN; ++i) fn[step][i] = *reinterpret_cast<const i32x4*>(fbase_n + o + i * 32 * 64);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) sm[j] = fp8_scale_float(dm[j] >> sh);
-    read(0, buf, 0);
+      for (int j = 0; j < TM; ++j) fm[step][j] = *reinterpret_cast<const i32x4*>(fbase_m + o + j * 32 * 64);
+    };
+    read(0);
+    read(1);
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      const int set = step & 1;
-      if (step < 3) read(set ^ 1, buf, step + 1);
+    for (int step = 0; step < 2; ++step) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         bf16x8 on[TN], om[TM];
 #pragma unroll
-        for (int i = 0; i < TN; ++i) on[i] = fp8_widen8(fn[set][i][2 * h], fn[set][i][2 * h + 1], sn[i]);
+        for (int i = 0; i < TN; ++i) on[i] = fp8_widen8(fn[step][i][2 * h], fn[step][i][2 * h + 1], sn[i]);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) om[j] = fp8_widen8(fm[set][j][2 * h], fm[set][j][2 * h + 1], sm[j]);
+        for (int j = 0; j < TM; ++j) om[j] = fp8_widen8(fm[step][j][2 * h], fm[step][j][2 * h + 1], sm[j]);
 #pragma unroll
         for (int i = 0; i < TN; ++i)
 #pragma unroll
           for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(on[i], om[j], acc[i][j], 0, 0, 0);
       }
     }
-    __syncthreads();
+    buf = buf + 1 == NST ? 0 : buf + 1;
+    fill = fill + 1 == NST ? 0 : fill + 1;
   }
-  // accumulator e of a lane: n = 8 (e / 4) + 4 (lane / 32) + e % 4, m = lane % 32.  64 m x 64 n floats of this wave's own LDS, the
+  __syncthreads();                               // (no load is in flight: the last stages waited for all of them)
+  // accumulator e of a lane: n = 8 (e / 4) + 4 (lane / 32) + e % 4, m = lane % 32.  32 m x 64 n floats of this wave's own LDS, the
   // 16-byte chunk n / 4 of row m at slot (n / 4) ^ (m & 15); the reads follow the writes of the same wave in order
-  float* const E = reinterpret_cast<float*>(smem) + wave * 4096;
-  mm_for<TN / 2 * (TM / 2)>([&](auto IP) {       // (an unrolled loop of this size leaves acc indexed at run time, in scratch)
-    constexpr int ip = decltype(IP)::value % (TN / 2), jp = decltype(IP)::value / (TN / 2);
+  float* const E = reinterpret_cast<float*>(smem) + wave * 2048;
+  mm_for<TN / 2 * TM>([&](auto IJ) {             // (an unrolled loop of this size leaves acc indexed at run time, in scratch)
+    constexpr int ip = decltype(IJ)::value % (TN / 2), j = decltype(IJ)::value / (TN / 2);
 #pragma unroll
     for (int i2 = 0; i2 < 2; ++i2)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int m = j * 32 + l31, c = i2 * 8 + g * 2 + kh;
-          const f32x16 t = acc[ip * 2 + i2][jp * 2 + j];
-          *reinterpret_cast<float4*>(E + m * 64 + ((c ^ (m & 15)) * 4)) = make_float4(t[4 * g], t[4 * g + 1], t[4 * g + 2], t[4 * g + 3]);
-        }
+      for (int g = 0; g < 4; ++g) {
+        const int c = i2 * 8 + g * 2 + kh;
+        const f32x16 t = acc[ip * 2 + i2][j];
+        *reinterpret_cast<float4*>(E + l31 * 64 + ((c ^ (l31 & 15)) * 4)) = make_float4(t[4 * g], t[4 * g + 1], t[4 * g + 2], t[4 * g + 3]);
+      }
     __builtin_amdgcn_wave_barrier();
     const int cl = (lane & 7) * 2, n = n0 + wn + ip * 64 + cl * 4;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < 4; ++r) {
       const int ml = r * 8 + (lane >> 3);
-      const long long m = m0 + wm + jp * 64 + ml;
+      const long long m = m0 + wm + j * 32 + ml;
       const float4 p = *reinterpret_cast<const float4*>(E + ml * 64 + ((cl ^ (ml & 15)) * 4));
       const float4 q = *reinterpret_cast<const float4*>(E + ml * 64 + (((cl + 1) ^ (ml & 15)) * 4));
       float v[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
@@ -576,7 +588,7 @@ __global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const 
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
   for (int kb = wave; kb < a.nkb; kb += WAVES) {
-    const i32x4* pw = reinterpret_cast<const i32x4*>(a.b + ((long long)kb * a.n + n) * 128 + g * 32);
+    const i32x4* pw = reinterpret_cast<const i32x4*>(a.b + ((long long)(kb * 2 + (g >> 1)) * a.n + n) * 64 + (g & 1) * 32);
     const i32x4 w0 = pw[0], w1 = pw[1];
     const float sw = fp8_scale_float(a.sb[((long long)(kb >> 2) * a.nsb + (n >> a.shb)) * 4 + (kb & 3)]);
     const bf16x8 on[4] = {fp8_widen8(w0[0], w0[1], sw), fp8_widen8(w0[2], w0[3], sw), fp8_widen8(w1[0], w1[1], sw), fp8_widen8(w1[2], w1[3], sw)};
@@ -584,7 +596,7 @@ __global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const 
     for (int t = 0; t < MT; ++t) {
       bf16x8 om[4];
       if constexpr (SRC == 3) {
-        const i32x4* pa = reinterpret_cast<const i32x4*>(a.a + ((long long)kb * a.m + row[t]) * 128 + g * 32);
+        const i32x4* pa = reinterpret_cast<const i32x4*>(a.a + ((long long)(kb * 2 + (g >> 1)) * a.m + row[t]) * 64 + (g & 1) * 32);
         const i32x4 a0 = pa[0], a1 = pa[1];
         const float sm = fp8_scale_float(a.sa[((long long)(kb >> 2) * a.nsa + (row[t] >> a.sha)) * 4 + (kb & 3)]);
         om[0] = fp8_widen8(a0[0], a0[1], sm), om[1] = fp8_widen8(a0[2], a0[3], sm);
@@ -647,16 +659,21 @@ __global__ __launch_bounds__(256) void fp8_mm_finish_kernel(const MmArgs a) {
 }
 
 struct MmPlan {
-  int few, big, ksplit;              // few: fp8_mm_few_kernel; big: 256 x 256 tiles
+  int few, bm, ksplit;               // few: fp8_mm_few_kernel; bm: activations per tile (of 128 weights)
   long long tm;
   int tn;
   long long ws;
 };
 
-// MM_FEW rows or fewer: fp8_mm_few_kernel.
-// 256 x 256 tiles (a wave widens 3 pairs of codes per MFMA, one block fills a CU and nothing covers its epilogue) when they fill the chip
-// and K is long, 128 x 128 (4 pairs per MFMA, two blocks per CU) else: 230 against 245 us at 8192 x 4096 x 4096, but 91 against 74 us at
-// 67200 x 512 x 768.  K is split while there are fewer than two small tiles per CU and every split keeps four blocks of 128.
+// Which kernel (us at m x n x k; the other sides measured in the same run):
+//   up to MM_FEW rows    fp8_mm_few_kernel
+//   256 x 128 tiles      long K and enough of them for two blocks per CU: half the bytes per MFMA (8192 x 4096 x 4096: 217, 128 rows 230)
+//   128 x 128            at least 512 of them, or a K long enough to make 512 by splitting with 16 blocks of 128 to each split (the
+//                        weight gradients: 512 x 768 x 67200: 60, 64 rows 67; 67200 x 512 x 768: 58, 64 rows 62, 256 rows 59)
+//   64 x 128             everything between: twice the blocks hide each other's latency, for 6 instead of 4 conversions per MFMA
+//                        (16800 x 256 x 1024: 17 against 20, 4200 x 512 x 2048: 21 / 26, 977 x 333 x 1131: 15 / 19)
+// K is split until there are 512 blocks, as long as every split keeps four blocks of 128.
+constexpr int MM_BLOCKS = 512;
 // Up to MM_FEW_QUANT rows the few-rows kernel quantises x itself, in every block again (15 us a call of 7 x 4096 x 4096 either way on
 // the host, but one launch instead of two); with 64 rows that repeated work took 28 us against 10 behind a quantiser launch.
 constexpr int MM_FEW = 64, MM_FEW_QUANT = 16;
@@ -667,16 +684,16 @@ int mm_plan(const sm_fp8_matmul_desc* d, MmPlan* p) {
       d->out_dtype < SM_DT_BF16 || d->out_dtype > SM_DT_F32)
     return SM_ERR_BAD_ARG;
   if (d->y_stride < d->n || d->n > 0x7fffff00 || d->k > 0x7fffff00) return SM_ERR_BAD_SHAPE;
-  const long long big = ((d->m + 255) / 256) * sm_cdiv(d->n, 256);
   p->few = d->m <= MM_FEW;
-  p->big = big >= 256 && d->k >= 2048;
-  const int t = p->big ? 256 : 128;
-  p->tm = (d->m + t - 1) / t;
-  p->tn = sm_cdiv(d->n, t);
+  const long long tn = sm_cdiv(d->n, 128);
   const int nkb = sm_cdiv(d->k, 128);
+  const long long t128 = (d->m + 127) / 128 * tn;
+  p->bm = d->k >= 2048 && (d->m + 255) / 256 * tn >= MM_BLOCKS ? 256 : (t128 >= MM_BLOCKS || t128 * nkb >= 16 * MM_BLOCKS ? 128 : 64);
+  p->tm = (d->m + p->bm - 1) / p->bm;
+  p->tn = (int)tn;
   const long long tiles = p->tm * p->tn;
   if (tiles > 0xfff000) return SM_ERR_UNSUPPORTED;
-  p->ksplit = tiles == 0 || p->big || p->few ? 1 : (int)std::max<long long>(1, std::min<long long>(512 / tiles, nkb / 4));
+  p->ksplit = tiles == 0 || p->few ? 1 : (int)std::max<long long>(1, std::min<long long>(MM_BLOCKS / tiles, nkb / 4));
   p->ws = p->ksplit > 1 ? (long long)p->ksplit * d->m * d->n * 4 : 0;
   return SM_OK;
 }
@@ -781,6 +798,14 @@ void mm_few_launch(const MmArgs& k, const void* x, long long ldx, long long cols
   hipLaunchKernelGGL((fp8_mm_few_kernel<SRC, VEC, 1>), dim3(sm_cdiv(k.n, 16)), dim3(1024), 0, s, k, x, ldx, cols);
 }
 
+// tiles of 128 weights x BM activations, waves of 64 x WM, two stages
+template <int BM, int WM>
+void mm_launch(const MmArgs& k, dim3 grid, hipStream_t s) {
+  constexpr int waves = 2 * (BM / WM), lds = mm_lds(128, BM, waves, 2);
+  if (lds > 65536) (void)sm_lds_optin((const void*)fp8_mm_kernel<128, BM, 64, WM, 2>, lds);     // (a refusal shows in the launch check)
+  hipLaunchKernelGGL((fp8_mm_kernel<128, BM, 64, WM, 2>), grid, dim3(waves * 64), lds, s, k);
+}
+
 // the product behind its checks.  x != null: a is quantised from it (x_dtype, row stride ldx) -- by the few-rows kernel itself, else into
 // the workspace behind the K splits' partials
 int mm_run(const sm_fp8_matmul_desc* d, const MmPlan& p, const void* a, const void* a_scale, const void* b, const void* b_scale,
@@ -819,13 +844,9 @@ int mm_run(const sm_fp8_matmul_desc* d, const MmPlan& p, const void* a, const vo
     return SM_OK;
   }
   const dim3 grid((unsigned)(p.tm * p.tn), p.ksplit);
-  if (p.big) {
-    const void* kern = (const void*)fp8_mm_kernel<256, 256, 128, 64>;
-    if (sm_lds_optin(kern, 131072) != hipSuccess) return SM_ERR_LAUNCH;
-    hipLaunchKernelGGL((fp8_mm_kernel<256, 256, 128, 64>), grid, dim3(512), 131072, s, k);
-  } else {
-    hipLaunchKernelGGL((fp8_mm_kernel<128, 128, 64, 64>), grid, dim3(256), 65536, s, k);
-  }
+  if (p.bm == 256) mm_launch<256, 64>(k, grid, s);
+  else if (p.bm == 128) mm_launch<128, 64>(k, grid, s);
+  else mm_launch<64, 32>(k, grid, s);
   if (p.ksplit > 1) {
     const long long total = k.m * ((k.n + 3) / 4);
     hipLaunchKernelGGL(fp8_mm_finish_kernel, dim3((unsigned)std::min<long long>((total + 255) / 256, 256 * 16)), dim3(256), 0, s, k);

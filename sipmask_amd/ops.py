@@ -488,7 +488,7 @@ def dropout(x, p, seed, offset=0, residual=None, training=True):
 # ------------------------------------------------------------------------------- 8-bit products
 class Fp8Blocks:
     """A matrix [rows, cols] in e4m3 with one power-of-two scale per block of block_rows x 128, laid out for the product:
-    `codes` float8_e4m3fn [ceil(cols / 128), rows, 128], `scales` uint8 (2^(byte - 127)) [ceil(cols / 512), ceil(rows / block_rows),
+    `codes` float8_e4m3fn [2 ceil(cols / 128), rows, 64], `scales` uint8 (2^(byte - 127)) [ceil(cols / 512), ceil(rows / block_rows),
     4].  code_matrix() / scale_matrix() put them back in rows."""
     __slots__ = ("codes", "scales", "rows", "cols", "block_rows")
 
@@ -536,7 +536,7 @@ def quantize_fp8(x, block_rows=1, transpose=False):
         rows, cols, _ = H.fp8_quantize(x, block_rows, not transpose, transpose)
     (r, c), buf = (x.shape, rows) if not transpose else ((x.shape[1], x.shape[0]), cols)
     nc = H.fp8_bytes(r, c, block_rows)[0]
-    return Fp8Blocks(buf.data[:nc].view(torch.float8_e4m3fn).view(-(-c // 128), r, 128),
+    return Fp8Blocks(buf.data[:nc].view(torch.float8_e4m3fn).view(-(-c // 128) * 2, r, 64),
                      buf.data[nc:].view(-(-c // 512), -(-r // block_rows), 4), r, c, block_rows)
 
 
@@ -546,7 +546,7 @@ class _Fp8Operand:
 
     def __init__(self, t):
         if t.codes.dtype != torch.float8_e4m3fn or t.scales.dtype != torch.uint8 or not t.codes.is_contiguous() or \
-                not t.scales.is_contiguous() or t.codes.shape != (-(-t.cols // 128), t.rows, 128) or \
+                not t.scales.is_contiguous() or t.codes.shape != (-(-t.cols // 128) * 2, t.rows, 64) or \
                 t.scales.shape != (-(-t.cols // 512), -(-t.rows // t.block_rows), 4) or t.scales.device != t.codes.device:
             raise ValueError("Fp8Blocks of %s: codes %s, scales %s do not have its layout" % (t.shape, tuple(t.codes.shape), tuple(t.scales.shape)))
         self.codes, self.scales = t.codes.data_ptr(), t.scales.data_ptr()

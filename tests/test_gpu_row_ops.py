@@ -379,7 +379,7 @@ def test_quantize_fp8_codes_and_scales(rows, cols, block_rows, transpose, dtype)
     code, byte, val = R.fp8_quantize(src, block_rows)
     r, c = src.shape
     nkb = -(-c // 128)
-    assert q.shape == (r, c) and q.codes.shape == (nkb, r, 128) and q.scales.shape == (-(-nkb // 4), byte.shape[0], 4)
+    assert q.shape == (r, c) and q.codes.shape == (2 * nkb, r, 64) and q.scales.shape == (-(-nkb // 4), byte.shape[0], 4)
     got = q.code_matrix().view(torch.uint8)
     zero = (code & 0x7F) == 0                                              # (+0 and -0 stand for the same value)
     assert torch.equal(torch.where(zero, code & 0x7F, code), torch.where(zero, got & 0x7F, got))
@@ -431,7 +431,8 @@ def test_quantize_fp8_strided_rows():
 
 
 MM_SHAPES = [(1, 1, 1), (1, 8, 128), (7, 512, 2048), (16, 33, 130), (17, 64, 64), (33, 3, 2000), (64, 64, 1000), (128, 128, 128), (129, 257, 385),
-             (300, 130, 16), (977, 333, 1131), (5, 1000, 4096), (2048, 256, 512), (700, 900, 640)]
+             (300, 130, 16), (977, 333, 1131), (5, 1000, 4096), (2048, 256, 512), (700, 900, 640), (4100, 2050, 140),
+             (500, 700, 44100), (8200, 2040, 2056)]
 
 
 @pytest.mark.parametrize("m,n,k", MM_SHAPES)
