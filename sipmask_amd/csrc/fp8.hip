@@ -73,6 +73,40 @@ __device__ __forceinline__ uint2 fp8_pack8(const float* f, float inv) {
   return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 
+// 8 consecutive values of a row from column c as they came from memory (any alignment: as floats); columns >= cols are 0
+template <int DT, bool VEC>
+struct Raw8 {
+  typename Elem<DT>::raw8 q;
+  __device__ __forceinline__ void load(const typename Elem<DT>::type* row, long long c, long long cols) {
+    if (c + 8 <= cols) {
+      q = Elem<DT>::load8(row + c);
+    } else {
+      typename Elem<DT>::type t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = c + e < cols ? row[c + e] : typename Elem<DT>::type(0);
+      q = __builtin_bit_cast(typename Elem<DT>::raw8, t);
+    }
+  }
+  __device__ __forceinline__ void zero() { q = typename Elem<DT>::raw8{}; }
+  __device__ __forceinline__ void get(float* f) const { Elem<DT>::unpack(q, f); }
+};
+template <int DT>
+struct Raw8<DT, false> {
+  float v[8];
+  __device__ __forceinline__ void load(const typename Elem<DT>::type* row, long long c, long long cols) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? Elem<DT>::load(row + c + e) : 0.f;
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = v[e];
+  }
+};
+
 // 8 consecutive values of a row from column c; columns >= cols read as 0
 template <int DT, bool VEC>
 __device__ __forceinline__ void fp8_load8(const typename Elem<DT>::type* row, long long c, long long cols, float* f) {
@@ -134,23 +168,34 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   __shared__ __attribute__((aligned(16))) uint8_t s_q[128 * 128];
   const long long rb = blockIdx.x, r0 = rb * 128, c0 = (long long)blockIdx.y * 128;
   const int cv = threadIdx.x & 15, rl = threadIdx.x >> 4;
-  float f[8][8];
+  // the values stay as they came (16-bit: half the registers of floats, twice the blocks per CU) and are widened again where needed
+  Raw8<DT, VEC> x8[8];
+  uint32_t open[2] = {~0u, ~0u};                 // gate bits of rows 0 - 3 and 4 - 7, 8 columns each
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const long long r = r0 + rl * 8 + u;
-    if (r < rows) {
-      fp8_load8<DT, VEC>(x + r * ldx, c0 + cv * 8, cols, f[u]);
-      if (gate != nullptr) {
-        float g[8];
-        fp8_load8<DT, VEC>(gate + r * ldg, c0 + cv * 8, cols, g);
+    if (r < rows) x8[u].load(x + r * ldx, c0 + cv * 8, cols);
+    else x8[u].zero();
+  }
+  if (gate != nullptr) {
+    open[0] = open[1] = 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[u][e] = g[e] > 0.f ? f[u][e] : 0.f;
-      }
-    } else {
+    for (int u = 0; u < 8; ++u) {
+      const long long r = r0 + rl * 8 + u;
+      if (r >= rows) continue;
+      float g[8];
+      fp8_load8<DT, VEC>(gate + r * ldg, c0 + cv * 8, cols, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[u][e] = 0.f;
+      for (int e = 0; e < 8; ++e) open[u >> 2] |= g[e] > 0.f ? 1u << ((u & 3) * 8 + e) : 0u;
     }
   }
+  auto row = [&](int u, float (&f)[8]) {
+    x8[u].get(f);
+    if (gate != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (open[u >> 2] >> ((u & 3) * 8 + e)) & 1u ? f[e] : 0.f;
+    }
+  };
   // byte of block kb of a scale row; the last block of a row fills the dword up with 127
   auto put_scale = [](uint8_t* base, long long r, long long nr, int kb, int nb, int byte) {
     uint8_t* p = base + ((long long)(kb >> 2) * nr + r) * 4;
@@ -161,7 +206,14 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   const int kb = (int)(c0 >> 7), kbt = (int)rb;
   int block_byte = 127;
   if constexpr (SQUARE) {
-    float m = max16(fp8_amax<64>(&f[0][0]));
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      float f[8];
+      row(u, f);
+      m = fmaxf(m, fp8_amax<8>(f));
+    }
+    m = max16(m);
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
     if ((threadIdx.x & 63) == 0) s_wmax[threadIdx.x >> 6] = m;
@@ -177,24 +229,29 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const long long r = r0 + rl * 8 + u;
+      float f[8];
+      row(u, f);
       int sb = block_byte;
       if constexpr (!SQUARE) {
-        sb = fp8_scale_byte(max16(fp8_amax<8>(f[u])));
+        sb = fp8_scale_byte(max16(fp8_amax<8>(f)));
         mine = cv == u ? sb : mine;
       }
       if (r < rows)
-        *reinterpret_cast<uint2*>(q + ((long long)(kb * 2 + (cv >> 3)) * rows + r) * 64 + (cv & 7) * 8) = fp8_pack8(f[u], fp8_inv_scale(sb));
+        *reinterpret_cast<uint2*>(q + ((long long)(kb * 2 + (cv >> 3)) * rows + r) * 64 + (cv & 7) * 8) = fp8_pack8(f, fp8_inv_scale(sb));
     }
     if (!SQUARE && cv < 8 && r0 + rl * 8 + cv < rows) put_scale(scale, r0 + rl * 8 + cv, rows, kb, nkb, mine);
   }
   if (colsum != nullptr) {
+    float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float t = 0.f;
+    for (int u = 0; u < 8; ++u) {
+      float f[8];
+      row(u, f);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) t += f[u][e];
-      s_red[rl][cv * 8 + e] = t;
+      for (int e = 0; e < 8; ++e) t[e] += f[e];
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_red[rl][cv * 8 + e] = t[e];
     __syncthreads();
     if (threadIdx.x < 128 && c0 + threadIdx.x < cols) {
       float t = 0.f;
@@ -206,11 +263,30 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   }
   if (qt == nullptr) return;
   if constexpr (!SQUARE) {
+    float m[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    bool inf = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t[8] = {f[0][e], f[1][e], f[2][e], f[3][e], f[4][e], f[5][e], f[6][e], f[7][e]};
-      s_red[rl][cv * 8 + e] = fp8_amax<8>(t);
+    for (int u = 0; u < 8; ++u) {
+      float f[8];
+      row(u, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[e] = fmaxf(m[e], __builtin_fabsf(f[e]));
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) inf |= m[e] > 3.402823466e38f;
+    if (inf) {                                   // (see fp8_amax)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[e] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float f[8];
+        row(u, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m[e] = fmaxf(m[e], fp8_abs_finite(f[e]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_red[rl][cv * 8 + e] = m[e];
     __syncthreads();
     if (threadIdx.x < 128) {
       float m = 0.f;
@@ -224,12 +300,25 @@ __global__ __launch_bounds__(256) void fp8_quant_pair_kernel(const typename Elem
   }
   // the transpose goes through LDS: 8 rows of a column = 8 bytes, chunk rl of column c at slot rl ^ (c / 8) (16 columns of a wave's
   // write then lie in 16 different slots)
+  // (two rows at a time: v_cvt_pk_fp8_f32 takes a pair; the codes of rows 2 h, 2 h + 1 of a column are half of its dword h / 2)
+  float inv[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float inv = fp8_inv_scale(SQUARE ? block_byte : s_byte[cv * 8 + e]);
-    const float t[8] = {f[0][e], f[1][e], f[2][e], f[3][e], f[4][e], f[5][e], f[6][e], f[7][e]};
-    *reinterpret_cast<uint2*>(s_q + (cv * 8 + e) * 128 + ((rl ^ cv) * 8)) = fp8_pack8(t, inv);
+  for (int e = 0; e < 8; ++e) inv[e] = fp8_inv_scale(SQUARE ? block_byte : s_byte[cv * 8 + e]);
+  int code[8][2];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    float f[8], g[8];
+    row(2 * h, f);
+    row(2 * h + 1, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (h & 1) code[e][h >> 1] = __builtin_amdgcn_cvt_pk_fp8_f32(f[e] * inv[e], g[e] * inv[e], code[e][h >> 1], true);
+      else code[e][h >> 1] = __builtin_amdgcn_cvt_pk_fp8_f32(f[e] * inv[e], g[e] * inv[e], 0, false);
+    }
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    *reinterpret_cast<uint2*>(s_q + (cv * 8 + e) * 128 + ((rl ^ cv) * 8)) = make_uint2((uint32_t)code[e][0], (uint32_t)code[e][1]);
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
