@@ -85,8 +85,20 @@ class SipMaskHead(nn.Module):
                  loss_cls=dict(type='FocalLoss', use_sigmoid=True, gamma=2.0, alpha=0.25, loss_weight=1.0),
                  loss_bbox=dict(type='IoULoss', loss_weight=1.0),
                  loss_centerness=dict(type='CrossEntropyLoss', use_sigmoid=True, loss_weight=1.0),
-                 conv_cfg=None, norm_cfg=dict(type='GN', num_groups=32, requires_grad=True)):
+                 conv_cfg=None, norm_cfg=dict(type='GN', num_groups=32, requires_grad=True), tower_dropout=0.0,
+                 tower_dropout_seed=0, mask_lat_fp8=False):
+        """tower_dropout (this framework's own, off by default): probability with which each tower layer's output is dropped while
+        training.  The masks are a function of (tower_dropout_seed, rank, number of the layer call since construction), so a run is
+        repeatable; tower_dropout_calls is that number -- carry it over by hand to go on with fresh masks after a resume (it is no
+        entry of the state dict).  It is counted on the host, so such a step cannot be captured into a graph.
+
+        mask_lat_fp8 (this framework's own, off by default): the training graph computes the mask branch's 1x1 convolution
+        sip_mask_lat0 and its gradients with e4m3 operands (ops.linear_fp8); the inference plan does not change."""
         super().__init__()
+        if not 0.0 <= tower_dropout < 1.0:
+            raise ValueError("tower_dropout %r: a probability in [0, 1)" % (tower_dropout,))
+        self.tower_dropout, self.tower_dropout_seed, self.tower_dropout_calls = float(tower_dropout), int(tower_dropout_seed), 0
+        self.mask_lat_fp8 = bool(mask_lat_fp8)
         self.num_classes = num_classes
         self.fp16_enabled = False            # fp16.wrap_fp16_model switches it on (sipmask_head.py: force_fp32 on loss / get_bboxes)
         self.cls_out_channels = num_classes - 1
@@ -160,13 +172,30 @@ class SipMaskHead(nn.Module):
         return self._engines.get(key, module_tensors(self), build)   # rebuilt when any weight has changed since
 
     # ------------------------------------------------------------------ forward, training mode (autograd)
+    def _tower_drop(self):
+        """dropout arguments of the next tower layer, {} when none is wanted"""
+        if not (self.tower_dropout > 0 and self.training):
+            return {}
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("tower_dropout takes its counter from the host: a replay of this graph would repeat its masks")
+        dist = torch.distributed
+        rank = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+        self.tower_dropout_calls += 1
+        return dict(dropout_p=self.tower_dropout, seed=self.tower_dropout_seed, offset=(rank << 48) + self.tower_dropout_calls)
+
     def _tower_train(self, x, convs):
         from . import ops as P
         for m in convs:
-            if m.with_norm:
+            drop = self._tower_drop()
+            if m.with_norm and drop:
+                x = P.group_norm_act(P.conv2d(x, m.conv.weight, None, 1, 1), m.norm.weight, m.norm.bias, m.norm.num_groups, m.norm.eps,
+                                     "relu", **drop)
+            elif m.with_norm:
                 x = P.group_norm(P.conv2d(x, m.conv.weight, None, 1, 1), m.norm.weight, m.norm.bias, 32, 1e-5, True)
             else:
                 x = torch.relu(P.conv2d(x, m.conv.weight, m.conv.bias, 1, 1))
+                if drop:
+                    x = P.dropout(x, drop["dropout_p"], drop["seed"], drop["offset"])
         return x
 
     def rows_path_ok(self):
@@ -177,11 +206,18 @@ class SipMaskHead(nn.Module):
     def _tower_rows(self, x, lv, convs):
         from . import ops_rows as R
         for m in convs:
-            if m.with_norm:
+            drop = self._tower_drop()
+            if m.with_norm and drop:
+                y, _ = R.conv_rows(x, lv, m.conv.weight, None, 1, 1)
+                x = R.gn_act_rows(y, lv, m.norm.weight, m.norm.bias, m.norm.num_groups, m.norm.eps, "relu", **drop)
+            elif m.with_norm:
                 y, _ = R.conv_rows(x, lv, m.conv.weight, None, 1, 1)
                 x = R.gn_rows(y, lv, m.norm.weight, m.norm.bias, m.norm.num_groups, m.norm.eps, True)
             else:
                 x, _ = R.conv_rows(x, lv, m.conv.weight, m.conv.bias, 1, 1, relu=True)
+                if drop:
+                    from . import ops as P
+                    x = P.dropout(x, drop["dropout_p"], drop["seed"], drop["offset"])
         return x
 
     def forward_rows(self, pyr, lv):
@@ -227,7 +263,10 @@ class SipMaskHead(nn.Module):
         h0, w0 = lv.sizes[0]
         l0 = H.Levels(b, [(h0, w0)])
         fm = R.mask_feat_rows(reg_feat, lv)
-        lat0, _ = R.conv_rows(fm, l0, self.sip_mask_lat0.weight, self.sip_mask_lat0.bias, 1, 0, relu=True)
+        if self.mask_lat_fp8:
+            lat0 = P.linear_fp8(fm, self.sip_mask_lat0.weight.flatten(1), self.sip_mask_lat0.bias, relu=True)
+        else:
+            lat0, _ = R.conv_rows(fm, l0, self.sip_mask_lat0.weight, self.sip_mask_lat0.bias, 1, 0, relu=True)
         lat, _ = R.conv_rows(lat0, l0, self.sip_mask_lat.weight, self.sip_mask_lat.bias, 1, 1, relu=True)
         feat_masks = P.upsample_bilinear(R.rows_to_nchw(lat, b, h0, w0), 4)
         return cls_scores, bbox_preds, centernesses, cof_preds, feat_masks
@@ -270,7 +309,11 @@ class SipMaskHead(nn.Module):
             cof_preds.append(P.conv2d(y, self.sip_cof.weight, self.sip_cof.bias, 1, 1))
             if li < 3:
                 fm.append(reg_feat if li == 0 else P.upsample_bilinear(reg_feat, 2 ** li))
-        lat0 = torch.relu(P.conv2d(torch.cat(fm, 1), self.sip_mask_lat0.weight, self.sip_mask_lat0.bias, 1, 0))
+        if self.mask_lat_fp8:
+            lat0 = P.linear_fp8(torch.cat(fm, 1).permute(0, 2, 3, 1), self.sip_mask_lat0.weight.flatten(1), self.sip_mask_lat0.bias,
+                                relu=True).permute(0, 3, 1, 2)
+        else:
+            lat0 = torch.relu(P.conv2d(torch.cat(fm, 1), self.sip_mask_lat0.weight, self.sip_mask_lat0.bias, 1, 0))
         lat = torch.relu(P.conv2d(lat0, self.sip_mask_lat.weight, self.sip_mask_lat.bias, 1, 1))
         return cls_scores, bbox_preds, centernesses, cof_preds, P.upsample_bilinear(lat, 4)
 
