@@ -775,6 +775,7 @@ int mm_plan(const sm_fp8_matmul_desc* d, MmPlan* p) {
     return SM_ERR_BAD_ARG;
   if (d->y_stride < d->n || d->n > 0x7fffff00 || d->k > 0x7fffff00) return SM_ERR_BAD_SHAPE;
   p->few = d->m <= MM_FEW;
+  if (p->few && d->n > 16LL * 0x3ff000) return SM_ERR_UNSUPPORTED;     // (blocks of 1024 threads: fewer than 2^32 in a launch)
   const long long tn = sm_cdiv(d->n, 128);
   const int nkb = sm_cdiv(d->k, 128);
   const long long t128 = (d->m + 127) / 128 * tn;
@@ -857,7 +858,8 @@ extern "C" int sm_fp8_quantize(int dtype, const void* x, int64_t rows, int64_t c
   if (rows < 0 || cols < 1 || x_stride < cols || cols > 0x7fffff00 || rows > (int64_t)1 << 40) return SM_ERR_BAD_SHAPE;
   if (q_t && (rows < 1 || rows > 0x7fffff00)) return SM_ERR_BAD_SHAPE;     // (the transpose sums over the rows)
   if (gate && gate_stride < cols) return SM_ERR_BAD_SHAPE;
-  if (!fp8_out_ok(q, scale) || !fp8_out_ok(q_t, scale_t) || (!q && !q_t && !col_sum)) return SM_ERR_BAD_ARG;
+  if (!fp8_out_ok(q, scale) || !fp8_out_ok(q_t, scale_t) || (rows > 0 && !q && !q_t && !col_sum)) return SM_ERR_BAD_ARG;
+  if (col_sum && cols > 32LL * 0x3ff000) return SM_ERR_UNSUPPORTED;         // (a launch dimension holds fewer than 2^32 threads)
   hipStream_t s = sm_hip_stream(stream);
   if (rows == 0) {
     if (col_sum && sm_zero_async(col_sum, sizeof(float) * cols, s) != hipSuccess) return SM_ERR_LAUNCH;

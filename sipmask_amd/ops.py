@@ -310,10 +310,14 @@ def _channels_last_rows(t):
 
 
 def _empty_channels_last(t):
-    """uninitialised tensor of t's shape, channels-last"""
+    """uninitialised tensor of t's shape, channels-last, and no view of another (an output that is one cannot be changed in place)"""
     if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
         return torch.empty_like(t)
-    return torch.empty(t.shape[:1] + t.shape[2:] + t.shape[1:2], dtype=t.dtype, device=t.device).movedim(-1, 1)
+    strides, step = [0, 1] + [0] * (t.dim() - 2), t.shape[1]
+    for i in (*range(t.dim() - 1, 1, -1), 0):
+        strides[i] = step
+        step *= max(t.shape[i], 1)
+    return torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
 
 
 def _f32(t):
@@ -505,12 +509,12 @@ class Fp8Blocks:
 
     def code_matrix(self):
         """codes [rows, cols]"""
-        c = self.codes.view(torch.uint8).transpose(0, 1).reshape(self.rows, -1)[:, :self.cols]
+        c = self.codes.view(torch.uint8).transpose(0, 1).reshape(self.rows, self.codes.shape[0] * 64)[:, :self.cols]
         return c.contiguous().view(torch.float8_e4m3fn)
 
     def scale_matrix(self):
         """scale bytes [ceil(rows / block_rows), ceil(cols / 128)]"""
-        return self.scales.transpose(0, 1).reshape(self.scales.shape[1], -1)[:, :-(-self.cols // 128)].contiguous()
+        return self.scales.transpose(0, 1).reshape(self.scales.shape[1], self.scales.shape[0] * 4)[:, :-(-self.cols // 128)].contiguous()
 
     def dequantize(self, dtype=torch.float32):
         """the values the codes stand for (for checks and for code without an 8-bit product)"""
@@ -599,9 +603,11 @@ class LinearFp8Function(Function):
                 y = H.fp8_matmul(xq, 1, wq, 128, m, n, k, b32, None, relu, x.dtype, x.device)
             else:
                 y = H.fp8_linear(rows, wq, 128, n, b32, relu, x.dtype)
+        if x.dim() != 2:                         # (no view of y: an output that is one cannot be changed in place)
+            y = torch.ops.aten._unsafe_view(y, x.shape[:-1] + (n,))
         ctx.save_for_backward(None if xt is None else xt.data, None if wt is None else wt.data, y if relu else None)
         ctx.cfg = (None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, k, x.shape[:-1])
-        return y.view(x.shape[:-1] + (n,))
+        return y
 
     @staticmethod
     @once_differentiable
@@ -617,7 +623,7 @@ class LinearFp8Function(Function):
                 dw = torch.zeros(wmeta[0], dtype=wmeta[1], device=dy.device) if need_w else None
                 db = torch.zeros(n, dtype=bdt, device=dy.device) if need_b else None
                 return dy.new_empty(shape + (k,)) if need_x else None, dw, db, None, None
-            g, gt, db = H.fp8_quantize(dy, 1, need_x, need_w, need_b, y)
+            g, gt, db = H.fp8_quantize(dy, 1, need_x, need_w, need_b, None if y is None else y.view(m, n))
             if need_x:
                 dx = H.fp8_matmul(g, 1, H.Fp8Buffer(k, n, 128, data=wt), 128, m, k, n, None, None, False, dy.dtype, dy.device).view(shape + (k,))
             if need_w:
@@ -637,13 +643,15 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
     H.dtype_code(x, "linear_fp8")
     if weight is None and weight_q is None:
         raise ValueError("linear_fp8: weight or weight_q")
+    if weight_q is not None and not isinstance(weight_q, Fp8Blocks):
+        raise TypeError("linear_fp8: weight_q comes from quantize_fp8")
     if weight is not None:
         if weight.dim() not in (2, 4) or (weight.dim() == 4 and tuple(weight.shape[2:]) != (1, 1)) or weight.device != x.device:
             raise ValueError("linear_fp8: weight is [n, k] or [n, k, 1, 1] on %s, got %s" % (x.device, tuple(weight.shape)))
         H.dtype_code(weight, "linear_fp8 weight")
     n, k = weight.shape[:2] if weight is not None else weight_q.shape
-    if weight_q is not None and (not isinstance(weight_q, Fp8Blocks) or weight_q.shape != (n, k) or weight_q.block_rows != 128):
-        raise ValueError("linear_fp8: weight_q is quantize_fp8(weight, block_rows=128) of [%d, %d]" % (n, k))
+    if weight_q is not None and (weight_q.shape != (n, k) or weight_q.block_rows != 128 or weight_q.device != x.device):
+        raise ValueError("linear_fp8: weight_q is quantize_fp8(weight, block_rows=128) of [%d, %d] on %s" % (n, k, x.device))
     if x.dim() < 1 or x.shape[-1] != k or n < 1 or k < 1:
         raise ValueError("linear_fp8: x %s for a weight of [%d, %d]" % (tuple(x.shape), n, k))
     if bias is not None and (bias.shape != (n,) or bias.device != x.device):

@@ -687,3 +687,176 @@ def test_training_step_captured_and_replayed():
         torch.cuda.synchronize()
         want = step(x, w0, ga0, be0)
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_fp8_matrices_without_rows():
+    q = P.quantize_fp8(torch.zeros(0, 40, device=DEV))
+    assert q.shape == (0, 40) and q.dequantize().shape == (0, 40)
+    w = P.quantize_fp8(rnd(8, 40), 128)
+    assert P.matmul_fp8(q, w).shape == (0, 8)
+    assert P.quantize_fp8(torch.zeros(0, 40, device=DEV), 128).scale_matrix().shape == (0, 1)
+
+
+def test_fp8_operands_of_another_place_are_refused():
+    x, w = rnd(4, 16), rnd(8, 16, seed=1)
+    q, wq = P.quantize_fp8(x), P.quantize_fp8(w, 128)
+    host = lambda t: P.Fp8Blocks(t.codes.cpu(), t.scales.cpu(), t.rows, t.cols, t.block_rows)
+    half = P.Fp8Blocks(wq.codes, wq.scales.cpu(), 8, 16, 128)
+    short = P.Fp8Blocks(wq.codes[:, :7], wq.scales, 8, 16, 128)
+    with pytest.raises(NotImplementedError):
+        P.matmul_fp8(q, host(wq))
+    for bad in (host(wq), half, short):
+        with pytest.raises(ValueError):
+            P.linear_fp8(x, None, weight_q=bad)
+    for bad in (half, short):
+        with pytest.raises(ValueError):
+            P.matmul_fp8(q, bad)
+    with pytest.raises(TypeError):
+        P.linear_fp8(x, w, weight_q=w)
+
+
+@pytest.mark.parametrize("m", [3, 40, 700])
+def test_linear_fp8_any_alignment(m):
+    """rows, bias and gradient that start 2 or 4 bytes behind a 16-byte boundary"""
+    k, n = 200, 56
+    x, w, b, dy = rnd(m, k, seed=1, dtype=BF16), rnd(n, k, seed=2), rnd(n, seed=3), rnd(m, n, seed=4, dtype=BF16)
+
+    def odd(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)
+        return flat.copy_(t)
+    got = []
+    for f in (lambda t: t, odd):
+        xl, wl, bl = (f(t).requires_grad_(True) for t in (x, w, b))
+        y = P.linear_fp8(xl, wl, bl, relu=True)
+        with torch.no_grad():
+            serving = P.linear_fp8(xl, None, bl, relu=True, weight_q=P.quantize_fp8(wl, 128))
+        got.append((y.detach(), serving) + torch.autograd.grad(y, [xl, wl, bl], f(dy)))
+    for a, c in zip(*got):
+        assert torch.equal(a, c)
+    assert torch.equal(got[0][0], got[0][1])
+
+
+def test_expanded_gradients_and_a_graph_walked_twice():
+    lv = H.Levels(2, [(5, 7)])
+    x, ga, be = rnd(lv.rows, 64, seed=1, dtype=BF16), 1 + 0.1 * rnd(64, seed=2), 0.1 * rnd(64, seed=3)
+    w, b = rnd(48, 64, seed=4) / 8, rnd(48, seed=5)
+    img = x.view(2, 5, 7, 64).permute(0, 3, 1, 2)
+    calls = ((lambda x, g, h, w, b: PR.gn_act_rows(x, lv, g, h, 8, activation="gelu", dropout_p=0.2, seed=1)),
+             (lambda x, g, h, w, b: P.group_norm_act(x.view(2, 5, 7, 64).permute(0, 3, 1, 2), g, h, 8, activation="silu")),
+             (lambda x, g, h, w, b: P.dropout(x, 0.3, 2, residual=x)), (lambda x, g, h, w, b: P.linear_fp8(x, w, b, relu=True)))
+    for call in calls:
+        leaves = [t.clone().requires_grad_(True) for t in (x, ga, be, w, b)]
+        y = call(*leaves)
+        one = torch.ones((), dtype=y.dtype, device=DEV)
+        first = torch.autograd.grad(y, leaves, one.expand(y.shape), retain_graph=True, allow_unused=True)
+        dense = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True, allow_unused=True)
+        dy = rnd(*y.shape, seed=9, dtype=y.dtype)
+        torch.autograd.grad(y, leaves, dy.transpose(-1, -2).contiguous().transpose(-1, -2), retain_graph=True, allow_unused=True)
+        again = torch.autograd.grad(y, leaves, torch.ones_like(y), allow_unused=True)
+        for a, c, d in zip(first, dense, again):
+            assert (a is None) == (c is None) == (d is None)
+            if a is not None:
+                assert torch.equal(a, c) and torch.equal(a, d)
+    assert img.shape == (2, 64, 5, 7)
+
+
+def test_changed_tensors_are_noticed_by_the_backward():
+    x, w = rnd(20, 64, seed=1, dtype=BF16).requires_grad_(True), (rnd(48, 64, seed=4) / 8).requires_grad_(True)
+    y = P.linear_fp8(x, w, relu=True)
+    y.detach().add_(1)                           # the ReLU's gate is the result itself
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    z = rnd(20, 64, seed=2, dtype=BF16)
+    lv = H.Levels(1, [(4, 5)])
+    h = PR.gn_act_rows(z, lv, (1 + 0 * rnd(64)).requires_grad_(True), rnd(64), 8)
+    z.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        h.sum().backward()
+    off = torch.zeros(1, dtype=torch.int64, device=DEV)
+    d = P.dropout(x, 0.5, 1, off)
+    off.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        d.sum().backward()
+
+
+def test_calls_on_two_streams_at_once():
+    """the same operators in two streams that run side by side: nothing is shared between the calls"""
+    lv = H.Levels(2, [(40, 52), (20, 26)])
+    ga, be, w = 1 + 0.1 * rnd(256, seed=2), 0.1 * rnd(256, seed=3), P.quantize_fp8(rnd(512, 256, seed=4) / 16, 128)
+    xs = [rnd(lv.rows, 256, seed=i, dtype=BF16) for i in range(2)]
+
+    def chain(x, seed):
+        h = PR.gn_act_rows(x, lv, ga, be, 32, activation="silu", dropout_p=0.1, seed=seed)
+        h = P.linear_fp8(h, None, relu=True, weight_q=w)
+        return P.matmul_fp8(P.quantize_fp8(h, transpose=True), P.quantize_fp8(x, transpose=True), out_dtype=F32)
+    want = [chain(x, i) for i, x in enumerate(xs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, (x, s) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(chain(x, i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_two_captured_graphs_replayed_in_turn():
+    """two graphs of one memory pool, one after the other and in the other order, with eager calls between: the workspaces are theirs"""
+    c, lv = 128, H.Levels(1, [(30, 40), (15, 20)])
+    ga, be, w = 1 + 0.1 * rnd(c, seed=2), 0.1 * rnd(c, seed=3), P.quantize_fp8(rnd(96, c, seed=4) / 8, 128)
+    off = torch.zeros(1, dtype=torch.int64, device=DEV)
+
+    def chain(x):
+        h = PR.gn_act_rows(x, lv, ga, be, 16, activation="relu", dropout_p=0.1, seed=3, offset=off)
+        return P.dropout(P.linear_fp8(h, None, weight_q=w), 0.2, 4, off)
+    bufs = [rnd(lv.rows, c, seed=i, dtype=BF16) for i in range(2)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for b in bufs:
+            chain(b)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for b in bufs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            y = chain(b)
+        pool = g.pool()
+        graphs.append(g)
+        outs.append(y)
+    for turn, order in enumerate(((0, 1), (1, 0), (0, 1))):
+        off.fill_(turn)
+        for i in order:
+            bufs[i].copy_(rnd(lv.rows, c, seed=10 * turn + i, dtype=BF16))
+            want = chain(bufs[i])
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want)
+
+
+def test_results_can_be_changed_in_place():
+    """what a residual branch does to a result it owns; the gradient is that of the sum"""
+    lv = H.Levels(2, [(5, 7)])
+    for shape in ((2, 64, 5, 7), (2, 64, 35), (2, 64, 1, 5, 7), (70, 64)):
+        for fmt in (0, 1):
+            x = rnd(*shape, seed=1, dtype=BF16)
+            x = (x.movedim(1, -1).contiguous().movedim(-1, 1) if fmt else x).requires_grad_(True)
+            calls = [lambda x: P.group_norm_act(x, None, None, 8, activation="silu", dropout_p=0.1, seed=1), lambda x: P.dropout(x, 0.3, 2)]
+            if x.dim() == 2:
+                calls.append(lambda x: PR.gn_act_rows(x, lv, None, None, 8))
+            else:
+                w = rnd(48, shape[-1], seed=4) / 4
+                calls += [lambda x: P.linear_fp8(x, w), lambda x: P.linear_fp8(x, w.clone().requires_grad_(True))]
+            for call in calls:
+                y = call(x)
+                dy = rnd(*y.shape, seed=5, dtype=BF16)
+                want, = torch.autograd.grad(y, [x], dy)
+                z = call(x)
+                z += 1
+                got, = torch.autograd.grad(z, [x], dy)
+                assert torch.equal(got, want) and torch.equal(z.detach(), y.detach() + 1)

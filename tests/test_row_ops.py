@@ -183,6 +183,19 @@ def test_fp8_bad_arguments():
     assert lin() == -2
 
 
+def test_fp8_launch_limits():
+    """more blocks than a launch holds: refused, not truncated"""
+    lib = _lib.load()
+    one = C.c_void_p(16)
+    d = _lib.Fp8MatmulDesc()
+    d.m, d.n, d.k, d.a_block_rows, d.b_block_rows, d.y_stride = 1, 1 << 30, 128, 1, 128, 1 << 30
+    assert lib.sm_fp8_matmul_workspace(C.byref(d)) == lib.sm_fp8_linear_workspace(C.byref(d)) != 0
+    assert lib.sm_fp8_linear_workspace(C.byref(d)) < 0
+    assert lib.sm_fp8_matmul(C.byref(d), one, one, one, one, None, None, one, one, 1 << 40, None) < 0
+    cols = 1 << 30
+    assert lib.sm_fp8_quantize(0, one, 1, cols, cols, 1, None, 0, one, one, None, None, one, one, 1 << 40, None) < 0
+
+
 # ------------------------------------------------------------------------------------------------ Python entry points
 def test_cpu_tensors_are_refused():
     x, w = torch.randn(4, 8), torch.randn(8)
