@@ -860,3 +860,16 @@ def test_results_can_be_changed_in_place():
                 z += 1
                 got, = torch.autograd.grad(z, [x], dy)
                 assert torch.equal(got, want) and torch.equal(z.detach(), y.detach() + 1)
+
+
+@pytest.mark.parametrize("nkb", [1, 2, 3, 5, 7, 31, 63, 64, 65, 130])
+def test_quantize_fp8_rows_of_any_number_of_blocks(nkb):
+    """a workgroup's 64 blocks end inside a row, span many rows, or lie in one"""
+    for rows in (1, 13, 70):
+        for cols in (nkb * 128, nkb * 128 - 53):
+            x = rnd(rows, cols, seed=nkb + rows, dtype=BF16)
+            q = P.quantize_fp8(x)
+            codes, byte, _ = R.fp8_quantize(x, 1)
+            assert torch.equal(q.code_matrix().view(torch.uint8), codes.to(torch.uint8)) and torch.equal(q.scale_matrix().long(), byte)
+            assert bool((q.codes.view(torch.uint8).transpose(0, 1).reshape(rows, -1)[:, cols:] == 0).all())
+            assert bool((q.scales.transpose(0, 1).reshape(rows, -1)[:, nkb:] == 127).all())
