@@ -748,22 +748,32 @@ __global__ __launch_bounds__(1024) void fp8_mm_few_kernel(const MmArgs a, const 
   }
 }
 
-// split-K: add the partials in order, then the epilogue
+// split-K: add the partials in order (four loads in flight), then the epilogue.  A product that is split has at most 256 tiles, so its
+// elements count in 32 bits
 __global__ __launch_bounds__(256) void fp8_mm_finish_kernel(const MmArgs a) {
-  const int n4 = (a.n + 3) >> 2;
-  const long long total = a.m * n4;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long m = i / n4;
+  const uint32_t n4 = (uint32_t)(a.n + 3) >> 2, total = (uint32_t)a.m * n4;
+  const long long slab = a.m * a.n;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const uint32_t m = i / n4;
     const int n = (int)(i - m * n4) * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < a.ksplit; ++k) {
-      const float* p = a.part + ((long long)k * a.m + m) * a.n + n;
-      if ((a.n & 3) == 0) {
+    const float* p = a.part + (long long)m * a.n + n;
+    if ((a.n & 3) == 0) {
+      int k = 0;
+      for (; k + 4 <= a.ksplit; k += 4, p += 4 * slab) {
+        float4 t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const float4*>(p + u * slab);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[0] += t[u].x, v[1] += t[u].y, v[2] += t[u].z, v[3] += t[u].w;
+      }
+      for (; k < a.ksplit; ++k, p += slab) {
         const float4 t = *reinterpret_cast<const float4*>(p);
         v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
-      } else {
-        for (int e = 0; e < 4 && n + e < a.n; ++e) v[e] += p[e];
       }
+    } else {
+      for (int k = 0; k < a.ksplit; ++k, p += slab)
+        for (int e = 0; e < 4 && n + e < a.n; ++e) v[e] += p[e];
     }
     mm_finish(a, m, n, v);
   }
