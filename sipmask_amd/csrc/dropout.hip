@@ -1,8 +1,9 @@
 // Dropout whose mask is a function of (seed, offset, element) -- philox.h -- optionally added to a residual:
 //   y = keep * x / (1 - p) [+ residual],   dx = keep * dy / (1 - p) (the same kernel without the residual)
 // Bound by memory (read x [and the residual], write y); nothing else is read or written.  A thread takes the 8 consecutive elements of
-// one generator block where rows and alignment allow it.  268 800 x 256 bf16: 49 us = 5.6 TB/s (a copy of the same tensor: 47 us); the generator's share of the vector
-// units is about half of that time.  Dropped elements are selected away, not multiplied by 0: Inf and NaN in x do not survive where keep = 0.
+// one generator block where rows and alignment allow it.  268 800 x 256 bf16: 49 us = 5.6 TB/s (a copy of the same tensor: 47 us); the
+// generator's share of the vector units is about half of that time.  Dropped elements are selected away, not multiplied by 0: Inf and
+// NaN in x do not survive where keep = 0.
 #include <algorithm>
 #include <type_traits>
 

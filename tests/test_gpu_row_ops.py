@@ -873,3 +873,30 @@ def test_quantize_fp8_rows_of_any_number_of_blocks(nkb):
             assert torch.equal(q.code_matrix().view(torch.uint8), codes.to(torch.uint8)) and torch.equal(q.scale_matrix().long(), byte)
             assert bool((q.codes.view(torch.uint8).transpose(0, 1).reshape(rows, -1)[:, cols:] == 0).all())
             assert bool((q.scales.transpose(0, 1).reshape(rows, -1)[:, nkb:] == 127).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("cols", [1, 3, 8, 63, 64, 65, 100, 255, 513])
+def test_dropout_rows_of_any_width_and_stride(cols, dtype):
+    """strided x, residual and result through the C entry: the mask is that of the dense tensor, other columns stay as they were"""
+    for rows in (1, 2, 41, 300):
+        x, r = rnd(rows, cols, seed=1, dtype=dtype), rnd(rows, cols, seed=2, dtype=dtype)
+        fac = R.keep_factor((rows, cols), 0.3, 7, 9).to(DEV)
+        want = x.double() * fac
+        bound = R.half_step(dtype) * want.abs() + 2 * R.E * want.abs() + R.tiny(dtype)
+        both = want + r.double()
+        bothb = R.half_step(dtype) * both.abs() + 2 * R.E * (want.abs() + both.abs()) + R.tiny(dtype)
+        for ox, orr, oy, wide in ((0, 0, 0, cols), (1, 2, 3, cols + 5), (8, 0, 16, (cols + 23) // 8 * 8)):
+            def place(t, o):
+                buf = torch.full((rows, wide + o), 5.0, dtype=dtype, device=DEV)
+                buf[:, o:o + cols] = t
+                return buf
+            bx, br, by = place(x, ox), place(r, orr), place(torch.zeros_like(x), oy)
+            e = x.element_size()
+            for res in (None, br):
+                by[:, oy:oy + cols] = 0
+                assert _lib.load().sm_dropout(H.DTYPE_CODES[dtype], bx.data_ptr() + ox * e, None if res is None else br.data_ptr() + orr * e,
+                                              by.data_ptr() + oy * e, rows, cols, bx.stride(0), br.stride(0), by.stride(0),
+                                              H.dropout_threshold(0.3), 7, 9, None, H._stream(x)) == 0
+                within(by[:, oy:oy + cols], want if res is None else both, bound if res is None else bothb, "y")
+                assert bool((by[:, :oy] == 5).all()) and bool((by[:, oy + cols:] == 5).all())
