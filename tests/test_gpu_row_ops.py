@@ -900,3 +900,61 @@ def test_dropout_rows_of_any_width_and_stride(cols, dtype):
                                               H.dropout_threshold(0.3), 7, 9, None, H._stream(x)) == 0
                 within(by[:, oy:oy + cols], want if res is None else both, bound if res is None else bothb, "y")
                 assert bool((by[:, :oy] == 5).all()) and bool((by[:, oy + cols:] == 5).all())
+
+
+@pytest.mark.parametrize("c,groups,hw", [(256, 32, 900), (256, 32, 60), (60, 12, 300), (48, 4, 700)])
+def test_group_norm_act_backward_over_its_own_gradient(c, groups, hw):
+    """dx may be dy"""
+    x, dy = rnd(2 * hw, c, seed=1, dtype=BF16), rnd(2 * hw, c, seed=2, dtype=BF16)
+    ga, be = 1 + 0.1 * rnd(c, seed=3), 0.1 * rnd(c, seed=4)
+    y = torch.empty_like(x)
+    d, need, stats = H.group_norm_act(x, c, y, 2, (hw,), c, groups, 1e-5, H.ACTIVATIONS["silu"], H.dropout_threshold(0.2), 3, (4, None), ga, be,
+                                      True)
+    outs = []
+    for dx in (torch.empty_like(x), dy):
+        dg, db = torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+        H.group_norm_act_bwd(d, need, x, dy, c, dx, ga, be, stats, dg, db)
+        outs.append((dx, dg, db))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 70, 300), (500, 333, 1200), (300, 256, 9000), (3000, 512, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_matmul_fp8_onto_its_residual(m, n, k, dtype):
+    """residual may be y (with K split and without)"""
+    a, b, r = P.quantize_fp8(rnd(m, k, seed=1)), P.quantize_fp8(rnd(n, k, seed=2), 128), rnd(m, n, seed=3, dtype=dtype)
+    want = P.matmul_fp8(a, b, relu=True, residual=r, out_dtype=dtype)
+    plan, need, _ = H._fp8_plan(m, n, k, 1, 128, H.DTYPE_CODES[dtype], 1)
+    d = _lib.Fp8MatmulDesc.from_buffer_copy(plan)
+    d.res_stride = n
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    assert _lib.load().sm_fp8_matmul(C.byref(d), a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(), None,
+                                     r.data_ptr(), r.data_ptr(), ws.data_ptr(), need, H._stream(r)) == 0
+    assert torch.equal(r, want)
+
+
+@pytest.mark.parametrize("cols,stride", [(64, 64), (64, 80), (37, 41)])
+def test_rows_written_over_their_input(cols, stride):
+    """y may be x (dropout, GroupNorm) or the residual (dropout)"""
+    for rows in (3, 500):
+        def rows_like(seed):
+            t = torch.zeros(rows, stride, dtype=F16, device=DEV)[:, :cols]
+            return t.copy_(rnd(rows, cols, seed=seed, dtype=F16))
+        x, r = rows_like(1), rows_like(2)
+        thr, s = H.dropout_threshold(0.4), H._stream(x)
+        want = P.dropout(x, 0.4, 5, 6, residual=r)
+        for y in (x.clone() if stride == cols else None, r):
+            if y is None:
+                continue
+            src, res = (y, r) if y is not r else (x, r)
+            assert _lib.load().sm_dropout(1, src.data_ptr(), res.data_ptr(), y.data_ptr(), rows, cols, src.stride(0), res.stride(0), y.stride(0),
+                                          thr, 5, 6, None, s) == 0
+            assert torch.equal(y, want)
+            r = rows_like(2)
+        want = P.group_norm_act(x, None, None, 1, activation="gelu")
+        plan, need, _ = H._gn_act_plan(rows, (1,), cols, 1, 1, 3, 1e-5, 0)
+        d = _lib.GnActDesc.from_buffer_copy(plan)
+        d.x_stride = d.y_stride = x.stride(0)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+        assert _lib.load().sm_group_norm_act(C.byref(d), x.data_ptr(), None, None, x.data_ptr(), None, ws.data_ptr(), need, s) == 0
+        assert torch.equal(x, want)

@@ -170,3 +170,44 @@ def test_mask_branch_with_e4m3_operands(monkeypatch, rows):
     out[4].float().square().mean().backward()
     for p in (h.sip_mask_lat0.weight, h.sip_mask_lat0.bias, h.sip_mask_lat.weight, h.reg_convs[0].conv.weight):
         assert p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0
+
+
+@pytest.mark.gpu
+def test_gradients_in_allreduce_buckets_match_plain_training():
+    """both options on: gradients that live in all-reduce buckets (a census step through autograd's add, then written directly) equal those
+    of a plain step with the same masks.  5e-3 relative, not bits: the deformable convolution's and the split-K convolutions' gradients are
+    added with float atomics; a lost or doubled contribution would be of the gradient's own size."""
+    from test_gpu_api import _synthetic_gt
+    from sipmask_amd.dist_train import GradBucketer, HipSGD, head_train_step
+    torch.manual_seed(9)
+    h = build_head(dict(type="SipMaskHead", num_classes=81, in_channels=256, stacked_convs=3, center_sampling=True,
+                        strides=[8, 16, 32, 64, 128], tower_dropout=0.1, tower_dropout_seed=5, mask_lat_fp8=True)).cuda()
+    g = torch.Generator().manual_seed(5)
+    feats = [torch.randn(2, 256, a, b, generator=g).cuda() for a, b in [(16, 20), (8, 10), (4, 5), (2, 3), (1, 2)]]
+    gtb, gtl, gtm = _synthetic_gt(g, 2, 128, 160, 4)
+    gtb, gtl = [b.cuda() for b in gtb], [l.cuda() for l in gtl]
+    metas = [dict(img_shape=(128, 160, 3), pad_shape=(128, 160, 3), scale_factor=1.0) for _ in range(2)]
+    opt = HipSGD(h.named_parameters(), lr=0.0, momentum=0.0, weight_decay=0.0)
+
+    def step(**kw):
+        h.tower_dropout_calls = 100
+        return head_train_step(h, feats, gtb, gtl, gtm, metas, opt, **kw)
+    plain_loss = step()
+    plain = {n: (None if p.grad is None else p.grad.detach().clone()) for n, p in h.named_parameters()}
+    opt.zero_grad()
+    bucket = GradBucketer([p for p in h.parameters() if p.requires_grad], bucket_bytes=4 << 20)
+    try:
+        for turn in range(3):
+            loss = step(bucketer=bucket)
+            if turn:
+                norm = h.cls_convs[0].norm
+                assert not H.GRAD_SINK.census and {norm.weight.data_ptr(), norm.bias.data_ptr()} <= H.GRAD_SINK.written
+            for k in plain_loss:
+                assert abs(loss[k] - plain_loss[k]) <= 1e-4 * max(1.0, abs(plain_loss[k])), (turn, k)
+            for n, p in h.named_parameters():
+                if plain[n] is None:
+                    assert float(p.grad.abs().max()) == 0.0, n
+                else:
+                    assert float((p.grad - plain[n]).norm() / (plain[n].norm() + 1e-20)) <= 5e-3, (turn, n)
+    finally:
+        bucket.remove()
