@@ -721,7 +721,7 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, bool backward, GaPlan* p) {
   const int vec = p->vec ? 8 : 1;
   p->whole = a.cpg % vec == 0;
   a.cols = a.C / vec;
-  a.ct = std::min(a.cols, p->vec ? GA_TILE : GA_TILE1);
+  a.ct = sm_cdiv(a.cols, sm_cdiv(a.cols, p->vec ? GA_TILE : GA_TILE1));      // (tiles of one width: 320 channels are 2 x 20 vectors)
   a.ntile = sm_cdiv(a.cols, a.ct);
   if (a.ntile > 65535 || a.G > 65535 * 32) return SM_ERR_UNSUPPORTED;
   const int tc = a.ct * vec;
@@ -741,8 +741,17 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, bool backward, GaPlan* p) {
   const long long tiles_per_group = (a.cpg - 1) / tc + 2;
   const long long smax = std::max<long long>(4, std::min<long long>(256, GA_COMBINE / (tiles_per_group * p->gpt)));
   const long long few = (hw_max + smax - 1) / smax, many = (hw_max + 2 * smax - 1) / (2 * smax);
-  const long long srpb = std::max(std::max<long long>(2 * ((backward ? GA_SUM : GA_STAT) / a.ct), total / 512),
-                                  few > 0 && total / few < 256 ? many : few);
+  long long srpb = std::max(std::max<long long>(2 * ((backward ? GA_SUM : GA_STAT) / a.ct), (total + 511) / 512),
+                            few > 0 && total / few < 256 ? many : few);
+  // Two blocks fit a CU, so a few more than 512 take twice the time of 512 (18 496 rows x 1024 channels backward, 516 blocks: 78 us, 512:
+  // 65): up to a quarter more rows per block where that does it
+  auto blocks = [&](long long rpb) {
+    long long n = 0;
+    for (int l = 0; l < d->nlev; ++l) n += (d->hw[l] + rpb - 1) / rpb;
+    return n * a.batch * a.ntile;
+  };
+  for (long long t = srpb; blocks(srpb) > 512 && t <= srpb + srpb / 4; t += std::max<long long>(1, srpb / 32))
+    if (blocks(t) <= 512) srpb = t;
   if (srpb > 0x3fffffff || arpb > 0x3fffffff) return SM_ERR_UNSUPPORTED;
   a.srpb = (int)srpb, a.arpb = (int)arpb;
   long long sb = 0, ab = 0;
