@@ -22,7 +22,7 @@
 //   8192 x 4096 x 4096 product alone       215 to 260 us by run, 8192^3 855 = 1.29 PFLOP/s: as the library's, half of the bf16 peak
 //   67 200 x 512 x 768 product alone       58 us = 0.91 PFLOP/s: twelve short steps between a block's first load and its last store
 //   7 x 512 x 2048 with its quantiser      5 us: one launch, latency
-//   quantiser, 16 800 x 1024               15 us = 3.5 TB/s; with the transpose, 67 200 x 768: 44 us = 4.7 TB/s
+//   quantiser, 67 200 x 768               29 us = 5.3 TB/s; with the transpose, 67 200 x 768: 44 us = 4.7 TB/s
 #include <algorithm>
 #include <type_traits>
 

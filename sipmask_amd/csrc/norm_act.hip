@@ -15,11 +15,11 @@
 // once and needs no partials -- there the launches, not the bytes, are the time.
 //
 // Measured (a copy of 2 GiB runs at 4.9 TB/s here):
-//   89 600 x 256 bf16 rows of five levels, ReLU, p = 0.1: forward 41 us (sums 15, apply 27), backward 67 (sums 34, apply 34); without
-//     dropout 38 and 58.  The rows are 46 MB, so a pass over them is 9 us; what is over that is latency at 1.4 blocks per CU (more row
-//     blocks cost more in partials than they hide) and the generator (10 us of the two backward launches).
-//   295 936 x 256 bf16, SiLU (151 MB, behind the memory-side cache): forward 85 us = 5.3 TB/s over its three passes, backward 165 =
-//     4.6 TB/s over five: bandwidth.
+//   89 600 x 256 bf16 rows of five levels, ReLU, p = 0.1: forward 40 us (sums 15, apply 26), backward 65 (sums 34, apply 32); without
+//     dropout 38 and 56.  The rows are 46 MB, so a pass over them is 9 us; what is over that is latency at 1.4 blocks per CU (more row
+//     blocks cost more in partials than they hide) and the generator (9 us of the two backward launches).
+//   295 936 x 256 bf16, SiLU (151 MB, behind the memory-side cache): forward 85 us = 5.3 TB/s over its three passes, backward 158 =
+//     4.8 TB/s over five: bandwidth.
 //   77 x 256 f16, SiLU: one launch, 8 us, of which the loads are less than 2: the two reductions.
 //
 // The sums are held in f64: x and x^2 add exactly enough that E[x^2] - m^2 keeps its digits for |m| >> sqrt(v) (1e4 standard deviations
