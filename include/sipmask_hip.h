@@ -841,6 +841,28 @@ int64_t sm_fp8_linear_workspace(const sm_fp8_matmul_desc* d);
 int sm_fp8_linear(const sm_fp8_matmul_desc* d, int x_dtype, const void* x, int64_t x_stride, const void* b, const void* b_scale,
                   const float* bias, const void* residual, void* y, void* workspace, int64_t workspace_bytes, sm_stream_t stream);
 
+/* A layer's training step in one call each way, y = relu?(q(x) q(w)^T + bias): the forward leaves the codes of the transposes of x (when
+ * dw is wanted) and of w (when dx is) in `saved`, the backward makes dx = q(dy) q(w), dw = q(dy^T) q(x^T)^T and dbias (the column sums
+ * of dy) from them; with relu, dy counts where y > 0.  y and dx are dense rows of dtype, dw f32 [n][k], dbias f32 [n]. */
+typedef struct {
+  int64_t m;
+  int32_t n, k;
+  int32_t dtype, w_dtype; /* sm_dtype of x, y, dy, dx and of w */
+  int32_t relu;
+  int32_t need_dx, need_dw, need_db; /* what the backward will be asked for */
+  int32_t have_wq;                   /* the forward takes w's codes (128 x 128 blocks) instead of making them */
+  int32_t reserved;
+  int64_t x_stride, dy_stride; /* elements */
+} sm_fp8_layer_desc;
+/* bytes of saved and of the two workspaces, each 16-byte aligned (0: NULL will do) */
+int sm_fp8_layer_bytes(const sm_fp8_layer_desc* d, int64_t* saved, int64_t* forward, int64_t* backward);
+/* w [n][k] (row stride w_stride) may be NULL with have_wq and without need_dx, w_codes / w_scales without have_wq */
+int sm_fp8_layer_fwd(const sm_fp8_layer_desc* d, const void* x, const void* w, int64_t w_stride, const void* w_codes, const void* w_scales,
+                     const float* bias, void* y, void* saved, void* workspace, int64_t workspace_bytes, sm_stream_t stream);
+/* y: the forward's result (may be NULL without relu) */
+int sm_fp8_layer_bwd(const sm_fp8_layer_desc* d, const void* dy, const void* y, const void* saved, void* dx, float* dw, float* dbias,
+                     void* workspace, int64_t workspace_bytes, sm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

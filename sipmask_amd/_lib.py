@@ -103,6 +103,15 @@ class Fp8MatmulDesc(C.Structure):
     ]
 
 
+class Fp8LayerDesc(C.Structure):
+    """sm_fp8_layer_desc"""
+    _fields_ = [
+        ("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("relu", C.c_int32),
+        ("need_dx", C.c_int32), ("need_dw", C.c_int32), ("need_db", C.c_int32), ("have_wq", C.c_int32), ("reserved", C.c_int32),
+        ("x_stride", C.c_int64), ("dy_stride", C.c_int64),
+    ]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _F = C.c_float
@@ -221,6 +230,9 @@ PROTOTYPES = {
     "sm_fp8_matmul": (_I, [C.POINTER(Fp8MatmulDesc), _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "sm_fp8_linear_workspace": (C.c_int64, [C.POINTER(Fp8MatmulDesc)]),
     "sm_fp8_linear": (_I, [_P, _I, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_fp8_layer_bytes": (_I, [C.POINTER(Fp8LayerDesc), C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    "sm_fp8_layer_fwd": (_I, [C.POINTER(Fp8LayerDesc), _P, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "sm_fp8_layer_bwd": (_I, [C.POINTER(Fp8LayerDesc), _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
 }
 
 _lib = None

@@ -1027,3 +1027,110 @@ extern "C" int sm_fp8_linear(const sm_fp8_matmul_desc* d, int x_dtype, const voi
   if (st != SM_OK) return st;
   return mm_run(d, p, nullptr, nullptr, b, b_scale, bias, residual, y, workspace, x_dtype, x, x_stride, sm_hip_stream(stream));
 }
+
+// ------------------------------------------------------------------------------------------------ a layer's step
+namespace {
+// sections of a buffer, 256 bytes apart
+struct Carve {
+  uint8_t* base;
+  int64_t at = 0;
+  void* take(int64_t bytes) {
+    void* p = base == nullptr ? nullptr : base + at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+struct LinMat {                                  // a quantised matrix in such a buffer
+  void *codes, *scales;
+  LinMat() : codes(nullptr), scales(nullptr) {}
+  LinMat(Carve& c, int64_t rows, int64_t cols, int br) : codes(c.take(sm_fp8_codes_bytes(rows, cols))), scales(c.take(sm_fp8_scales_bytes(rows, cols, br))) {}
+};
+
+struct LinPlan {
+  sm_fp8_matmul_desc y, dx, dw;                  // the three products
+  int64_t saved, fwd, bwd;                       // bytes
+  LinMat xt, wt;                                 // kept for the backward: the transposes of x and w
+  LinMat wq, xq, g, gt;                          // in the workspaces
+  void *yws, *colws, *pws;
+  int64_t yws_bytes, colws_bytes, pws_bytes;
+};
+
+int lin_plan(const sm_fp8_layer_desc* d, void* saved, void* fwd, void* bwd, LinPlan* p) {
+  if (d == nullptr) return SM_ERR_BAD_ARG;
+  if (d->m < 1 || d->n < 1 || d->k < 1 || d->m > 0x7fffff00 || d->x_stride < d->k || d->dy_stride < d->n) return SM_ERR_BAD_SHAPE;
+  if (d->dtype < SM_DT_BF16 || d->dtype > SM_DT_F32 || d->w_dtype < SM_DT_BF16 || d->w_dtype > SM_DT_F32) return SM_ERR_BAD_ARG;
+  const int64_t m = d->m, n = d->n, k = d->k;
+  p->y = {m, d->n, d->k, 1, 128, d->dtype, d->relu, n, 0};
+  p->dx = {m, d->k, d->n, 1, 128, d->dtype, 0, k, 0};
+  p->dw = {n, d->k, (int32_t)m, 1, 1, SM_DT_F32, 0, k, 0};
+  Carve s{(uint8_t*)saved}, f{(uint8_t*)fwd}, b{(uint8_t*)bwd};
+  if (d->need_dw) p->xt = LinMat(s, k, m, 1);
+  if (d->need_dx) p->wt = LinMat(s, k, n, 128);
+  if (!d->have_wq) p->wq = LinMat(f, n, k, 128);
+  if (d->need_dw) p->xq = LinMat(f, m, k, 1);
+  p->yws_bytes = d->need_dw ? sm_fp8_matmul_workspace(&p->y) : sm_fp8_linear_workspace(&p->y);
+  if (p->yws_bytes < 0) return (int)p->yws_bytes;
+  p->yws = f.take(p->yws_bytes);
+  if (d->need_dx) p->g = LinMat(b, m, n, 1);
+  if (d->need_dw) p->gt = LinMat(b, n, m, 1);
+  p->colws_bytes = d->need_db ? sm_fp8_quantize_workspace(m, n, 1) : 0;
+  p->colws = b.take(p->colws_bytes);
+  const int64_t w1 = d->need_dx ? sm_fp8_matmul_workspace(&p->dx) : 0, w2 = d->need_dw ? sm_fp8_matmul_workspace(&p->dw) : 0;
+  if (w1 < 0 || w2 < 0) return (int)std::min(w1, w2);
+  p->pws_bytes = std::max(w1, w2);
+  p->pws = b.take(p->pws_bytes);
+  p->saved = s.at, p->fwd = f.at, p->bwd = b.at;
+  return SM_OK;
+}
+bool lin_buf_ok(const void* p, int64_t need) { return need == 0 || (p != nullptr && ((uintptr_t)p & 15) == 0); }
+}  // namespace
+
+extern "C" int sm_fp8_layer_bytes(const sm_fp8_layer_desc* d, int64_t* saved, int64_t* forward, int64_t* backward) {
+  if (!saved || !forward || !backward) return SM_ERR_BAD_ARG;
+  LinPlan p;
+  const int st = lin_plan(d, nullptr, nullptr, nullptr, &p);
+  if (st == SM_OK) *saved = p.saved, *forward = p.fwd, *backward = p.bwd;
+  return st;
+}
+
+extern "C" int sm_fp8_layer_fwd(const sm_fp8_layer_desc* d, const void* x, const void* w, int64_t w_stride, const void* w_codes,
+                                const void* w_scales, const float* bias, void* y, void* saved, void* workspace, int64_t workspace_bytes,
+                                sm_stream_t stream) {
+  LinPlan p;
+  int st = lin_plan(d, saved, workspace, nullptr, &p);
+  if (st != SM_OK) return st;
+  if (!x || !y || !lin_buf_ok(saved, p.saved) || !lin_buf_ok(workspace, p.fwd) || (d->have_wq && (!w_codes || !w_scales))) return SM_ERR_BAD_ARG;
+  if (workspace_bytes < p.fwd) return SM_ERR_WORKSPACE;
+  if (!d->have_wq || d->need_dx) {
+    if (!w || w_stride < d->k) return SM_ERR_BAD_ARG;
+    st = sm_fp8_quantize(d->w_dtype, w, d->n, d->k, w_stride, 128, nullptr, 0, p.wq.codes, p.wq.scales, p.wt.codes, p.wt.scales, nullptr, nullptr,
+                         0, stream);
+    if (st != SM_OK) return st;
+  }
+  const void *wc = d->have_wq ? w_codes : p.wq.codes, *ws = d->have_wq ? w_scales : p.wq.scales;
+  if (!d->need_dw)
+    return sm_fp8_linear(&p.y, d->dtype, x, d->x_stride, wc, ws, bias, nullptr, y, p.yws, p.yws_bytes, stream);
+  st = sm_fp8_quantize(d->dtype, x, d->m, d->k, d->x_stride, 1, nullptr, 0, p.xq.codes, p.xq.scales, p.xt.codes, p.xt.scales, nullptr, nullptr, 0,
+                       stream);
+  if (st != SM_OK) return st;
+  return sm_fp8_matmul(&p.y, p.xq.codes, p.xq.scales, wc, ws, bias, nullptr, y, p.yws, p.yws_bytes, stream);
+}
+
+extern "C" int sm_fp8_layer_bwd(const sm_fp8_layer_desc* d, const void* dy, const void* y, const void* saved, void* dx, float* dw, float* dbias,
+                                void* workspace, int64_t workspace_bytes, sm_stream_t stream) {
+  LinPlan p;
+  int st = lin_plan(d, const_cast<void*>(saved), nullptr, workspace, &p);
+  if (st != SM_OK) return st;
+  if (!dy || !lin_buf_ok(saved, p.saved) || !lin_buf_ok(workspace, p.bwd) || (d->need_dx && !dx) || (d->need_dw && !dw) || (d->need_db && !dbias) ||
+      (d->relu && !y))
+    return SM_ERR_BAD_ARG;
+  if (workspace_bytes < p.bwd) return SM_ERR_WORKSPACE;
+  if (!d->need_dx && !d->need_dw && !d->need_db) return SM_OK;
+  st = sm_fp8_quantize(d->dtype, dy, d->m, d->n, d->dy_stride, 1, d->relu ? y : nullptr, d->n, p.g.codes, p.g.scales, p.gt.codes, p.gt.scales,
+                       d->need_db ? dbias : nullptr, p.colws, p.colws_bytes, stream);
+  if (st == SM_OK && d->need_dx)
+    st = sm_fp8_matmul(&p.dx, p.g.codes, p.g.scales, p.wt.codes, p.wt.scales, nullptr, nullptr, dx, p.pws, p.pws_bytes, stream);
+  if (st == SM_OK && d->need_dw)
+    st = sm_fp8_matmul(&p.dw, p.gt.codes, p.gt.scales, p.xt.codes, p.xt.scales, nullptr, nullptr, dw, p.pws, p.pws_bytes, stream);
+  return st;
+}

@@ -1547,23 +1547,14 @@ class Fp8Buffer:
         self.scales = self.codes + nc
 
 
-def fp8_quantize(x, block_rows, rows=True, transpose=False, col_sum=False, gate=None):
-    """x (and gate) [r, c] with dense rows, read once -> (Fp8Buffer or None, the transpose's or None, f32 column sums or None); gate:
-    values whose gate is not > 0 count as 0"""
-    lib = _lib.load()
+def fp8_quantize(x, block_rows, transpose=False):
+    """x [r, c] with dense rows -> Fp8Buffer of x or of its transpose"""
     r, c = x.shape
-    q = Fp8Buffer(r, c, block_rows, x.device) if rows else None
+    q = None if transpose else Fp8Buffer(r, c, block_rows, x.device)
     t = Fp8Buffer(c, r, block_rows, x.device) if transpose else None
-    cs = ws = None
-    need = 0
-    if col_sum:
-        cs = torch.empty(c, dtype=torch.float32, device=x.device)
-        need = lib.sm_fp8_quantize_workspace(r, c, 1)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _lib.check(lib.sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _p(x), r, c, row_stride(x), block_rows, _p(gate),
-                                   0 if gate is None else row_stride(gate), q and q.codes, q and q.scales, t and t.codes, t and t.scales,
-                                   _p(cs), _p(ws), need, _stream(x)), "sm_fp8_quantize")
-    return q, t, cs
+    _lib.check(_lib.load().sm_fp8_quantize(dtype_code(x, "quantize_fp8"), _p(x), r, c, row_stride(x), block_rows, None, 0, q and q.codes,
+                                           q and q.scales, t and t.codes, t and t.scales, None, None, 0, _stream(x)), "sm_fp8_quantize")
+    return t if transpose else q
 
 
 @functools.lru_cache(maxsize=512)
@@ -1601,3 +1592,39 @@ def fp8_linear(x, b, b_block_rows, n, bias, relu, out_dtype):
     _lib.check(_lib.load().sm_fp8_linear(plan, dtype_code(x, "linear_fp8"), _p(x), row_stride(x), b.codes, b.scales, _p(bias), None, _p(y),
                                          _p(ws), need, _stream(x)), "sm_fp8_linear")
     return y
+
+
+@functools.lru_cache(maxsize=512)
+def _fp8_layer_plan(m, n, k, dtype, w_dtype, relu, need_dx, need_dw, need_db, have_wq):
+    """(sm_fp8_layer_desc as bytes, bytes saved for the backward, of the forward's and the backward's workspace)"""
+    d = _lib.Fp8LayerDesc()
+    d.m, d.n, d.k, d.dtype, d.w_dtype, d.relu = m, n, k, dtype, w_dtype, relu
+    d.need_dx, d.need_dw, d.need_db, d.have_wq = need_dx, need_dw, need_db, have_wq
+    d.x_stride, d.dy_stride = k, n
+    b = [C.c_int64() for _ in range(3)]
+    _lib.check(_lib.load().sm_fp8_layer_bytes(C.byref(d), *map(C.byref, b)), "sm_fp8_layer")
+    return (bytes(d),) + tuple(v.value for v in b)
+
+
+def fp8_layer_fwd(x, w, wq, n, bias, relu, need_dx, need_dw, need_db):
+    """x [m, k], w [n, k] (or None) with dense rows, wq: codes of w or None -> (y [m, n], what the backward needs, its plan)"""
+    m, k = x.shape
+    plan = _fp8_layer_plan(m, n, k, DTYPE_CODES[x.dtype], 0 if w is None else DTYPE_CODES[w.dtype], int(relu), int(need_dx), int(need_dw),
+                           int(need_db), int(wq is not None))
+    d = _lib.Fp8LayerDesc.from_buffer_copy(plan[0])
+    d.x_stride = row_stride(x)
+    y = torch.empty(m, n, dtype=x.dtype, device=x.device)
+    saved = torch.empty(plan[1], dtype=torch.uint8, device=x.device) if plan[1] else None
+    ws = torch.empty(plan[2], dtype=torch.uint8, device=x.device) if plan[2] else None
+    _lib.check(_lib.load().sm_fp8_layer_fwd(C.byref(d), _p(x), _p(w), 0 if w is None else row_stride(w), wq and wq.codes, wq and wq.scales,
+                                            _p(bias), _p(y), _p(saved), _p(ws), plan[2], _stream(x)), "sm_fp8_layer_fwd")
+    return y, saved, plan
+
+
+def fp8_layer_bwd(plan, dy, y, saved, dx, dw, db):
+    """writes those of dx (dense rows), dw f32 and db f32 that the forward announced"""
+    d = _lib.Fp8LayerDesc.from_buffer_copy(plan[0])
+    d.dy_stride = row_stride(dy)
+    ws = torch.empty(plan[3], dtype=torch.uint8, device=dy.device) if plan[3] else None
+    _lib.check(_lib.load().sm_fp8_layer_bwd(C.byref(d), _p(dy), _p(y), _p(saved), _p(dx), _p(dw), _p(db), _p(ws), plan[3], _stream(dy)),
+               "sm_fp8_layer_bwd")

@@ -537,8 +537,8 @@ def quantize_fp8(x, block_rows=1, transpose=False):
         raise ValueError("quantize_fp8: the transpose of 0 rows has no columns")
     x = H.dense_rows(x.detach(), x.shape[1])
     with _lib.on_device(x):
-        rows, cols, _ = H.fp8_quantize(x, block_rows, not transpose, transpose)
-    (r, c), buf = (x.shape, rows) if not transpose else ((x.shape[1], x.shape[0]), cols)
+        buf = H.fp8_quantize(x, block_rows, transpose)
+    r, c = (x.shape[1], x.shape[0]) if transpose else x.shape
     nc = H.fp8_bytes(r, c, block_rows)[0]
     return Fp8Blocks(buf.data[:nc].view(torch.float8_e4m3fn).view(-(-c // 128) * 2, r, 64),
                      buf.data[nc:].view(-(-c // 512), -(-r // block_rows), 4), r, c, block_rows)
@@ -587,49 +587,37 @@ class LinearFp8Function(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, relu, weight_q):
-        need_x, need_w = ctx.needs_input_grad[:2]
         rows = H.dense_rows(x, x.shape[-1])
         m, k = rows.shape
         n = weight.shape[0] if weight is not None else weight_q.rows
-        b32 = _f32(bias)
-        xt = wt = None
-        with _lib.on_device(x):
-            wq = None if weight_q is None else _Fp8Operand(weight_q)
-            if wq is None or need_x:
-                made, wt, _ = H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128, wq is None, need_x)
-                wq = made if wq is None else wq
-            if need_w and m > 0:
-                xq, xt, _ = H.fp8_quantize(rows, 1, True, True)
-                y = H.fp8_matmul(xq, 1, wq, 128, m, n, k, b32, None, relu, x.dtype, x.device)
-            else:
-                y = H.fp8_linear(rows, wq, 128, n, b32, relu, x.dtype)
+        y, saved, plan = x.new_empty(0, n), None, None
+        if m > 0:
+            w = None if weight is None else H.dense_rows(weight if weight.dim() == 2 else weight.flatten(1), k)
+            with _lib.on_device(x):
+                y, saved, plan = H.fp8_layer_fwd(rows, w, None if weight_q is None else _Fp8Operand(weight_q), n, _f32(bias), relu,
+                                                 *ctx.needs_input_grad[:3])
         if x.dim() != 2:                         # (no view of y: an output that is one cannot be changed in place)
             y = torch.ops.aten._unsafe_view(y, x.shape[:-1] + (n,))
-        ctx.save_for_backward(None if xt is None else xt.data, None if wt is None else wt.data, y if relu else None)
-        ctx.cfg = (None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, k, x.shape[:-1])
+        ctx.save_for_backward(saved, y if relu else None)
+        ctx.cfg = (plan, None if weight is None else (weight.shape, weight.dtype), None if bias is None else bias.dtype, x.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        xt, wt, y = ctx.saved_tensors
-        wmeta, bdt, k, shape = ctx.cfg
+        saved, y = ctx.saved_tensors
+        plan, wmeta, bdt, shape = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dy = H.dense_rows(dy, dy.shape[-1])
-        m, n = dy.shape
-        dx = dw = db = None
+        dx = torch.empty(shape, dtype=dy.dtype, device=dy.device) if need_x else None
+        if plan is None:                         # no rows
+            return (dx, torch.zeros(wmeta[0], dtype=wmeta[1], device=dy.device) if need_w else None,
+                    torch.zeros(dy.shape[-1], dtype=bdt, device=dy.device) if need_b else None, None, None)
+        dw = torch.empty(wmeta[0], dtype=torch.float32, device=dy.device) if need_w else None
+        db = torch.empty(dy.shape[-1], dtype=torch.float32, device=dy.device) if need_b else None
         with _lib.on_device(dy):
-            if m == 0:
-                dw = torch.zeros(wmeta[0], dtype=wmeta[1], device=dy.device) if need_w else None
-                db = torch.zeros(n, dtype=bdt, device=dy.device) if need_b else None
-                return dy.new_empty(shape + (k,)) if need_x else None, dw, db, None, None
-            g, gt, db = H.fp8_quantize(dy, 1, need_x, need_w, need_b, None if y is None else y.view(m, n))
-            if need_x:
-                dx = H.fp8_matmul(g, 1, H.Fp8Buffer(k, n, 128, data=wt), 128, m, k, n, None, None, False, dy.dtype, dy.device).view(shape + (k,))
-            if need_w:
-                dw = H.fp8_matmul(gt, 1, H.Fp8Buffer(k, m, 1, data=xt), 1, n, k, m, None, None, False, torch.float32, dy.device)
-                dw = dw.view(wmeta[0]) if wmeta[1] == torch.float32 else dw.view(wmeta[0]).to(wmeta[1])
-        return dx, dw, db if db is None or bdt == torch.float32 else db.to(bdt), None, None
+            H.fp8_layer_bwd(plan, H.dense_rows(dy, dy.shape[-1]), y, saved, dx, dw, db)
+        return (dx, dw if dw is None or wmeta[1] == torch.float32 else dw.to(wmeta[1]),
+                db if db is None or bdt == torch.float32 else db.to(bdt), None, None)
 
 
 def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
@@ -662,7 +650,7 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
         return LinearFp8Function.apply(x, weight, bias, relu, weight_q)
     rows = H.dense_rows(x, k)
     with _lib.on_device(x):
-        wq = _Fp8Operand(weight_q) if weight_q is not None else H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128)[0]
+        wq = _Fp8Operand(weight_q) if weight_q is not None else H.fp8_quantize(H.dense_rows(weight.flatten(1), k), 128)
         y = H.fp8_linear(rows, wq, 128, n, _f32(bias), relu, x.dtype)
     return y.view(x.shape[:-1] + (n,))
 

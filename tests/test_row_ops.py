@@ -196,6 +196,49 @@ def test_fp8_launch_limits():
     assert lib.sm_fp8_quantize(0, one, 1, cols, cols, 1, None, 0, one, one, None, None, one, one, 1 << 40, None) < 0
 
 
+def test_fp8_layer_bad_arguments():
+    lib = _lib.load()
+    one, odd = C.c_void_p(16), C.c_void_p(17)
+    out = [C.c_int64() for _ in range(3)]
+
+    def desc(**kw):
+        d = _lib.Fp8LayerDesc()
+        d.m, d.n, d.k, d.need_dx, d.need_dw, d.need_db, d.x_stride, d.dy_stride = 200, 96, 300, 1, 1, 1, 300, 96
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def size(**kw):
+        st = lib.sm_fp8_layer_bytes(C.byref(desc(**kw)), *map(C.byref, out))
+        return st or tuple(v.value for v in out)
+    full = size()
+    # codes of x^T (300 x 200) and w^T (300 x 96) with their scales, 256 bytes apart
+    assert full[0] == 300 * 256 + 1280 + 300 * 128 + 256
+    assert size(need_dx=0, need_dw=0)[0] == 0 and size(need_dx=0)[0] == 300 * 256 + 1280
+    assert size(have_wq=1)[1] < full[1] and size(need_dw=0, need_db=0)[2] < full[2]
+    for bad in (dict(m=0), dict(n=0), dict(k=0), dict(x_stride=299), dict(dy_stride=95), dict(m=1 << 31)):
+        assert size(**bad) == -1, bad
+    for bad in (dict(dtype=3), dict(w_dtype=-1)):
+        assert size(**bad) == -2, bad
+    assert lib.sm_fp8_layer_bytes(C.byref(desc()), None, C.byref(out[1]), C.byref(out[2])) == -2
+    assert lib.sm_fp8_layer_bytes(None, *map(C.byref, out)) == -2
+
+    def fwd(x=one, w=one, ld=300, wc=None, ws=None, y=one, saved=one, wsp=one, n=full[1], **kw):
+        return lib.sm_fp8_layer_fwd(C.byref(desc(**kw)), x, w, ld, wc, ws, None, y, saved, wsp, n, None)
+    for bad in (dict(x=None), dict(y=None), dict(saved=None), dict(saved=odd), dict(wsp=None), dict(w=None), dict(ld=299), dict(have_wq=1),
+                dict(have_wq=1, wc=one)):
+        assert fwd(**bad) == -2, bad
+    assert fwd(n=full[1] - 1) == -5
+
+    def bwd(dy=one, y=None, saved=one, dx=one, dw=one, db=one, wsp=one, n=full[2], **kw):
+        return lib.sm_fp8_layer_bwd(C.byref(desc(**kw)), dy, y, saved, dx, dw, db, wsp, n, None)
+    for bad in (dict(dy=None), dict(saved=None), dict(saved=odd), dict(dx=None), dict(dw=None), dict(db=None), dict(wsp=odd), dict(relu=1)):
+        assert bwd(**bad) == -2, bad
+    assert bwd(n=full[2] - 1) == -5
+    assert bwd(need_dx=0, need_dw=0, need_db=0, dx=None, dw=None, db=None, saved=None, wsp=None, n=0) == 0
+
+
+
 # ------------------------------------------------------------------------------------------------ Python entry points
 def test_cpu_tensors_are_refused():
     x, w = torch.randn(4, 8), torch.randn(8)
