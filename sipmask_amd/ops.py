@@ -453,16 +453,17 @@ class DropoutFunction(Function):
     @staticmethod
     def forward(ctx, x, residual, thr, seed, offset):
         off = H.dropout_offset(offset, x.device)
-        ctx.save_for_backward(off[1])
-        ctx.cfg = (thr, seed, off[0])
+        if off[1] is not None:
+            ctx.save_for_backward(off[1])        # (an offset that changed before the backward is an error)
+        ctx.cfg = (thr, seed, off[0], off[1] is not None)
         return _dropout_rows(x, residual, thr, seed, off)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        thr, seed, host = ctx.cfg
-        dev, = ctx.saved_tensors
-        return (_dropout_rows(dy, None, thr, seed, (host, dev)) if ctx.needs_input_grad[0] else None,
+        thr, seed, host, on_device = ctx.cfg
+        off = (host, ctx.saved_tensors[0] if on_device else None)
+        return (_dropout_rows(dy, None, thr, seed, off) if ctx.needs_input_grad[0] else None,
                 dy if ctx.needs_input_grad[1] else None, None, None, None)
 
 
