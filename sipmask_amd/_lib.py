@@ -4,7 +4,6 @@ The product path has NO fallback: if the shared library is missing or a call
 returns a non-zero status a RuntimeError is raised.  Build with
 ``python -c "import __graft_entry__ as g; g.build()"`` or ``make -C sipmask_amd/csrc``.
 """
-import contextlib
 import ctypes as C
 import os
 
@@ -274,12 +273,28 @@ def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_HERE_ALREADY = contextlib.nullcontext()
+class _HereAlready:
+    __slots__ = ()
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_HERE_ALREADY = _HereAlready()
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def here(t):
+    """`t`'s device is the current one"""
+    return t.get_device() == _get_device()
 
 
 def on_device(t):
     """context in which `t`'s device is the current one (launches, workspaces and stream_ptr() follow the current device)"""
-    if t.device.index == torch.cuda.current_device():
+    if here(t):
         return _HERE_ALREADY
     return torch.cuda.device(t.device)
 

@@ -1430,7 +1430,7 @@ def _p(t):
 def _stream(t):
     """the current stream of t's device, as the handle the C entry points take"""
     if _raw_stream is not None:                  # (a stream object per call costs 2 us of host time, 12 in autograd's thread)
-        return _raw_stream(t.device.index)
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -1515,18 +1515,26 @@ def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, s
     return d, bwd_need, stats
 
 
+# (autograd's thread runs Python several times slower than the caller's, whose caches hold it: what the backwards call is spelt out)
 def group_norm_act_bwd(d, need, x, dy, dy_stride, dx, gamma, beta, stats, dgamma, dbeta):
     """dx (contiguous rows) and dgamma / dbeta f32 [C] are written where given"""
     d.dy_stride = dy_stride
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _lib.check(_lib.load().sm_group_norm_act_bwd(C.byref(d), _p(x), _p(dy), _p(gamma), _p(beta), _p(stats), _p(dx), _p(dgamma), _p(dbeta),
-                                                 _p(ws), need, _stream(x)), "sm_group_norm_act_bwd")
+    st = _lib.load().sm_group_norm_act_bwd(d, x.data_ptr(), dy.data_ptr(), None if gamma is None else gamma.data_ptr(),
+                                           None if beta is None else beta.data_ptr(), stats.data_ptr(), None if dx is None else dx.data_ptr(),
+                                           None if dgamma is None else dgamma.data_ptr(), None if dbeta is None else dbeta.data_ptr(),
+                                           None if ws is None else ws.data_ptr(), need, _stream(x))
+    if st:
+        _lib.check(st, "sm_group_norm_act_bwd")
 
 
 def dropout_rows(x, residual, y, rows, cols, x_stride, res_stride, thr, seed, offset):
     """rows x cols values, rows x_stride / res_stride elements apart -> y, contiguous"""
-    _lib.check(_lib.load().sm_dropout(DTYPE_CODES[x.dtype], _p(x), _p(residual), _p(y), rows, cols, x_stride, res_stride, cols, thr,
-                                      int(seed) & _MASK64, offset[0], _p(offset[1]), _stream(x)), "sm_dropout")
+    off, dev = offset
+    st = _lib.load().sm_dropout(DTYPE_CODES[x.dtype], x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), rows, cols,
+                                x_stride, res_stride, cols, thr, int(seed) & _MASK64, off, None if dev is None else dev.data_ptr(), _stream(x))
+    if st:
+        _lib.check(st, "sm_dropout")
     return y
 
 
@@ -1625,6 +1633,10 @@ def fp8_layer_bwd(plan, dy, y, saved, dx, dw, db):
     """writes those of dx (dense rows), dw f32 and db f32 that the forward announced"""
     d = _lib.Fp8LayerDesc.from_buffer_copy(plan[0])
     d.dy_stride = row_stride(dy)
-    ws = torch.empty(plan[3], dtype=torch.uint8, device=dy.device) if plan[3] else None
-    _lib.check(_lib.load().sm_fp8_layer_bwd(C.byref(d), _p(dy), _p(y), _p(saved), _p(dx), _p(dw), _p(db), _p(ws), plan[3], _stream(dy)),
-               "sm_fp8_layer_bwd")
+    need = plan[3]
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device) if need else None
+    st = _lib.load().sm_fp8_layer_bwd(d, dy.data_ptr(), None if y is None else y.data_ptr(), None if saved is None else saved.data_ptr(),
+                                      None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                      None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(dy))
+    if st:
+        _lib.check(st, "sm_fp8_layer_bwd")

@@ -369,8 +369,9 @@ class GroupNormActFunction(Function):
             dy_stride = H.row_stride(dyr)
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
             # the row graph's parameters may live in all-reduce buckets
-            tg = H.GRAD_SINK.target(g32) if need_g else None
-            tb = H.GRAD_SINK.target(b32) if need_b else None
+            if H.GRAD_SINK.views:
+                tg = H.GRAD_SINK.target(g32) if need_g else None
+                tb = H.GRAD_SINK.target(b32) if need_b else None
         else:
             rows = _channels_last_rows(x)[0]
             dyr, dy_stride = _channels_last_rows(dy)
@@ -435,6 +436,8 @@ def _dropout_rows(x, residual, thr, seed, offset):
     if n == 0:
         return y
     if x.is_contiguous() and (residual is None or residual.is_contiguous()):
+        if _lib.here(x):
+            return H.dropout_rows(x, residual, y, 1, n, n, n, thr, seed, offset)
         rows, cols, ldx, ldr = 1, n, n, n
     else:
         cols = x.shape[-1] if x.dim() else 1
