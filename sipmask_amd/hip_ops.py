@@ -1481,6 +1481,7 @@ def dropout_offset(offset, device):
     return int(offset) & _MASK64, None
 
 
+# (sizes enter these caches through int(): while torch.jit.trace records, shapes hold tensors)
 @functools.lru_cache(maxsize=512)
 def _gn_act_plan(batch, hw, channels, groups, dtype, act, eps, thr):
     """(sm_gn_act_desc as bytes, forward and backward workspace) of a geometry; level l holds batch * hw[l] rows"""
@@ -1502,7 +1503,7 @@ def _gn_act_plan(batch, hw, channels, groups, dtype, act, eps, thr):
 def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, seed, offset, gamma, beta, want_stats):
     """x: channels-last values, rows x_stride elements apart; y: contiguous rows.  -> (descriptor, backward workspace bytes, stats f64
     [batch * nlev * groups, 2] or None)"""
-    plan, need, bwd_need = _gn_act_plan(batch, hw, channels, groups, dtype_code(x, "group_norm_act"), act, eps, thr)
+    plan, need, bwd_need = _gn_act_plan(int(batch), tuple(map(int, hw)), int(channels), int(groups), dtype_code(x, "group_norm_act"), act, eps, thr)
     d = _lib.GnActDesc.from_buffer_copy(plan)
     d.x_stride = x_stride
     if thr:
@@ -1580,7 +1581,7 @@ def _fp8_plan(m, n, k, a_block_rows, b_block_rows, out_dtype, relu):
 
 def fp8_matmul(a, a_block_rows, b, b_block_rows, m, n, k, bias, residual, relu, out_dtype, device):
     """a, b: codes / scales as Fp8Buffer (or anything with these two addresses)"""
-    plan, need, _ = _fp8_plan(m, n, k, a_block_rows, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
+    plan, need, _ = _fp8_plan(int(m), int(n), int(k), a_block_rows, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
     d = _lib.Fp8MatmulDesc.from_buffer_copy(plan)
     if residual is not None:
         d.res_stride = row_stride(residual)
@@ -1594,7 +1595,7 @@ def fp8_matmul(a, a_block_rows, b, b_block_rows, m, n, k, bias, residual, relu, 
 def fp8_linear(x, b, b_block_rows, n, bias, relu, out_dtype):
     """x [m, k] with dense rows, quantised on the way, times the codes b"""
     m, k = x.shape
-    plan, _, need = _fp8_plan(m, n, k, 1, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
+    plan, _, need = _fp8_plan(int(m), int(n), int(k), 1, b_block_rows, DTYPE_CODES[out_dtype], int(relu))
     y = torch.empty(m, n, dtype=out_dtype, device=x.device)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _lib.check(_lib.load().sm_fp8_linear(plan, dtype_code(x, "linear_fp8"), _p(x), row_stride(x), b.codes, b.scales, _p(bias), None, _p(y),
@@ -1617,7 +1618,7 @@ def _fp8_layer_plan(m, n, k, dtype, w_dtype, relu, need_dx, need_dw, need_db, ha
 def fp8_layer_fwd(x, w, wq, n, bias, relu, need_dx, need_dw, need_db):
     """x [m, k], w [n, k] (or None) with dense rows, wq: codes of w or None -> (y [m, n], what the backward needs, its plan)"""
     m, k = x.shape
-    plan = _fp8_layer_plan(m, n, k, DTYPE_CODES[x.dtype], 0 if w is None else DTYPE_CODES[w.dtype], int(relu), int(need_dx), int(need_dw),
+    plan = _fp8_layer_plan(int(m), int(n), int(k), DTYPE_CODES[x.dtype], 0 if w is None else DTYPE_CODES[w.dtype], int(relu), int(need_dx), int(need_dw),
                            int(need_db), int(wq is not None))
     d = _lib.Fp8LayerDesc.from_buffer_copy(plan[0])
     d.x_stride = row_stride(x)

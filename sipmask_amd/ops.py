@@ -19,7 +19,7 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 from torch.nn.modules.utils import _pair, _single
 
@@ -297,6 +297,11 @@ group_norm = GroupNormFunction.apply
 
 # ------------------------------------------------------------------------------- GroupNorm + activation, dropout
 def _wants_grad(*tensors):
+    """the call has to go through Function.apply: a gradient is wanted; or a forward-mode level is open (a dual tensor has requires_grad
+    False, and apply refuses it where a result filled through its address would have lost the tangent); or torch.jit.trace is recording
+    (it takes down the Function and calls it again; of a bare call it would only see the uninitialised result)"""
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing():
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

@@ -1,0 +1,150 @@
+"""How the residual-block operators are called by autograd and the tracer: forward mode, torch.jit.trace, saved-tensor hooks, activation
+checkpointing.  On the CPU the C entry points are replaced by stand-ins that note what they are given (and fill the result with something
+that depends on x), on the device they are the real ones."""
+import contextlib
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import row_ops_ref as R
+from sipmask_amd import _lib
+from sipmask_amd import hip_ops as H
+from sipmask_amd import ops as P
+from sipmask_amd import ops_rows as PR
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def floats(address, rows, cols, stride):
+    """f32 rows at an address as a numpy view"""
+    flat = np.ctypeslib.as_array((C.c_float * ((rows - 1) * stride + cols)).from_address(address))
+    return np.lib.stride_tricks.as_strided(flat, (rows, cols), (4 * stride, 4))
+
+
+class StandIn:
+    """the library with its launches on f32 rows replaced: y = 2 x (products: y[i][j] = x[i][0])"""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+    @staticmethod
+    def struct(d, cls):
+        return cls.from_buffer_copy(d if isinstance(d, (bytes, cls)) else d._obj)
+
+    def sm_group_norm_act(self, d, x, gamma, beta, y, stats, ws, need, stream):
+        d = self.struct(d, _lib.GnActDesc)
+        rows = d.batch * sum(d.hw[l] for l in range(d.nlev))
+        floats(y, rows, d.channels, d.y_stride)[...] = 2 * floats(x, rows, d.channels, d.x_stride)
+        self.calls.append(("gn", d, x))
+        return 0
+
+    def sm_group_norm_act_bwd(self, d, x, dy, gamma, beta, stats, dx, dgamma, dbeta, ws, need, stream):
+        self.calls.append(("gn_bwd", self.struct(d, _lib.GnActDesc), x))
+        return 0
+
+    def sm_dropout(self, dtype, x, res, y, rows, cols, ldx, ldr, ldy, *rest):
+        floats(y, rows, cols, ldy)[...] = 2 * floats(x, rows, cols, ldx)
+        self.calls.append(("dropout", rows, cols))
+        return 0
+
+    def _product(self, m, n, x, stride, y):
+        floats(y, m, n, n)[...] = floats(x, m, 1, stride)
+        return 0
+
+    def sm_fp8_quantize(self, *args):
+        return 0
+
+    def sm_fp8_linear(self, d, dtype, x, stride, *rest):
+        d = self.struct(d, _lib.Fp8MatmulDesc)
+        return self._product(d.m, d.n, x, stride, rest[4])
+
+    def sm_fp8_layer_fwd(self, d, x, w, ldw, wc, ws, bias, y, *rest):
+        d = self.struct(d, _lib.Fp8LayerDesc)
+        return self._product(d.m, d.n, x, d.x_stride, y)
+
+
+@pytest.fixture
+def standin(monkeypatch):
+    s = StandIn(_lib.load())
+    monkeypatch.setattr(_lib, "load", lambda: s)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "on_device", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "here", lambda t: True)
+    monkeypatch.setattr(H, "_stream", lambda t: 0)
+    return s
+
+
+def _cl(*shape, seed=0, dtype=F32, device="cpu"):
+    t = torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(device)
+    return t.movedim(-1, 1) if t.dim() == 4 else t
+
+
+LV = H.Levels(1, [(2, 3), (1, 2)])
+
+
+def _operators(device="cpu"):
+    """name -> (function of one tensor, shape of that tensor (channels last))"""
+    c = 16
+    w, b = 1 + 0.1 * _cl(c, seed=1, device=device), 0.1 * _cl(c, seed=2, device=device)
+    lw, lb = 0.3 * _cl(24, c, seed=3, device=device), 0.1 * _cl(24, seed=4, device=device)
+    return {
+        "group_norm_act": (lambda x: P.group_norm_act(x, w, b, 4, 1e-5, "silu", 0.25, 3, 5), (2, 3, 4, c)),
+        "gn_act_rows": (lambda x: PR.gn_act_rows(x, LV, w, b, 4, 1e-5, "gelu"), (LV.rows, c)),
+        "dropout": (lambda x: P.dropout(x, 0.5, 7, 1), (5, c)),
+        "dropout_residual": (lambda x: P.dropout(x, 0.5, 7, 1, residual=x), (5, c)),
+        "linear_fp8": (lambda x: P.linear_fp8(x, lw, lb, relu=True), (6, c)),
+        "linear_fp8_3d": (lambda x: P.linear_fp8(x, lw, lb), (2, 3, c)),
+    }
+
+
+NAMES = sorted(_operators())
+
+
+def _trace(f, x):
+    with torch.no_grad():
+        return torch.jit.trace(f, (x,), check_trace=False)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode and the tracer
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(standin, name):
+    f, shape = _operators()[name]
+    x = _cl(*shape)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward mode|jvp"):
+            f(d)
+        f(x)                                     # (a tensor without a tangent is none of its business)
+    assert torch.equal(f(x), f(x))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", NAMES)
+def test_a_traced_call_follows_its_input(standin, name):
+    f, shape = _operators()[name]
+    t = _trace(f, _cl(*shape, seed=10))
+    for seed in (11, 12):
+        x = _cl(*shape, seed=seed)
+        y = t(x)
+        assert y.shape == f(x).shape and torch.equal(y, f(x)) and float(y.abs().max()) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_and_trace_on_the_device(name):
+    f, shape = _operators("cuda")[name]
+    x = _cl(*shape, seed=10, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward mode|jvp"):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+    t = _trace(f, x)
+    for seed in (11, 12):
+        x = _cl(*shape, seed=seed, device="cuda")
+        assert torch.equal(t(x), f(x))
