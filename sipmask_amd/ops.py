@@ -532,11 +532,17 @@ class Fp8Blocks:
         return (self.code_matrix().to(torch.float64) * s).to(dtype)
 
 
+def _refuse_trace(what):
+    if torch.jit.is_tracing():                   # (the tracer sees neither the launch nor, in an Fp8Blocks, the tensors)
+        raise RuntimeError("%s: torch.jit.trace would record its result uninitialised; linear_fp8 can be traced (lay weight_q out before)" % what)
+
+
 def quantize_fp8(x, block_rows=1, transpose=False):
     """x [rows, cols] bf16 / f16 / f32 -> Fp8Blocks.  block_rows 1: a scale per row and 128 columns (activations, gradients);
     128: per 128 x 128 (weights).  transpose: the transposed matrix, blocks along the rows of x.  Inf and NaN are stored as NaN.
-    Not differentiable (linear_fp8 is)."""
+    Not differentiable (linear_fp8 is); refused while torch.jit.trace records."""
     _lib.require_cuda(x)
+    _refuse_trace("quantize_fp8")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("quantize_fp8: x is [rows, cols >= 1], got %s" % (tuple(x.shape),))
     H.dtype_code(x, "quantize_fp8")
@@ -567,7 +573,9 @@ class _Fp8Operand:
 
 def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloat16):
     """a [m, k] . b [n, k]^T (+ bias [n]) (+ residual [m, n] of out_dtype) (ReLU) of two Fp8Blocks: exact products, f32
-    accumulation, one rounding to out_dtype (bf16 / f16 / f32).  Not differentiable (linear_fp8 is)."""
+    accumulation, one rounding to out_dtype (bf16 / f16 / f32).  Not differentiable (linear_fp8 is); refused while torch.jit.trace
+    records."""
+    _refuse_trace("matmul_fp8")
     if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
         raise TypeError("matmul_fp8: operands come from quantize_fp8")
     _lib.require_cuda(a.codes, b.codes, bias, residual)

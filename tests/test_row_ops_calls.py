@@ -135,6 +135,19 @@ def test_a_traced_call_follows_its_input(standin, name):
         assert y.shape == f(x).shape and torch.equal(y, f(x)) and float(y.abs().max()) > 0
 
 
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_operators_on_codes_are_not_traced(standin):
+    """their results are filled behind the tracer's back and are no inputs of an autograd function"""
+    w = _cl(24, 16, seed=3)
+    wq = P.quantize_fp8(w, 128)
+    for f in (lambda x: P.matmul_fp8(P.quantize_fp8(x), wq), lambda x: P.quantize_fp8(x).dequantize(), lambda x: P.matmul_fp8(wq, wq) + x[0, 0]):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            _trace(f, _cl(6, 16))
+    t = _trace(lambda x: P.linear_fp8(x, None, weight_q=wq), _cl(6, 16))
+    x = _cl(6, 16, seed=1)
+    assert torch.equal(t(x), P.linear_fp8(x, None, weight_q=wq))
+
+
 @pytest.mark.gpu
 @pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("name", NAMES)
