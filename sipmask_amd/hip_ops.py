@@ -1517,6 +1517,13 @@ def group_norm_act(x, x_stride, y, batch, hw, channels, groups, eps, act, thr, s
 
 
 # (autograd's thread runs Python several times slower than the caller's, whose caches hold it: what the backwards call is spelt out)
+def group_norm_act_bwd_desc(d, x_stride, offset_dev):
+    """the forward's descriptor for a backward on these tensors: a copy, since a graph that is kept may be walked by two threads"""
+    d = _lib.GnActDesc.from_buffer_copy(d)
+    d.x_stride, d.drop_offset_dev = x_stride, None if offset_dev is None else offset_dev.data_ptr()
+    return d
+
+
 def group_norm_act_bwd(d, need, x, dy, dy_stride, dx, gamma, beta, stats, dgamma, dbeta):
     """dx (contiguous rows) and dgamma / dbeta f32 [C] are written where given"""
     d.dy_stride = dy_stride

@@ -365,20 +365,21 @@ class GroupNormActFunction(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, g32, b32, stats, _ = ctx.saved_tensors
+        # (saved-tensor hooks and checkpointing may hand back other tensors than the forward had: strides and addresses come from these)
+        x, g32, b32, stats, dev = ctx.saved_tensors
         (d, need), pyramid, gdt, bdt = ctx.cfg
         need_x, need_g, need_b = ctx.needs_input_grad[:3]
         dx = dg = db = tg = tb = None
         if pyramid:
             rows, dyr = H.dense_rows(x, x.shape[1]), H.dense_rows(dy, x.shape[1])
-            dy_stride = H.row_stride(dyr)
+            x_stride, dy_stride = H.row_stride(rows), H.row_stride(dyr)
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
             # the row graph's parameters may live in all-reduce buckets
             if H.GRAD_SINK.views:
                 tg = H.GRAD_SINK.target(g32) if need_g else None
                 tb = H.GRAD_SINK.target(b32) if need_b else None
         else:
-            rows = _channels_last_rows(x)[0]
+            rows, x_stride = _channels_last_rows(x)
             dyr, dy_stride = _channels_last_rows(dy)
             dx = _empty_channels_last(x) if need_x else None
         if need_g:
@@ -386,7 +387,7 @@ class GroupNormActFunction(Function):
         if need_b:
             db = tb if tb is not None else torch.empty(x.shape[1], dtype=torch.float32, device=x.device)
         with _lib.on_device(x):
-            H.group_norm_act_bwd(d, need, rows, dyr, dy_stride, dx, g32, b32, stats, dg, db)
+            H.group_norm_act_bwd(H.group_norm_act_bwd_desc(d, x_stride, dev), need, rows, dyr, dy_stride, dx, g32, b32, stats, dg, db)
         if tg is not None:
             H.GRAD_SINK.commit(g32)
             dg = None

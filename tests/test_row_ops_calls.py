@@ -7,6 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.autograd import forward_ad
 
 import row_ops_ref as R
@@ -161,3 +162,111 @@ def test_forward_mode_and_trace_on_the_device(name):
     for seed in (11, 12):
         x = _cl(*shape, seed=seed, device="cuda")
         assert torch.equal(t(x), f(x))
+
+
+# ------------------------------------------------------------------------------------------------ saved tensors that come back as others
+def _dense_copy(t):
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+@pytest.mark.parametrize("pyramid", [False, True])
+def test_backward_takes_strides_and_offset_from_the_saved_tensors(standin, pyramid):
+    """hooks that hand back dense copies: the backward steps x by the copy's stride and reads the copy of the offset, not the address that
+    the forward's (long freed) one had; the descriptor that the graph keeps stays the forward's"""
+    if pyramid:
+        x = _cl(LV.rows, 40)[:, 8:24].requires_grad_(True)
+        call = lambda off: PR.gn_act_rows(x, LV, None, None, 4, 1e-5, "relu", 0.5, 3, off)
+    else:
+        x = _cl(2, 3, 4, 40)[:, 8:24].requires_grad_(True)
+        call = lambda off: P.group_norm_act(x, None, None, 4, 1e-5, "relu", 0.5, 3, off)
+    copies = []
+
+    def unpack(t):
+        copies.append(_dense_copy(t))
+        return copies[-1]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = call(torch.tensor([7]) * 2 + 1)
+    (_, fwd, _), = standin.calls
+    assert fwd.x_stride == 40 and fwd.drop_offset_dev
+    for turn in range(2):
+        del standin.calls[:], copies[:]
+        torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+        (_, bwd, address), = standin.calls
+        off, = [t for t in copies if t.dtype == torch.int64]
+        dense, = [t for t in copies if t.shape == x.shape]
+        assert bwd.x_stride == 16 and bwd.drop_offset_dev == off.data_ptr() and int(off) == 15
+        if pyramid:
+            assert address == dense.data_ptr()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+        y = call(0)                              # nothing changed hands: as the forward had it, no offset
+    del standin.calls[:]
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    (_, bwd, address), = standin.calls
+    assert bwd.x_stride == 40 and not bwd.drop_offset_dev and address == x.data_ptr()
+
+
+def _gn_case(layout, dev):
+    """(x, function of x and an offset) of a slice of channels"""
+    w, b = (1 + 0.1 * _cl(16, seed=1, device=dev)).requires_grad_(True), (0.1 * _cl(16, seed=2, device=dev)).requires_grad_(True)
+    if layout == "rows":
+        lv = H.Levels(2, [(9, 13), (5, 7)])
+        x = _cl(lv.rows, 40, dtype=BF16, device=dev)[:, 8:24]
+        return x, w, b, lambda x, off: PR.gn_act_rows(x, lv, w, b, 4, 1e-5, "silu", 0.3, 5, off)
+    x = _cl(2, 33, 31, 40, dtype=BF16, device=dev)[:, 8:24]
+    return x, w, b, lambda x, off: P.group_norm_act(x, w, b, 4, 1e-5, "silu", 0.3, 5, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "nchw"])
+@pytest.mark.parametrize("how", ["cpu", "pinned", "checkpoint", "checkpoint_reentrant"])
+def test_group_norm_act_through_hooks_and_checkpoints(layout, how):
+    """saved tensors that were on the host in between, and an activation that is computed again, with an offset that lives only inside the
+    region: the gradients of the plain call, bit for bit (no atomics)"""
+    x, w, b, f = _gn_case(layout, "cuda")
+    base = torch.tensor([20], device="cuda")
+    layer = lambda x: f(x, base * 2 + 1)
+    plain = x.detach().requires_grad_(True)
+    y0 = layer(plain)
+    dy = torch.randn(y0.shape, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    want = torch.autograd.grad(y0, [plain, w, b], dy)
+    x = x.detach().requires_grad_(True)
+    assert x.stride() == plain.stride()
+    if how in ("cpu", "pinned"):
+        with torch.autograd.graph.save_on_cpu(pin_memory=how == "pinned"):
+            y = layer(x)
+    else:
+        y = torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=how == "checkpoint_reentrant")
+    junk = [torch.full((1,), 999, device="cuda") for _ in range(64)]     # (where the forward's offset was)
+    assert torch.equal(y, y0)
+    if how == "checkpoint_reentrant":
+        for t in (w, b):
+            t.grad = None
+        y.backward(dy)
+        got = (x.grad, w.grad, b.grad)
+    else:
+        got = torch.autograd.grad(y, [x, w, b], dy)
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
+    del junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["cpu", "checkpoint"])
+def test_dropout_and_linear_through_hooks_and_checkpoints(how):
+    w, b = (0.3 * _cl(24, 40, seed=3, device="cuda")).requires_grad_(True), (0.1 * _cl(24, seed=4, device="cuda")).requires_grad_(True)
+    x = _cl(70, 56, device="cuda")[:, 8:48].requires_grad_(True)
+    base = torch.tensor([20], device="cuda")
+    layer = lambda x: P.dropout(P.linear_fp8(x, w, b, relu=True), 0.3, 5, base * 2 + 1)
+    y0 = layer(x)
+    dy = _cl(70, 24, seed=6, device="cuda")
+    want = torch.autograd.grad(y0, [x, w, b], dy)
+    if how == "cpu":
+        with torch.autograd.graph.save_on_cpu():
+            y = layer(x)
+    else:
+        y = torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=False)
+    junk = [torch.full((1,), 999, device="cuda") for _ in range(64)]
+    assert torch.equal(y, y0)
+    for u, v in zip(torch.autograd.grad(y, [x, w, b], dy), want):
+        assert torch.equal(u, v)
+    del junk
