@@ -15,6 +15,8 @@ from sipmask_amd import _lib
 from sipmask_amd import hip_ops as H
 from sipmask_amd import ops as P
 from sipmask_amd import ops_rows as PR
+from sipmask_amd import sipmask_head  # noqa: F401
+from sipmask_amd.registry import build_head
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -248,6 +250,24 @@ def test_group_norm_act_through_hooks_and_checkpoints(layout, how):
     for u, v in zip(got, want):
         assert torch.equal(u, v)
     del junk
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_tower_dropout_is_not_computed_again(reentrant):
+    """the counter has moved on when a checkpoint calls the forward a second time: refused, not another mask"""
+    h = build_head(dict(type="SipMaskHead", num_classes=5, in_channels=64, feat_channels=64, stacked_convs=2, tower_dropout=0.25)).train()
+
+    def layer(x):
+        d = h._tower_drop()
+        return x.square() * R.keep_factor(x.shape, d["dropout_p"], d["seed"], d["offset"])
+    x = torch.randn(4, 8, dtype=torch.float64, requires_grad=True)
+    y = torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=reentrant)
+    assert h.tower_dropout_calls == 1
+    with pytest.raises(RuntimeError, match="checkpoint computes again"):
+        y.sum().backward()
+    assert h.tower_dropout_calls == 1
+    layer(x).sum().backward()                    # without one, and behind that: as ever
+    assert h.tower_dropout_calls == 2 and torch.equal(x.grad, 2 * x.detach() * R.keep_factor(x.shape, 0.25, 0, 2))
 
 
 @pytest.mark.gpu
