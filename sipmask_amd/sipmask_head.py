@@ -90,8 +90,8 @@ class SipMaskHead(nn.Module):
         """tower_dropout (this framework's own, off by default): probability with which each tower layer's output is dropped while
         training.  The masks are a function of (tower_dropout_seed, rank, number of the layer call since construction), so a run is
         repeatable; tower_dropout_calls is that number -- carry it over by hand to go on with fresh masks after a resume (it is no
-        entry of the state dict).  It is counted on the host, so such a step can neither be captured into a graph nor be computed again by
-        activation checkpointing (both raise).
+        entry of the state dict).  It is counted on the host, so such a step can neither be captured into a graph, traced, nor be computed
+        again by activation checkpointing (all three raise).
 
         mask_lat_fp8 (this framework's own, off by default): the training graph computes the mask branch's 1x1 convolution
         sip_mask_lat0 and its gradients with e4m3 operands (ops.linear_fp8); the inference plan does not change."""
@@ -177,7 +177,7 @@ class SipMaskHead(nn.Module):
         """dropout arguments of the next tower layer, {} when none is wanted"""
         if not (self.tower_dropout > 0 and self.training):
             return {}
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        if torch.jit.is_tracing() or (torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()):
             raise RuntimeError("tower_dropout takes its counter from the host: a replay of this graph would repeat its masks")
         if torch._C._current_graph_task_id() != -1:          # inside a backward pass: activation checkpointing computes the forward again
             raise RuntimeError("tower_dropout counts its calls: a forward that a checkpoint computes again would draw other masks")

@@ -270,6 +270,15 @@ def test_tower_dropout_is_not_computed_again(reentrant):
     assert h.tower_dropout_calls == 2 and torch.equal(x.grad, 2 * x.detach() * R.keep_factor(x.shape, 0.25, 0, 2))
 
 
+def test_tower_dropout_is_not_traced():
+    """the tracer would bake the counter in: every call of the traced function would repeat one mask"""
+    h = build_head(dict(type="SipMaskHead", num_classes=5, in_channels=64, feat_channels=64, stacked_convs=2, tower_dropout=0.25)).train()
+    with pytest.raises(RuntimeError, match="repeat its masks"):
+        _trace(lambda x: x * h._tower_drop()["offset"], torch.randn(4))
+    assert h.tower_dropout_calls == 0
+    assert torch.equal(_trace(lambda x: x * len(h.eval()._tower_drop()), torch.randn(4))(torch.ones(4)), torch.zeros(4))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("how", ["cpu", "checkpoint"])
 def test_dropout_and_linear_through_hooks_and_checkpoints(how):
