@@ -1481,10 +1481,17 @@ def dropout_offset(offset, device):
     return int(offset) & _MASK64, None
 
 
+def _int32(what, *sizes):
+    """sizes that go into 32-bit fields of a descriptor (ctypes would cut them off silently)"""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError("%s: sizes %s, at most 2^31 - 1" % (what, sizes))
+
+
 # (sizes enter these caches through int(): while torch.jit.trace records, shapes hold tensors)
 @functools.lru_cache(maxsize=512)
 def _gn_act_plan(batch, hw, channels, groups, dtype, act, eps, thr):
     """(sm_gn_act_desc as bytes, forward and backward workspace) of a geometry; level l holds batch * hw[l] rows"""
+    _int32("group_norm_act: images, channels", batch, channels)
     lib = _lib.load()
     d = _lib.GnActDesc()
     d.nlev, d.batch, d.channels, d.groups = len(hw), batch, channels, groups
@@ -1576,6 +1583,7 @@ def fp8_quantize(x, block_rows, transpose=False):
 @functools.lru_cache(maxsize=512)
 def _fp8_plan(m, n, k, a_block_rows, b_block_rows, out_dtype, relu):
     """(sm_fp8_matmul_desc as bytes, workspace of sm_fp8_matmul, of sm_fp8_linear)"""
+    _int32("fp8 product: columns, summed axis", n, k)
     lib = _lib.load()
     d = _lib.Fp8MatmulDesc()
     d.m, d.n, d.k, d.a_block_rows, d.b_block_rows = m, n, k, a_block_rows, b_block_rows
@@ -1613,6 +1621,7 @@ def fp8_linear(x, b, b_block_rows, n, bias, relu, out_dtype):
 @functools.lru_cache(maxsize=512)
 def _fp8_layer_plan(m, n, k, dtype, w_dtype, relu, need_dx, need_dw, need_db, have_wq):
     """(sm_fp8_layer_desc as bytes, bytes saved for the backward, of the forward's and the backward's workspace)"""
+    _int32("linear_fp8: outputs, inputs", n, k)
     d = _lib.Fp8LayerDesc()
     d.m, d.n, d.k, d.dtype, d.w_dtype, d.relu = m, n, k, dtype, w_dtype, relu
     d.need_dx, d.need_dw, d.need_db, d.have_wq = need_dx, need_dw, need_db, have_wq

@@ -299,3 +299,17 @@ def test_dropout_and_linear_through_hooks_and_checkpoints(how):
     for u, v in zip(torch.autograd.grad(y, [x, w, b], dy), want):
         assert torch.equal(u, v)
     del junk
+
+
+# ------------------------------------------------------------------------------------------------ sizes
+def test_sizes_beyond_the_descriptors_fields_are_refused():
+    """2^32 + 2 images are not 2: the descriptors hold 32 bits"""
+    big = (1 << 32) + 2
+    for call in (lambda: H._gn_act_plan(big, (1,), 8, 2, 0, 1, 1e-5, 0), lambda: H._gn_act_plan(1, (1,), big, 2, 0, 1, 1e-5, 0),
+                 lambda: H._fp8_plan(4, big, 16, 1, 128, 0, 0), lambda: H._fp8_plan(4, 8, big, 1, 128, 0, 0),
+                 lambda: H._fp8_layer_plan(4, big, 16, 0, 0, 0, 1, 1, 1, 0), lambda: H._fp8_layer_plan(4, 8, big, 0, 0, 0, 1, 1, 1, 0)):
+        with pytest.raises(ValueError, match="at most"):
+            call()
+    assert H._fp8_plan(4, 8, 16, 1, 128, 0, 0)[1:] == (0, 0)
+    with pytest.raises(RuntimeError):            # (rows are 64 bits wide; a layer's gradients sum over them)
+        H._fp8_layer_plan(big, 8, 16, 0, 0, 0, 1, 1, 1, 0)
