@@ -36,7 +36,7 @@ constexpr int GA_THREADS = 256;     // element-wise launches
 constexpr int GA_STAT = 1024;       // threads of the forward's reduction: few blocks with many waves, so that few partials are left
 constexpr int GA_STAT1 = 256;       // ... where a vector spans groups (16 sums a thread)
 constexpr int GA_SUM = 512;         // threads of the backward's reduction
-constexpr int GA_COMBINE = 2048;    // partials that an element-wise block has to add up (32 KB out of L2), see ga_plan
+constexpr int GA_COMBINE = 1024;    // partials that an element-wise block has to add up (16 KB out of L2), see ga_plan
 constexpr int GA_TILE = 32;         // column vectors per block: 512-byte row segments for 16-bit types
 constexpr int GA_TILE1 = 64;        // columns per block of the any-alignment path
 
@@ -725,7 +725,14 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, bool backward, GaPlan* p) {
   a.ntile = sm_cdiv(a.cols, a.ct);
   if (a.ntile > 65535 || a.G > 65535 * 32) return SM_ERR_UNSUPPORTED;
   const int tc = a.ct * vec;
-  p->gpt = std::min(std::min(a.G, (tc - 1) / a.cpg + 2), tc);
+  // Groups in a tile, and the partials of a row block that a tile has to add up: a group may lie in several tiles, one at a tile's end in two
+  int entries;
+  if (tc % a.cpg == 0) p->gpt = entries = tc / a.cpg;
+  else if (a.cpg % tc == 0) p->gpt = 1, entries = a.cpg / tc;
+  else {
+    p->gpt = std::min(std::min(a.G, (tc - 1) / a.cpg + 2), tc);
+    entries = a.cpg < tc ? p->gpt + 2 : p->gpt * std::min(a.ntile, (a.cpg - 1) / tc + 2);
+  }
   long long rows = 0, hw_max = 0;
   for (int l = 0; l < d->nlev; ++l) {
     if (d->hw[l] < 0 || d->row0[l] < 0) return SM_ERR_BAD_SHAPE;
@@ -734,12 +741,16 @@ int ga_plan(const sm_gn_act_desc* d, bool aligned, bool backward, GaPlan* p) {
   }
   // Element-wise: about 1024 blocks (all resident at once) of at least 4 rows per row lane.  Reductions: about 512 blocks of at least
   // 2 rows per row lane; every element-wise block adds up the partials of its (image, level), so a level has no more row blocks than
-  // fit into GA_COMBINE entries (89 600 x 256 rows of five levels forward: 37 us with 64 row blocks to a level, 41 with 96), twice as
-  // many where the chip would else be empty (one 100 x 168 map backward: 45 us with 64, 36 with 128).
+  // fit into GA_COMBINE entries: 32 for 256 channels in 32 groups (four 100 x 168 maps forward / backward: 31 / 47 us, with 64: 36 / 52),
+  // twice as many where the chip would else be empty (one such map: 20 / 34 us with 64, 22 / 33 with 128).  With many groups that would
+  // leave a large map to four row blocks: up to 32 there, as long as one has 1024 rows (in 256 groups, with four, doubled, and with this:
+  // 280 x 320 x 256 214 / 292 and 67 / 106 us, 136 x 136 43 / 82 and 30 / 52; of smaller maps the partials cost more than the rows: 25 x 42
+  // backward 23, with 16 row blocks 27).
   const long long total = rows * a.batch * a.ntile;
   long long arpb = std::max<long long>(4 * (GA_THREADS / a.ct), (total + 1023) / 1024);
-  const long long tiles_per_group = (a.cpg - 1) / tc + 2;
-  const long long smax = std::max<long long>(4, std::min<long long>(256, GA_COMBINE / (tiles_per_group * p->gpt)));
+  long long smin = 4;
+  while (smin < 32 && smin * 2048 <= hw_max) smin *= 2;
+  const long long smax = std::max<long long>(smin, std::min(256, GA_COMBINE / entries));
   const long long few = (hw_max + smax - 1) / smax, many = (hw_max + 2 * smax - 1) / (2 * smax);
   long long srpb = std::max(std::max<long long>(2 * ((backward ? GA_SUM : GA_STAT) / a.ct), (total + 511) / 512),
                             few > 0 && total / few < 256 ? many : few);

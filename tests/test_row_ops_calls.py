@@ -313,3 +313,33 @@ def test_sizes_beyond_the_descriptors_fields_are_refused():
     assert H._fp8_plan(4, 8, 16, 1, 128, 0, 0)[1:] == (0, 0)
     with pytest.raises(RuntimeError):            # (rows are 64 bits wide; a layer's gradients sum over them)
         H._fp8_layer_plan(big, 8, 16, 0, 0, 0, 1, 1, 1, 0)
+
+
+# ------------------------------------------------------------------------------------------------ groups and column tiles of every relation
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("shape", [(1, 256, 256, 130, 127),      # one channel a group, more row blocks than the partials alone would allow
+                                   (1, 768, 256, 40, 33),        # groups of three channels that lie in two tiles
+                                   (2, 264, 88, 50, 31),         # ... in tiles of 17 vectors
+                                   (1, 1024, 2, 41, 37),         # a group of two whole tiles
+                                   (1, 640, 2, 60, 23),          # ... of one and a half
+                                   (1, 130, 26, 97, 30),         # five channels, any alignment
+                                   (3, 96, 96, 70, 61)])
+def test_group_norm_act_groups_and_tiles(shape, dtype):
+    n, c, g, h, w = shape
+    x = (_cl(n, h, w, c, seed=1, device="cuda") * 1.5 + torch.linspace(-1, 1, c, device="cuda").view(1, c, 1, 1)).to(dtype)
+    x = x.contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    ga, be = (1 + 0.3 * _cl(c, seed=5, device="cuda")).requires_grad_(True), (0.3 * _cl(c, seed=6, device="cuda")).requires_grad_(True)
+    dy = _cl(n, h, w, c, seed=7, dtype=dtype, device="cuda")
+    y = P.group_norm_act(x, ga, be, g, 1e-5, "silu")
+    got = torch.autograd.grad(y, [x, ga, be], dy)
+    rows = lambda t: t.detach().movedim(1, -1).reshape(-1, c)
+    ref = R.GroupNormAct(rows(x), n, g, ga.detach(), be.detach(), 1e-5, "silu")
+    ref.backward(rows(dy))
+    # a block of at most h w / 4 rows has 512 / 64 threads or more to a column: their rows, then the tree over the threads
+    bounds = ref.bounds(dtype, run=h * w // 32 + 10)
+    for name, u, want, bound in [("y", rows(y), ref.y, ref.y_bound(dtype)), ("dx", rows(got[0]), ref.dx, bounds[0]),
+                                 ("dgamma", got[1], ref.dgamma, bounds[1]), ("dbeta", got[2], ref.dbeta, bounds[2])]:
+        assert bool(((u.double() - want).abs() <= bound).all()), name
+    again = torch.autograd.grad(P.group_norm_act(x, ga, be, g, 1e-5, "silu"), [x, ga, be], dy)
+    assert all(torch.equal(u, v) for u, v in zip(got, again))
