@@ -810,7 +810,8 @@ int sm_dropout(int dtype, const void* x, const void* residual, void* y, int64_t 
  * column; scales (E8M0: 2^(byte - 127)) uint8 [ceil(cols / 512)][ceil(rows / block_rows)][4], 4-byte aligned: the byte of K block kb and
  * row block r is [kb / 4][r][kb % 4], 127 behind the last block.  scale = smallest power of two >= 2^-127 with max |x| / scale <= 448
  * over the block of block_rows x 128 (1 for a block of zeros), code = x / scale rounded to nearest even; Inf and NaN become the NaN
- * code and leave the block's scale alone. */
+ * code and leave the block's scale alone.  The products take code * scale as bf16: exact for scale bytes >= 3, multiples of 2^-133 below;
+ * |x| > 248 * 2^120 (code 256 at 2^120) counts as Inf. */
 int64_t sm_fp8_codes_bytes(int64_t rows, int64_t cols);
 int64_t sm_fp8_scales_bytes(int64_t rows, int64_t cols, int block_rows);
 /* x [rows][cols] (row stride x_stride) -> any of: q / scale, its codes; q_t / scale_t, the codes of the transpose (cols x rows, blocks

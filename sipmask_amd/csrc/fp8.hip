@@ -7,12 +7,13 @@
 // range that a power of two gives away, and the scale enters the product for nothing: v_cvt_scalef32_pk_bf16_fp8 multiplies by it while
 // it widens two codes.
 //
-// Why bf16 MFMAs and not the 8-bit ones: a code times a power of two is exact in bf16, and v_mfma_f32_32x32x16_bf16 adds the exact
-// products in f32.  The 8-bit MFMAs (plain and block-scaled) align the products of an instruction to the largest one and drop what
-// lies 2^-14 below it (measured with one large and one small product; sums of 64 products over 8 binades were off by 2^-12 of the
-// largest): less than f32 sums.  The price is the matrix peak, 2.5 instead of 5 PFLOP/s; the widening itself hides behind the MFMAs
-// (one conversion is 8 cycles; 16 of them beside 4 MFMAs measured 161 cycles against 154 for the MFMAs alone), and the bytes moved
-// through HBM and LDS stay 8-bit.
+// Why bf16 MFMAs and not the 8-bit ones: a code times its scale is exact in bf16 (for scale bytes from 3 on; below, it is rounded to a
+// multiple of 2^-133, bf16's smallest subnormal; a block maximum above 248 * 2^120 has the code 256 at 2^120, which is Inf in bf16 and in
+// f32), and v_mfma_f32_32x32x16_bf16 adds the exact products in f32.  The 8-bit MFMAs (plain and block-scaled) align the products of an
+// instruction to the largest one and drop what lies 2^-14 below it (measured with one large and one small product; sums of 64 products
+// over 8 binades were off by 2^-12 of the largest): less than f32 sums.  The price is the matrix peak, 2.5 instead of 5 PFLOP/s; the
+// widening itself hides behind the MFMAs (one conversion is 8 cycles; 16 of them beside 4 MFMAs measured 161 cycles against 154 for the
+// MFMAs alone), and the bytes moved through HBM and LDS stay 8-bit.
 //
 // Layout of a quantised matrix: codes [K / 64][row][64] (two slabs per block of 128, zero codes behind the last column), scales
 // [K block / 4][row block][4] (127, i.e. 1, behind the last block).  One K step of a tile is then one contiguous piece of memory, and
@@ -397,7 +398,7 @@ __device__ __forceinline__ float fp8_scale_float(uint32_t w) {
   const uint32_t u = (w & 0xffu) << 23;
   return __uint_as_float(u == 0u ? 0x00400000u : u);
 }
-// 8 codes (two dwords) times a power of two as bf16: exact
+// 8 codes (two dwords) times a power of two as bf16: exact within the range stated at the top
 __device__ __forceinline__ bf16x8 fp8_widen8(int lo, int hi, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
   const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);

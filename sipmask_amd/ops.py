@@ -573,9 +573,9 @@ class _Fp8Operand:
 
 
 def matmul_fp8(a, b, bias=None, relu=False, residual=None, out_dtype=torch.bfloat16):
-    """a [m, k] . b [n, k]^T (+ bias [n]) (+ residual [m, n] of out_dtype) (ReLU) of two Fp8Blocks: exact products, f32
-    accumulation, one rounding to out_dtype (bf16 / f16 / f32).  Not differentiable (linear_fp8 is); refused while torch.jit.trace
-    records."""
+    """a [m, k] . b [n, k]^T (+ bias [n]) (+ residual [m, n] of out_dtype) (ReLU) of two Fp8Blocks: exact products (blocks with a
+    scale below 2^-124 are first rounded to multiples of 2^-133, and a value that was quantised to 2^128 is Inf), f32 accumulation, one
+    rounding to out_dtype (bf16 / f16 / f32).  Not differentiable (linear_fp8 is); refused while torch.jit.trace records."""
     _refuse_trace("matmul_fp8")
     if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
         raise TypeError("matmul_fp8: operands come from quantize_fp8")
@@ -642,7 +642,7 @@ def linear_fp8(x, weight, bias=None, relu=False, weight_q=None):
     """x [..., k] . weight [n, k]^T (+ bias) (ReLU) with both operands quantised to e4m3 blocks (1 x 128 for x, 128 x 128 for the
     weight), f32 accumulation, result of x's type (bf16 / f16 / f32): the 8-bit form of a 1x1 conv_rows; a [n, k, 1, 1] conv weight is
     taken as it is.  Differentiable in x, weight and bias: the gradients' products are 8-bit as well (dy in 1 x 128 blocks along the
-    axis each product sums over), dbias is exact.
+    axis each product sums over), dbias the column sums of dy as it came (f32 over 128 rows, joined in f64).
 
     Serving: weight_q = quantize_fp8(weight, block_rows=128), laid out once, with weight=None when x needs no gradient."""
     _lib.require_cuda(x, weight, bias)
