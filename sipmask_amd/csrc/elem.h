@@ -81,14 +81,16 @@ struct RowVec<DT, 1> {
   static __device__ __forceinline__ void store(T* p, const float* f) { E::store(p, f[0]); }
 };
 
-// sigmoid(t) = 1 / (1 + 2^(-t log2 e)) on the hardware exp2 and reciprocal (1 ulp each): relative error (|t| + 3) 2^-24, i.e. below
-// 2^-24 of t sigmoid(t)'s slope everywhere; the library expf and an IEEE division made SiLU 1.7 times as long as the copy it rides on
+// sigmoid(t) = 1 / (1 + 2^(-t log2 e)) on the hardware exp2 and reciprocal (1 ulp each).  Absolute errors: t sigmoid(t) is off by at most
+// (0.7 + 6 |t sigmoid(t)|) 2^-24 (the exponent's rounding is 1.3 |t| 2^-24 of e^-t), its derivative by (5 + 2 t) 2^-24 up to t = 17 (from
+// 1 - sigmoid(t)), 5 * 2^-24 for t < 0; relative to the derivative that is not small near its zero at t = -1.278.  The library expf and an
+// IEEE division made SiLU 1.7 times as long as the copy it rides on.
 __device__ __forceinline__ float fast_sigmoid(float t) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t * -1.4426950408889634f));
 }
 
 // q = Phi(-|t|) and e = exp(-t^2 / 2) of a standard normal t.  erfc(z) = exp(-z^2) s P(s) with s = 1 / (1 + 0.4 z): P is a degree-8
-// least-squares fit (reweighted to equal ripple) of erfcx(z) / s over 0 <= z <= 10, relative error 6.2e-8, so that the tail keeps its
+// least-squares fit (reweighted to equal ripple) of erfcx(z) / s over 0 <= z <= 10, relative error 6.8e-8, so that the tail keeps its
 // relative precision (1 + erf(u) cancels there) and the exponential is shared with the density.  The library erfcf took 2 x the time of
 // the copy a GELU rides on.
 __device__ __forceinline__ void normal_tail(float t, float& q, float& e) {
