@@ -12,7 +12,7 @@
 // does not depend on which block came first, and there is nothing to clear between the replays of a captured graph.
 //
 // Maps of a few hundred rows take one launch instead (ga_small_*): a block holds all rows of its columns in registers, reads x (and dy)
-// once and needs no partials -- there the launches, not the bytes, are the time.
+// once and needs no partials -- there the launches, not the bytes, are the time.  Of many such maps a block takes several (ga_many_*).
 //
 // Measured (a copy of 2 GiB runs at 4.9 TB/s here):
 //   89 600 x 256 bf16 rows of five levels, ReLU, p = 0.1: forward 40 us (sums 15, apply 26), backward 65 (sums 34, apply 32); without
