@@ -26,7 +26,7 @@ def check(named):
 
 # images, channels, groups, map: one block a map, several maps a block, tiles with idle columns, groups of a whole tile of 32 columns
 SHAPES = [(300, 64, 8, (7, 7)), (9001, 64, 8, (1, 1)), (70, 256, 32, (14, 14)), (1100, 256, 32, (2, 2)), (150, 72, 9, (5, 3)),
-          (130, 512, 2, (3, 3)), (17, 1024, 4, (9, 7)), (400, 24, 1, (8, 8)), (66, 320, 10, (4, 4))]
+          (130, 512, 2, (3, 3)), (70, 1024, 4, (8, 7)), (200, 256, 2, (6, 6)), (400, 24, 1, (8, 8)), (66, 320, 10, (4, 4))]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
