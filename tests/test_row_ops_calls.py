@@ -127,6 +127,17 @@ def test_forward_mode_is_refused(standin, name):
     assert torch.equal(f(x), f(x))
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_function_transforms_are_refused(standin, name):
+    """torch.func: no rule of these operators, so an error and no result"""
+    f, shape = _operators()[name]
+    x = _cl(*shape)
+    for call in (lambda: torch.func.jvp(f, (x,), (torch.ones_like(x),)), lambda: torch.func.jacfwd(f)(x), lambda: torch.func.vmap(f)(x[None])):
+        with pytest.raises(RuntimeError):
+            call()
+    assert not standin.calls
+
+
 @pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("name", NAMES)
 def test_a_traced_call_follows_its_input(standin, name):
